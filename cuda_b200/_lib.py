@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libcuda_llm_b200.so")
 OK, EINVAL, EALIGN, EWORKSPACE, ECUDA, EDEVICE = 0, -1, -2, -3, -4, -5
 ST_BAD_BLOCK, ST_BAD_CTX, ST_TIMEOUT, ST_BAD_QLEN, ST_SCALE_RANGE, ST_INCOMPLETE, ST_BAD_POSITION = 1, 2, 4, 8, 16, 32, 64
 F32, F16, BF16 = 0, 1, 2
-KV_FP8_E4M3, KV_FP4_E2M1, KV_INT8, KV_F16, KV_BF16 = 0, 1, 2, 3, 4
+KV_FP8_E4M3, KV_FP4_E2M1, KV_INT8, KV_F16, KV_BF16, KV_F32 = 0, 1, 2, 3, 4, 5
 SCALE_PER_HEAD, SCALE_PER_BLOCK, SCALE_PER_TOKEN, SCALE_MX_E8M0 = 0, 1, 2, 3
 FLAG_SKIP_MERGE = 1
 FLAG_STABLE_METADATA = 64   # lengths / offsets / block tables are not written by the kernel in front of the call
@@ -43,6 +43,43 @@ class KvCacheTarget(C.Structure):
         ("key_cache", C.c_void_p), ("value_cache", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
         ("slot_block", C.c_void_p), ("slot_offset", C.c_void_p), ("status", C.c_void_p),
         ("page_size", C.c_int32), ("num_blocks", C.c_int32), ("v_format", C.c_int32), ("scale_mode", C.c_int32),
+    ]
+
+
+class CrossAttentionParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("kv_lens", C.c_void_p),
+        ("q_strides", C.c_int64 * 3), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3), ("out_strides", C.c_int64 * 3),
+        ("batch_size", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("q_len", C.c_int32),
+        ("kv_len", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("softmax_scale", C.c_float),
+    ]
+
+
+class KvWeightsParams(C.Structure):
+    _fields_ = [
+        ("query", C.c_void_p), ("key_cache", C.c_void_p), ("k_scale", C.c_void_p), ("block_tables", C.c_void_p),
+        ("context_lens", C.c_void_p), ("cu_q_lens", C.c_void_p), ("lse", C.c_void_p), ("scores", C.c_void_p), ("status", C.c_void_p),
+        ("score_strides", C.c_int64 * 2),
+        ("num_seqs", C.c_int32), ("total_q", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_blocks_per_seq", C.c_int32), ("num_blocks", C.c_int32),
+        ("max_tokens", C.c_int32), ("max_q_len", C.c_int32), ("q_dtype", C.c_int32), ("k_format", C.c_int32),
+        ("scale_mode", C.c_int32), ("is_causal", C.c_int32), ("softmax_scale", C.c_float), ("decay", C.c_float),
+    ]
+
+
+EVICT_MAX_TOKENS = 786432
+
+
+class KvEvictParams(C.Structure):
+    _fields_ = [
+        ("scores", C.c_void_p), ("new_scores", C.c_void_p), ("key_cache", C.c_void_p), ("value_cache", C.c_void_p),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("block_tables", C.c_void_p), ("new_block_tables", C.c_void_p),
+        ("context_lens", C.c_void_p), ("new_context_lens", C.c_void_p), ("kept", C.c_void_p), ("status", C.c_void_p),
+        ("score_strides", C.c_int64 * 2), ("new_score_strides", C.c_int64 * 2),
+        ("num_seqs", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+        ("max_blocks_per_seq", C.c_int32), ("new_max_blocks_per_seq", C.c_int32), ("num_blocks", C.c_int32),
+        ("max_tokens", C.c_int32), ("k_format", C.c_int32), ("v_format", C.c_int32), ("scale_mode", C.c_int32),
+        ("budget", C.c_int32), ("sink", C.c_int32), ("recent", C.c_int32),
     ]
 
 
@@ -76,6 +113,10 @@ SYMBOLS = {
     "cuda_llm_mx_attention_ws": (C.c_int, [C.c_void_p] * 7 + [C.c_int32] * 5 + [C.c_float, C.c_int32, C.c_int32, C.c_void_p,
                                                                                  C.c_size_t, C.c_void_p]),
     "cuda_llm_mx_attention_tcgen05_launches": (C.c_int, [C.POINTER(C.c_uint64)]),
+    "cuda_llm_cross_attention": (C.c_int, [C.POINTER(CrossAttentionParams), C.c_void_p]),
+    "cuda_llm_cross_attention_wait_timeouts": (C.c_int, [C.POINTER(C.c_uint32)]),
+    "cuda_llm_kv_accumulate_weights": (C.c_int, [C.POINTER(KvWeightsParams), C.c_void_p]),
+    "cuda_llm_kv_evict": (C.c_int, [C.POINTER(KvEvictParams), C.c_void_p]),
     "cuda_llm_dequant_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                          C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                          C.c_void_p]),

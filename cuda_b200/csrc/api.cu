@@ -102,6 +102,9 @@ static int check_device() {
   return CUDA_LLM_OK;
 }
 
+int check_current_device() { return check_device(); }
+int current_sm_count() { return sm_count_cached(); }
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point look-up (libcuda is not linked).
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

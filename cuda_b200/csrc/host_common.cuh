@@ -1,0 +1,32 @@
+// Host-side helpers shared by the entry points that live beside their kernels (defined in api.cu).
+#pragma once
+#include <cstdio>
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "cuda_llm_b200.h"
+
+namespace b200 {
+
+void set_error_message(const char* msg);
+int check_current_device();  // CUDA_LLM_OK on an sm_100 device
+int current_sm_count();
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn tensor_map_encoder();
+
+inline int refuse(int code, const char* msg) {
+  set_error_message(msg);
+  return code;
+}
+inline int cuda_result(cudaError_t e, const char* where) {
+  if (e == cudaSuccess) return CUDA_LLM_OK;
+  char msg[192];
+  snprintf(msg, sizeof(msg), "%s: %s", where, cudaGetErrorString(e));
+  set_error_message(msg);
+  return CUDA_LLM_ECUDA;
+}
+
+}  // namespace b200

@@ -457,6 +457,210 @@ def kv_cache_append(k_new, v_new, slot_block, slot_offset, key_cache, value_cach
                                             _stream_ptr(k_new.device)), "cuda_llm_kv_append")
 
 
+def _addressable(t: torch.Tensor) -> torch.Tensor:
+    """``t`` if the kernels can address it as it lies (contiguous head_dim, 16-byte steps), else a copy."""
+    step = 16 // t.element_size()
+    fine = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        n == 1 or (st >= 0 and st % step == 0) for n, st in zip(t.shape[:-1], t.stride()[:-1]))
+    return t if fine else t.clone(memory_format=torch.contiguous_format)
+
+
+def cross_attention_forward(q, k, v, kv_lens=None, softmax_scale=None, *, return_lse=False):
+    """Attention of a decoder's positions to an encoder's states, no causal mask: q ``[B, Hq, Sq, D]``, k / v
+    ``[B, Hkv, Skv, D]`` of one dtype -> ``[B, Hq, Sq, D]`` (GQA: kv_head = q_head // (Hq // Hkv)).  ``kv_lens`` (int32
+    ``[B]``): how many states each sequence has; what lies behind them is not looked at.  A sequence without states
+    gives zeros.  ``return_lse`` adds the natural log-sum-exp ``[B, Hq, Sq]`` (-inf without states).  Strided views
+    (``[B, S, H, D].transpose(1, 2)``, expanded batch rows) are read as they lie, and the output has q's layout.  No
+    counterpart in the reference, whose attention calls take one sequence length."""
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise RuntimeError("Inputs must be on CUDA")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise RuntimeError("Inputs must be 4D [batch, heads, seq, dim]")
+    if k.shape != v.shape:
+        raise RuntimeError("K and V must have identical shapes")
+    b, hq, sq, d = q.shape
+    hkv, skv = k.shape[1], k.shape[2]
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise RuntimeError("num_q_heads must be divisible by num_kv_heads")
+    if d not in (64, 128):
+        raise RuntimeError("Only head_dim 64 and 128 supported")
+    if q.dtype not in _DTYPE:
+        raise RuntimeError("Unsupported scalar type for cross attention. Supported: Float32, Float16, BFloat16.")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape[0] != b or k.shape[3] != d:
+        raise RuntimeError("q, k and v must share dtype, batch and head_dim")
+    if k.device != q.device or v.device != q.device:
+        raise RuntimeError("Inputs must be on one device")
+    if kv_lens is not None and not (kv_lens.device == q.device and kv_lens.dtype == torch.int32 and kv_lens.shape == (b,)
+                                    and kv_lens.is_contiguous()):
+        raise RuntimeError("kv_lens must be a contiguous int32 tensor [batch] on the inputs' device")
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    lib = L.load()
+    with torch.cuda.device(q.device):
+        q, k, v = _addressable(q), _addressable(k), _addressable(v)
+        out = torch.empty_like(q)
+        lse = torch.empty(b, hq, sq, dtype=torch.float32, device=q.device) if return_lse else None
+        p = L.CrossAttentionParams(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=_ptr(lse), kv_lens=_ptr(kv_lens),
+            q_strides=q.stride()[:3], k_strides=k.stride()[:3], v_strides=v.stride()[:3], out_strides=out.stride()[:3],
+            batch_size=b, num_q_heads=hq, num_kv_heads=hkv, q_len=sq, kv_len=skv, head_dim=d, dtype=_DTYPE[q.dtype],
+            softmax_scale=scale)
+        L.check(lib.cuda_llm_cross_attention(C.byref(p), _stream_ptr(q.device)), "cuda_llm_cross_attention")
+    return (out, lse) if return_lse else out
+
+
+def _cache_format(cache, kv_format, packed_head_dim=None) -> int:
+    """CudaLlmKvFormat of one cache tensor (``packed_head_dim``: two E2M1 codes per byte if the rows are half as many)."""
+    wide = {torch.float16: L.KV_F16, torch.bfloat16: L.KV_BF16, torch.float32: L.KV_F32}
+    if cache.dtype in wide:
+        return wide[cache.dtype]
+    fmt = _byte_cache_format(cache, cache, kv_format)
+    return L.KV_FP4_E2M1 if packed_head_dim is not None and cache.shape[2] * 2 == packed_head_dim else fmt
+
+
+def _check_int32(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and not (t.device == device and t.dtype == torch.int32 and t.is_contiguous()):
+            raise RuntimeError(f"{name} must be a contiguous int32 tensor on the cache's device")
+
+
+def _check_scores(name, t, device, num_seqs, hkv):
+    if not (t.device == device and t.dtype == torch.float32 and t.dim() == 3 and t.shape[0] == num_seqs and t.shape[1] == hkv
+            and (t.stride(2) == 1 or t.shape[2] <= 1)):
+        raise RuntimeError(f"{name} must be float32 [num_seqs, num_kv_heads, tokens] with contiguous rows on the cache's device")
+
+
+def kv_cache_accumulate_weights(query, key_cache, k_scale, block_tables, context_lens, lse, scores, softmax_scale=None, *,
+                                cu_q_lens: Optional[torch.Tensor] = None, max_q_len: int = 1, is_causal: bool = True,
+                                decay: float = 1.0, kv_format: Optional[str] = None, status: Optional[torch.Tensor] = None):
+    """Add to ``scores`` (fp32 ``[num_seqs, Hkv, tokens]``, in place, returned) the attention weight that ``query`` ``[total_q,
+    Hq, D]`` spends on every cached token: ``decay * old + sum exp(scale * q . k_t - lse)`` over the queries that see the
+    token and the heads that share its KV head.  ``lse`` ``[total_q, Hq]`` is what the decode of the same queries returned
+    (``return_lse=True``).  The tokens the queries brought themselves (the last q_len) start from 0; ``decay=0`` reads no old
+    score.  ``is_causal=False``: every query sees every token (encoder states in a paged cache).  ``key_cache`` and
+    ``k_scale`` as in ``fp8_paged_attention_forward``, or a 16-bit cache of the query's type with ``k_scale=None``.
+    ``status``: int32 tensor into which run-time findings (``ST_*`` bits) are OR-ed.  No counterpart in the reference."""
+    if not (query.is_cuda and key_cache.is_cuda):
+        raise RuntimeError("Inputs must be on CUDA")
+    if query.dim() != 3:
+        raise RuntimeError("Query must be 3D [num_seqs, num_heads, head_dim]")
+    if key_cache.dim() != 4:
+        raise RuntimeError("KV caches must be 4D [num_blocks, num_heads, head_dim, page_size]")
+    if query.dtype not in _DTYPE:
+        raise RuntimeError("Unsupported query scalar type. Supported: Float32, Float16, BFloat16.")
+    total_q, hq, d = query.shape
+    nb, hkv, dk, page = key_cache.shape
+    dev = key_cache.device
+    if d not in (64, 128) or dk != d:
+        raise RuntimeError("Only head_dim 64 and 128 supported")
+    if hkv == 0 or hq % hkv:
+        raise RuntimeError("num_heads must be a multiple of the cache's num_kv_heads")
+    k_format = _cache_format(key_cache, kv_format)
+    if k_format == L.KV_F32:
+        raise RuntimeError("the key cache must be 8-bit, float16 or bfloat16")
+    mode = 0
+    if k_format == L.KV_FP8_E4M3:
+        if k_scale is None:
+            raise RuntimeError("an 8-bit cache needs k_scale")
+        mode = _scale_mode(k_scale)
+        k_scale = (k_scale if mode == L.SCALE_MX_E8M0 else k_scale.to(torch.float32)).contiguous()
+        want = {L.SCALE_PER_HEAD: (hkv,), L.SCALE_PER_BLOCK: (nb, hkv), L.SCALE_PER_TOKEN: (nb, hkv, page),
+                L.SCALE_MX_E8M0: (nb, hkv, d // 32, page)}[mode]
+        if tuple(k_scale.shape) != want or k_scale.device != dev:
+            raise RuntimeError(f"k_scale must be {list(want)} on the cache's device")
+    elif k_scale is not None:
+        raise RuntimeError("a 16-bit cache takes no scales")
+    num_seqs = context_lens.shape[0]
+    _check_int32(dev, block_tables=block_tables, context_lens=context_lens, cu_q_lens=cu_q_lens, status=status)
+    if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs or context_lens.dim() != 1:
+        raise RuntimeError("block_tables must be [num_seqs, max_blocks] and context_lens [num_seqs]")
+    if cu_q_lens is not None and cu_q_lens.shape != (num_seqs + 1,):
+        raise RuntimeError("cu_q_lens must be [num_seqs + 1]")
+    if cu_q_lens is None and total_q != num_seqs:
+        raise RuntimeError("query has more rows than sequences: pass cu_q_lens")
+    _check_scores("scores", scores, dev, num_seqs, hkv)
+    if not (lse.device == dev and lse.dtype == torch.float32 and lse.shape == (total_q, hq) and lse.is_contiguous()):
+        raise RuntimeError("lse must be a contiguous float32 tensor [total_q, num_heads]")
+    for t, name in ((query, "query"), (key_cache, "key_cache")):
+        if not t.is_contiguous() or t.device != dev:
+            raise RuntimeError(f"{name} must be contiguous, on the cache's device")
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    lib = L.load()
+    with torch.cuda.device(dev):
+        p = L.KvWeightsParams(
+            query=query.data_ptr(), key_cache=key_cache.data_ptr(), k_scale=_ptr(k_scale), block_tables=block_tables.data_ptr(),
+            context_lens=context_lens.data_ptr(), cu_q_lens=_ptr(cu_q_lens), lse=lse.data_ptr(), scores=scores.data_ptr(),
+            status=_ptr(status), score_strides=scores.stride()[:2], num_seqs=num_seqs, total_q=total_q, num_q_heads=hq,
+            num_kv_heads=hkv, head_dim=d, page_size=page, max_blocks_per_seq=block_tables.shape[1], num_blocks=nb,
+            max_tokens=scores.shape[2], max_q_len=max_q_len, q_dtype=_DTYPE[query.dtype], k_format=k_format, scale_mode=mode,
+            is_causal=1 if is_causal else 0, softmax_scale=scale, decay=decay)
+        L.check(lib.cuda_llm_kv_accumulate_weights(C.byref(p), _stream_ptr(dev)), "cuda_llm_kv_accumulate_weights")
+    return scores
+
+
+def kv_cache_evict(scores, key_cache, value_cache, k_scale, v_scale, block_tables, context_lens, budget, *, sink=0, recent=0,
+                   new_block_tables: Optional[torch.Tensor] = None, new_scores: Optional[torch.Tensor] = None,
+                   kv_format: Optional[str] = None, status: Optional[torch.Tensor] = None):
+    """Shrink every sequence with more than ``budget`` cached tokens to ``budget``, each KV head by itself: the first ``sink``
+    and the last ``recent`` tokens stay, and of the others those with the largest ``scores`` (fp32 ``[num_seqs, Hkv, tokens]``;
+    of equal ones the earliest; NaN ranks lowest).  The kept tokens move, in order, to the front of the sequence's pages: K, V
+    and scales, bit for bit.  Returns ``(kept, new_context_lens)``: int32 ``[num_seqs, Hkv, budget]`` with the old position of
+    every kept token (-1 behind the new length) and int32 ``[num_seqs]``.  ``new_block_tables``: copy the kept tokens there and
+    leave the old pages alone (pages shared with other sequences).  ``new_scores`` (it may be ``scores``) receives the kept
+    tokens' scores.  Caches as in ``fp8_paged_attention_forward`` / ``paged_attention_forward``; scales ``None`` for 16- and
+    32-bit caches; per-block scales are refused.  No counterpart in the reference."""
+    if not (scores.is_cuda and key_cache.is_cuda and value_cache.is_cuda):
+        raise RuntimeError("Inputs must be on CUDA")
+    if key_cache.dim() != 4 or value_cache.dim() != 4:
+        raise RuntimeError("KV caches must be 4D [num_blocks, num_heads, head_dim, page_size]")
+    nb, hkv, d, page = key_cache.shape
+    dev = key_cache.device
+    k_format = _cache_format(key_cache, kv_format)
+    v_format = _cache_format(value_cache, kv_format, packed_head_dim=d)
+    rows = d // 2 if v_format == L.KV_FP4_E2M1 else d
+    if tuple(value_cache.shape) != (nb, hkv, rows, page) or value_cache.device != dev:
+        raise RuntimeError("key and value caches do not match")
+    mode = 0
+    if k_format == L.KV_FP8_E4M3:
+        if k_scale is None or v_scale is None:
+            raise RuntimeError("an 8-bit cache needs k_scale and v_scale")
+        mode = _scale_mode(k_scale)
+        want = {L.SCALE_PER_HEAD: (hkv,), L.SCALE_PER_BLOCK: (nb, hkv), L.SCALE_PER_TOKEN: (nb, hkv, page),
+                L.SCALE_MX_E8M0: (nb, hkv, d // 32, page)}[mode]
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if tuple(t.shape) != want or t.device != dev or not t.is_contiguous() or t.element_size() != (1 if mode == L.SCALE_MX_E8M0 else 4) \
+                    or (mode != L.SCALE_MX_E8M0 and t.dtype != torch.float32):
+                raise RuntimeError(f"{name} must be {list(want)}, contiguous, float32 (E8M0: bytes), on the cache's device")
+    elif k_scale is not None or v_scale is not None:
+        raise RuntimeError("16- and 32-bit caches take no scales")
+    num_seqs = context_lens.shape[0]
+    target = block_tables if new_block_tables is None else new_block_tables
+    _check_int32(dev, block_tables=block_tables, context_lens=context_lens, new_block_tables=target, status=status)
+    if block_tables.dim() != 2 or target.dim() != 2 or block_tables.shape[0] != num_seqs or target.shape[0] != num_seqs or context_lens.dim() != 1:
+        raise RuntimeError("block tables must be [num_seqs, max_blocks] and context_lens [num_seqs]")
+    _check_scores("scores", scores, dev, num_seqs, hkv)
+    if new_scores is not None:
+        _check_scores("new_scores", new_scores, dev, num_seqs, hkv)
+        if new_scores.shape[2] < min(budget, scores.shape[2]):
+            raise RuntimeError("new_scores needs at least budget entries per row")
+    for t, name in ((key_cache, "key_cache"), (value_cache, "value_cache")):
+        if not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
+    lib = L.load()
+    with torch.cuda.device(dev):
+        new_lens = torch.empty_like(context_lens)
+        kept = torch.empty(num_seqs, hkv, max(int(budget), 0), dtype=torch.int32, device=dev)
+        p = L.KvEvictParams(
+            scores=scores.data_ptr(), new_scores=_ptr(new_scores), key_cache=key_cache.data_ptr(), value_cache=value_cache.data_ptr(),
+            k_scale=_ptr(k_scale), v_scale=_ptr(v_scale), block_tables=block_tables.data_ptr(), new_block_tables=target.data_ptr(),
+            context_lens=context_lens.data_ptr(), new_context_lens=new_lens.data_ptr(), kept=kept.data_ptr(), status=_ptr(status),
+            score_strides=scores.stride()[:2], new_score_strides=(0, 0) if new_scores is None else new_scores.stride()[:2],
+            num_seqs=num_seqs, num_kv_heads=hkv, head_dim=d, page_size=page, max_blocks_per_seq=block_tables.shape[1],
+            new_max_blocks_per_seq=target.shape[1], num_blocks=nb, max_tokens=scores.shape[2], k_format=k_format, v_format=v_format,
+            scale_mode=mode, budget=budget, sink=sink, recent=recent)
+        L.check(lib.cuda_llm_kv_evict(C.byref(p), _stream_ptr(dev)), "cuda_llm_kv_evict")
+    return kept, new_lens
+
+
 def decode_status(workspace: torch.Tensor, device=None) -> int:
     """Read and clear the device status word (synchronises the current stream)."""
     device = workspace.device if device is None else device

@@ -92,7 +92,8 @@ enum CudaLlmKvFormat {
   CUDA_LLM_KV_FP4_E2M1 = 1, /* uint8 [num_blocks, Hkv, D/2, page], low nibble = even d (V only) */
   CUDA_LLM_KV_INT8 = 2,     /* reference's integer reading of the byte (fp8_paged_attention_kernel.cuh:102) */
   CUDA_LLM_KV_F16 = 3,      /* fp16 [num_blocks, Hkv, D, page], no scales (K and V alike)    */
-  CUDA_LLM_KV_BF16 = 4      /* bf16 [num_blocks, Hkv, D, page], no scales (K and V alike)    */
+  CUDA_LLM_KV_BF16 = 4,     /* bf16 [num_blocks, Hkv, D, page], no scales (K and V alike)    */
+  CUDA_LLM_KV_F32 = 5       /* fp32 [num_blocks, Hkv, D, page]; cuda_llm_kv_evict only       */
 };
 
 enum CudaLlmScaleMode {
@@ -324,6 +325,137 @@ int cuda_llm_mx_attention_ws(const void* q, const float* q_scale, const void* k,
                              int32_t is_causal, int32_t out_dtype, void* workspace, size_t workspace_bytes,
                              void* stream);
 int cuda_llm_mx_attention_tcgen05_launches(uint64_t* launches);
+
+/* ---- attention to an encoder's states ------------------------------------------------- */
+/* No counterpart in the reference (its attention entry points take one sequence length).  Attention of
+ * q_len decoder positions to kv_len encoder states, no causal mask:
+ *   out[b, h, i] = sum_t softmax_t(softmax_scale * q[b, h, i] . k[b, h / group, t]) v[b, h / group, t]
+ * over the states t < kv_lens[b], group = num_q_heads / num_kv_heads.  A length of 0 (or less) gives zeros and a
+ * log-sum-exp of -inf; a length above kv_len counts as kv_len.  What lies behind a sequence's length is not read into any
+ * result (it may hold infinities and NaN).  Tensors are addressed by three strides each (batch, head, position, in
+ * elements; head_dim is contiguous): [B, H, S, D] and [B, S, H, D] need no copy, a stride of 0 shares states
+ * between batch rows (beams) or heads.  A dimension of one element may carry any stride.  No workspace; any
+ * number of calls may be in flight, on any streams.
+ *   16-bit types: few query rows per KV head stream the states once, split over a thread-block cluster and joined
+ *   through its shared memory; more rows run on tcgen05.mma.  fp32: a plain fp32 kernel. */
+typedef struct CudaLlmCrossAttentionParams {
+  const void* q;           /* [batch_size, num_q_heads, q_len, head_dim] of dtype              */
+  const void* k;           /* [batch_size, num_kv_heads, kv_len, head_dim]                     */
+  const void* v;           /* as k                                                             */
+  void* out;               /* as q                                                             */
+  float* lse;              /* optional [batch_size, num_q_heads, q_len], contiguous, natural log */
+  const int32_t* kv_lens;  /* [batch_size], or NULL: every sequence has kv_len states          */
+  int64_t q_strides[3];    /* batch, head, position; base addresses and strides are multiples of 16 bytes */
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t out_strides[3];  /* no two elements of out share an address                          */
+  int32_t batch_size;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;    /* divides num_q_heads                                              */
+  int32_t q_len;
+  int32_t kv_len;
+  int32_t head_dim;        /* 64 or 128                                                        */
+  int32_t dtype;           /* CudaLlmDType of q, k, v and out                                  */
+  float softmax_scale;     /* positive                                                         */
+} CudaLlmCrossAttentionParams;
+
+int cuda_llm_cross_attention(const CudaLlmCrossAttentionParams* params, void* stream);
+
+/* Number of bounded waits of the 16-bit cross-attention kernels that ran out on the current device (0 in a healthy
+ * process).  Synchronises the device. */
+int cuda_llm_cross_attention_wait_timeouts(uint32_t* count);
+
+/* ---- eviction from a paged cache by accumulated attention weight ------------------------ */
+/* No counterpart in the reference.  Adds, for every cached token t of every KV head, the attention weight that the
+ * given queries spend on it:
+ *   scores[s, h, t] = decay * old + sum exp(softmax_scale * q . k_t - lse[q])
+ * over the query tokens of sequence s that see t and the num_q_heads / num_kv_heads heads that share KV head h.  `lse` is
+ * what the decode of the same queries returned (a row of -inf saw nothing and adds nothing).  Which query sees which
+ * token: is_causal, token t < context_len - q_len + 1 + j for query token j, as in the decode; otherwise every query sees
+ * every token below the context length.  `old` is 0 for the tokens that the queries brought themselves, t >=
+ * context_len - q_len, so that a token's score needs no clearing when it is appended; decay 0 reads no old score
+ * at all.  Scores at t >= context_len are neither read nor written.  Reads K once and no V; no atomics: the same inputs
+ * give the same bits.  A context longer than the block table or the score row is cut to it (CUDA_LLM_ST_BAD_CTX), a
+ * block index outside the pool leaves its tokens' scores alone (CUDA_LLM_ST_BAD_BLOCK), query offsets that decrease
+ * or leave [0, total_q] count as no queries (CUDA_LLM_ST_BAD_QLEN). */
+typedef struct CudaLlmKvWeightsParams {
+  const void* query;           /* [total_q, num_q_heads, head_dim] of q_dtype                   */
+  const void* key_cache;       /* CUDA_LLM_KV_FP8_E4M3, or _F16 / _BF16 with queries of that type */
+  const void* k_scale;         /* see CudaLlmScaleMode; NULL for a 16-bit cache                 */
+  const int32_t* block_tables; /* [num_seqs, max_blocks_per_seq]                                */
+  const int32_t* context_lens; /* [num_seqs]                                                    */
+  const int32_t* cu_q_lens;    /* [num_seqs + 1], or NULL: one query token per sequence         */
+  const float* lse;            /* [total_q, num_q_heads] natural log                            */
+  float* scores;               /* [num_seqs, num_kv_heads, max_tokens], read and written        */
+  uint32_t* status;            /* optional: CUDA_LLM_ST_* bits are OR-ed into it                */
+  int64_t score_strides[2];    /* sequence, KV head, in elements                                */
+  int32_t num_seqs;
+  int32_t total_q;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;            /* 64 or 128                                                     */
+  int32_t page_size;           /* 16, 32 or 64                                                  */
+  int32_t max_blocks_per_seq;
+  int32_t num_blocks;
+  int32_t max_tokens;          /* entries of a score row                                        */
+  int32_t max_q_len;           /* expected query tokens per sequence (longer ones are right, not fast) */
+  int32_t q_dtype;
+  int32_t k_format;
+  int32_t scale_mode;
+  int32_t is_causal;
+  float softmax_scale;
+  float decay;                 /* 0 to 1                                                        */
+} CudaLlmKvWeightsParams;
+
+int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* params, void* stream);
+
+/* No counterpart in the reference.  Shrinks every sequence with more than `budget` cached tokens to `budget`, for each KV
+ * head by itself: the first `sink` and the last `recent` tokens stay, and of the others those with the largest
+ * scores (of equal scores the lowest position first; NaN ranks below everything).  The kept tokens move, in order, to
+ * positions 0.. of the pages of new_block_tables: K, V and their scales, bit for bit.  kept[s, h, i] is the old
+ * position of the token now at i, -1 from the new length on; new_context_lens[s] = min(context_len, budget).
+ *   new_block_tables == block_tables: in place; sequences within the budget are not touched, and pages behind the new
+ *   length hold what they held.  The pages of a sequence must then be its own.
+ *   another table: every sequence is copied, also one within its budget; its pages must not be pages that block_tables
+ *   names, and the old ones are not written.
+ * `new_scores`, if not NULL, receives the kept tokens' scores (it may be `scores` itself).  Entries behind the new
+ * length are not written, in the caches, the scales and new_scores alike.  Per-block scales are refused: tokens
+ * of pages with different scales cannot share a page without being quantised again.  Lengths that pass the table or
+ * the score row are cut (CUDA_LLM_ST_BAD_CTX); tokens whose old or new page index is outside the pool are not
+ * moved (CUDA_LLM_ST_BAD_BLOCK). */
+typedef struct CudaLlmKvEvictParams {
+  const float* scores;             /* [num_seqs, num_kv_heads, max_tokens]                      */
+  float* new_scores;               /* optional [num_seqs, num_kv_heads, >= budget]              */
+  void* key_cache;                 /* see CudaLlmKvFormat                                       */
+  void* value_cache;
+  void* k_scale;                   /* NULL for 16- and 32-bit caches                            */
+  void* v_scale;
+  const int32_t* block_tables;     /* [num_seqs, max_blocks_per_seq]                            */
+  const int32_t* new_block_tables; /* [num_seqs, new_max_blocks_per_seq]                        */
+  const int32_t* context_lens;     /* [num_seqs]                                                */
+  int32_t* new_context_lens;       /* [num_seqs], not context_lens itself                         */
+  int32_t* kept;                   /* [num_seqs, num_kv_heads, budget]                          */
+  uint32_t* status;                /* optional                                                  */
+  int64_t score_strides[2];        /* sequence, KV head, in elements                            */
+  int64_t new_score_strides[2];
+  int32_t num_seqs;
+  int32_t num_kv_heads;
+  int32_t head_dim;                /* 64 or 128                                                 */
+  int32_t page_size;               /* 16, 32 or 64                                              */
+  int32_t max_blocks_per_seq;
+  int32_t new_max_blocks_per_seq;
+  int32_t num_blocks;
+  int32_t max_tokens;              /* entries of a score row, at most CUDA_LLM_EVICT_MAX_TOKENS */
+  int32_t k_format;                /* CUDA_LLM_KV_FP4_E2M1 is for V only                        */
+  int32_t v_format;
+  int32_t scale_mode;
+  int32_t budget;                  /* at least 1, at least sink + recent                        */
+  int32_t sink;
+  int32_t recent;
+} CudaLlmKvEvictParams;
+#define CUDA_LLM_EVICT_MAX_TOKENS 786432
+
+int cuda_llm_kv_evict(const CudaLlmKvEvictParams* params, void* stream);
 
 /* Bit-exact dequantisation of whole pages to fp32 (test and debugging aid):
  * out [n_pages, Hkv, D, page] fp32 for the pages listed in `pages`. */
