@@ -47,11 +47,13 @@ extern "C" int cuda_llm_cross_attention(const CudaLlmCrossAttentionParams* p, vo
   int rc = check_current_device();
   if (rc != CUDA_LLM_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a.dtype != CUDA_LLM_F32 && (long long)group * a.Sq <= 64) return cuda_result(launch_cross_token(a, D, st), "cross_token_kernel launch");
   return cuda_result(launch_cross_simt(a, D, st), "cross_simt_kernel launch");
 }
 
 extern "C" int cuda_llm_cross_attention_wait_timeouts(uint32_t* count) {
   if (!count) return refuse(CUDA_LLM_EINVAL, "count is null");
   *count = 0;
-  return check_current_device();
+  const int rc = check_current_device();
+  return rc != CUDA_LLM_OK ? rc : cuda_result(cross_wait_timeouts(count), "cudaMemcpyFromSymbol");
 }

@@ -24,6 +24,8 @@ __device__ __forceinline__ int cross_kv_len(const CrossArgs& a, int b) {
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-cudaError_t launch_cross_simt(const CrossArgs& a, int D, cudaStream_t st);
+cudaError_t launch_cross_simt(const CrossArgs& a, int D, cudaStream_t st);   // fp32 arithmetic
+cudaError_t launch_cross_token(const CrossArgs& a, int D, cudaStream_t st);  // 16-bit types, up to 64 query rows per KV head
+cudaError_t cross_wait_timeouts(unsigned int* count);
 
 }  // namespace b200
