@@ -48,6 +48,7 @@ extern "C" int cuda_llm_cross_attention(const CudaLlmCrossAttentionParams* p, vo
   if (rc != CUDA_LLM_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a.dtype != CUDA_LLM_F32 && (long long)group * a.Sq <= 64) return cuda_result(launch_cross_token(a, D, st), "cross_token_kernel launch");
+  if (a.dtype != CUDA_LLM_F32) return cuda_result(launch_cross_prompt(a, D, st), "cross_prompt_kernel launch");
   return cuda_result(launch_cross_simt(a, D, st), "cross_simt_kernel launch");
 }
 
@@ -55,5 +56,10 @@ extern "C" int cuda_llm_cross_attention_wait_timeouts(uint32_t* count) {
   if (!count) return refuse(CUDA_LLM_EINVAL, "count is null");
   *count = 0;
   const int rc = check_current_device();
-  return rc != CUDA_LLM_OK ? rc : cuda_result(cross_wait_timeouts(count), "cudaMemcpyFromSymbol");
+  if (rc != CUDA_LLM_OK) return rc;
+  unsigned int token = 0, prompt = 0;
+  cudaError_t e = cross_wait_timeouts(&token);
+  if (e == cudaSuccess) e = cross_prompt_timeouts(&prompt);
+  *count = token + prompt;
+  return cuda_result(e, "cudaMemcpyFromSymbol");
 }

@@ -26,6 +26,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 cudaError_t launch_cross_simt(const CrossArgs& a, int D, cudaStream_t st);   // fp32 arithmetic
 cudaError_t launch_cross_token(const CrossArgs& a, int D, cudaStream_t st);  // 16-bit types, up to 64 query rows per KV head
-cudaError_t cross_wait_timeouts(unsigned int* count);
+cudaError_t launch_cross_prompt(const CrossArgs& a, int D, cudaStream_t st); // 16-bit types, many query rows
+cudaError_t cross_wait_timeouts(unsigned int* count);    // bounded waits that ran out, per kernel
+cudaError_t cross_prompt_timeouts(unsigned int* count);
 
 }  // namespace b200

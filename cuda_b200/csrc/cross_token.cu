@@ -103,11 +103,11 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
 
   if (warp == 4) {
     if (lane == 0) {
-      for (int j = j0; j < j1; ++j) {
+      int j = j0;
+      for (; j < j1; ++j) {
         const int i = j - j0, st = i % NST;
         if (i >= NST && !tc_wait(empty + 8 * st, ((i / NST) - 1) & 1)) {
           *fail_ptr = 1;
-          for (int x = max(0, i - NST); x < i; ++x) tc_wait(full + 8 * (x % NST), (x / NST) & 1);  // copies in flight land first
           break;
         }
         mbar_arrive_expect_tx(full + 8 * st, STAGE);
@@ -117,6 +117,8 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
           tma_tile_4d(ring + st * STAGE + TILE + c * CH, &a.v, c * 64, j * kTokTile, kvh * a.v_hmul, b * a.v_bmul, full + 8 * st);
         }
       }
+      // copies in flight land before the ring is used for anything else, also after a wait that ran out
+      for (int x = max(0, j - j0 - NST); x < j - j0; ++x) tc_wait(full + 8 * (x % NST), (x / NST) & 1);
     }
   } else {
     // query fragments: rows g and g + 8 of this warp's block, two 16-bit elements per register
