@@ -49,7 +49,7 @@ template <int D>
 constexpr size_t prompt_smem() { return 1024 + (size_t)kPromptRows * D * 2 + (size_t)prompt_slots<D>() * kPromptKeys * D * 2; }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kPromptThreads) __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ CrossPromptArgs a) {
+__global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ CrossPromptArgs a) {
   constexpr int NCH = D / 64, NS = prompt_slots<D>();
   constexpr uint32_t QCH = kPromptRows * 128, KCH = kPromptKeys * 128, SLOT = NCH * KCH;
   constexpr float NEG_INF = -__builtin_huge_valf();
