@@ -7,7 +7,7 @@
 //   warps 0..3, 4..7  softmax of tile 0 and tile 1, one thread per row (= per TMEM lane): S with tcgen05.ld, maximum,
 //                     exponentials, P (16-bit) back over the columns of S
 //   warp 8            TMA: Q once, then K and V tiles of 128 states into a ring of 32 KB slots
-//   warp 9            allocates TMEM, issues the MMAs of both tiles in turn: PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
+//   warp 9            (10, 11 idle) allocates TMEM, issues the MMAs of both tiles in turn: PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
 // Tensor memory: S0/P0 | S1/P1 | O0 | O1, 128 columns each.  P overwrites S: every MMA that reads P of step j is issued
 // before the S of step j + 1, and the tensor pipe works in order.  The same order makes "S(j) is complete" mean "P V (j - 1) is
 // complete", so a softmax thread may rescale O without another barrier.  O is rescaled only when a row maximum grew
@@ -32,7 +32,7 @@ struct alignas(64) CrossPromptArgs {
   int gsz;  // query heads per CTA: 1, 2, 4, 8 or 16, divides the group
 };
 
-constexpr int kPromptThreads = 320;
+constexpr int kPromptThreads = 384;  // three warpgroups: registers are dealt out per warpgroup
 constexpr int kPromptKeys = 128;
 constexpr int kPromptRows = 256;
 
@@ -43,13 +43,32 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
       : "memory");
 }
 
+// Batch rows in the order of falling length: blocks of the longest start first and the short ones fill the last wave.
+// (Block-uniform; every thread counts for one row how many go before it.)
+__device__ __forceinline__ int longest_first(const CrossArgs& c, int z) {
+  if (!c.kv_lens || c.B == 1 || c.B > kPromptThreads) return z;
+  __shared__ int pick;
+  const int b = threadIdx.x;
+  if (b < c.B) {
+    const int n = cross_kv_len(c, b);
+    int before = 0;
+    for (int x = 0; x < c.B; ++x) {
+      const int y = cross_kv_len(c, x);
+      before += (y > n || (y == n && x < b)) ? 1 : 0;
+    }
+    if (before == z) pick = b;
+  }
+  __syncthreads();
+  return pick;
+}
+
 template <int D>
 constexpr int prompt_slots() { return D == 128 ? 5 : 8; }
 template <int D>
 constexpr size_t prompt_smem() { return 1024 + (size_t)kPromptRows * D * 2 + (size_t)prompt_slots<D>() * kPromptKeys * D * 2; }
 
 template <int D, bool BF16>
-__global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ CrossPromptArgs a) {
+__global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const __grid_constant__ CrossPromptArgs a) {
   constexpr int NCH = D / 64, NS = prompt_slots<D>();
   constexpr uint32_t QCH = kPromptRows * 128, KCH = kPromptKeys * 128, SLOT = NCH * KCH;
   constexpr float NEG_INF = -__builtin_huge_valf();
@@ -60,7 +79,7 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
   const uint32_t sQ = base + 1024, ring = sQ + NCH * QCH;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = blockIdx.z;
+  const int b = longest_first(a.c, blockIdx.z);
   const int chunks = a.c.group / a.gsz;
   const int kvh = blockIdx.y / chunks, head0 = kvh * a.c.group + (blockIdx.y - kvh * chunks) * a.gsz;
   const int BQ = kPromptRows / a.gsz;  // positions per CTA
@@ -95,6 +114,9 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
   const uint32_t tmem = *tmem_slot_ptr;
   auto give_up = [&]() { atomicAdd(&g_cross_prompt_timeouts, 1u); };
 
+  // 384 threads x 168 registers at launch = 128 x (88 + 208 + 208): the softmax threads hold a row of 128 scores
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 8) {
     if (n_tiles > 0) {
       bool ok = true;
@@ -194,7 +216,10 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
       }
       if (!ok) give_up();
     }
-  } else if ((warp >> 2) < n_q) {
+  }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  if ((warp >> 2) < n_q) {
     const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + 256 + i * 128;
@@ -226,22 +251,25 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
           mx8[(e >> 1) & 7] = fmax3(mx8[(e >> 1) & 7], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
       const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
       const float m_tile = mx * a.c.scale_log2;
-      const float m_new = (m_tile > m_run + 8.f) ? m_tile : m_run;
-      const float alpha = fast_exp2(m_run - m_new);
-      m_run = m_new;
-      if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+      if (__any_sync(0xffffffffu, m_tile > m_run + 8.f)) {  // some row of the warp needs a new reference
+        const float m_new = (m_tile > m_run + 8.f) ? m_tile : m_run;
+        const float alpha = fast_exp2(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+        if (j > 0) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t x[32];
-          tmem_ld32(tO + c * 32, x);
-          tc_wait_ld();
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            tmem_ld32(tO + c * 32, x);
+            tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-          tmem_st32(tO + c * 32, x);
+            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+            tmem_st32(tO + c * 32, x);
+          }
         }
       }
       float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      const float neg_m = -m_new;
+      const float neg_m = -m_run;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
@@ -249,12 +277,8 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
         for (int e = 0; e < 32; e += 2) {
           float x0, x1, p0, p1;
           ffma2(x0, x1, __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]), a.c.scale_log2, a.c.scale_log2, neg_m, neg_m);
-          if ((e & 6) == 6) {
-            exp2_poly2(x0, x1, p0, p1);
-          } else {
-            p0 = fast_exp2(x0);
-            p1 = fast_exp2(x1);
-          }
+          p0 = fast_exp2(x0);
+          p1 = fast_exp2(x1);
           const int k = (e >> 1) & 3;
           fadd2(ps[2 * k], ps[2 * k + 1], ps[2 * k], ps[2 * k + 1], p0, p1);
           pk[e >> 1] = BF16 ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
@@ -262,7 +286,7 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
         tmem_st16(tS + c * 16, pk);
       }
       tc_wait_st();
-      l_run = l_run * alpha + (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
+      l_run += (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + 8 * i);
@@ -301,6 +325,7 @@ __global__ void __maxnreg__(200) cross_prompt_kernel(const __grid_constant__ Cro
       if (store && a.c.lse)
         a.c.lse[((size_t)b * a.c.Hq + head) * a.c.Sq + pos] = n_tiles > 0 ? kLn2 * (m_run + log2f(l_run)) : NEG_INF;
     }
+  }
   }
   tc_fence_before();
   __syncthreads();
