@@ -2,7 +2,7 @@
 #include <cmath>
 
 #include "host_common.cuh"
-#include "sm100_primitives.cuh"
+#include "tcgen05_primitives.cuh"
 
 namespace b200 {
 
@@ -16,86 +16,562 @@ struct WeightsArgs {
   uint32_t* status;
   long long st_seq, st_head;
   int S, total_q, Hq, Hkv, group, D, page, max_blocks, num_blocks, max_tokens, q_dtype, k_format, scale_mode, causal;
+  int group_shift;  // log2(group), or -1
+  int q_first;  // query row of the first sequence when there are no offsets
   float scale_log2, decay;
 };
 
-__device__ __forceinline__ float load_q(const void* q, size_t i, int dtype) {
-  if (dtype == CUDA_LLM_F32) return static_cast<const float*>(q)[i];
-  if (dtype == CUDA_LLM_F16) return __half2float(static_cast<const __half*>(q)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(q)[i]);
+// ---------------------------------------------------------------------------------------------------------------------
+// Geometry.  A stage of the ring holds K of `hg` KV heads of one sequence for tok_stage consecutive tokens (whole pages, one
+// bulk copy per page: the heads of a page are contiguous) and their scales.  Its 16-token units, one head each, go to the
+// computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
+// ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
+constexpr int kWgtWarps = 16;         // computing warps, resident rows
+constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
+constexpr int kWgtMaxStages = 8;
+constexpr uint32_t kWgtHeader = 192 + 8 * kWgtSeqs + 64;  // barriers, flag, prefix sums, lengths: a multiple of 128
+constexpr uint32_t kWgtBudget = 224 * 1024;
+
+struct WeightsGeom {
+  int hg, n_hg, pages, tok_stage, units;   // pages, tokens and units (head x 16 tokens) of a stage
+  int n_stages;
+  uint32_t k_head, s_head;                 // bytes of one head of one page, K / scales
+  uint32_t k_bytes, s_bytes, stage_bytes;  // of the head group of one page; of a stage
+};
+
+// B fragments of mma.m16n8k16 for 8 query rows: lane (g, t) holds 8 consecutive elements of every 32 of row g, d = 32 p + 8 t ..
+// 8 t + 7.  Word w of them meets matrix (w - t) & 3 of the ldmatrix below, which for lane t brings K at d = 32 p + 8 t +
+// 2 ((m + t) & 3): every product finds its partner, and the eight rows of a matrix lie in different banks.
+__device__ __forceinline__ void rotate_words(uint32_t (&w)[4], int t) {
+  if (t & 1) {
+    const uint32_t x = w[0];
+    w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = x;
+  }
+  if (t & 2) {
+    uint32_t x = w[0];
+    w[0] = w[2]; w[2] = x;
+    x = w[1];
+    w[1] = w[3]; w[3] = x;
+  }
 }
 
-// One thread per cached token of one KV head; the queries of the sequence pass through shared memory eight rows at a time.
-__global__ void __launch_bounds__(128) kv_weights_kernel(const WeightsArgs a) {
-  constexpr int R = 8;
-  __shared__ float sq[R][128];
-  __shared__ float slse[R];
-  const int s = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-  const int cap = min(a.max_blocks * (long long)a.page, (long long)a.max_tokens);
-  int ctx = a.ctx[s];
-  if (ctx > cap) {
-    if (a.status && blockIdx.x == 0 && h == 0 && tid == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_CTX);
-    ctx = cap;
-  }
-  int q0 = a.cuq ? a.cuq[s] : s, q1 = a.cuq ? a.cuq[s + 1] : s + 1;
-  if (q0 < 0 || q1 < q0 || q1 > a.total_q) {
-    if (a.status && blockIdx.x == 0 && h == 0 && tid == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_QLEN);
-    q0 = q1 = 0;
-  }
-  const int t0 = blockIdx.x * 128;
-  if (t0 >= ctx) return;
-  const int n_q = q1 - q0, rows = n_q * a.group, t = t0 + tid;
-  const int blk = t < ctx ? a.bt[(size_t)s * a.max_blocks + t / a.page] : 0, off = t % a.page;
-  bool live = t < ctx;
-  if (live && (blk < 0 || blk >= a.num_blocks)) {
-    if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
-    live = false;
-  }
-  const size_t base = ((size_t)(live ? blk : 0) * a.Hkv + h) * a.D * a.page + off;
-  float sum = 0.f;
-  for (int r0 = 0; r0 < rows; r0 += R) {
-    __syncthreads();
-    for (int i = tid; i < R * a.D; i += 128) {
-      const int r = r0 + i / a.D, d = i % a.D;
-      sq[i / a.D][d] = r < rows ? load_q(a.q, ((size_t)(q0 + r / a.group) * a.Hq + h * a.group + r % a.group) * a.D + d, a.q_dtype) : 0.f;
+enum { KF_E4M3 = 0, KF_F16 = 1, KF_BF16 = 2 };
+
+template <bool BF>
+__device__ __forceinline__ void mma_any(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF) mma_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+  else mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// What the rows of one 8-column block need after the product, for the two columns 2t, 2t + 1 of a lane.
+struct RowPair {
+  float lse2[2], inv[2];  // log-sum-exp in units of log2; 1 / (power of two the query row was multiplied by)
+  int limit[2];           // tokens below it are seen
+};
+
+// row r of a sequence: query token r / group, head r % group of the KV head's group
+__device__ __forceinline__ void row_pair(const WeightsArgs& a, int r0, int rows, int q0, int n_q, int ctx, int h, int t, RowPair& rp) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = r0 + 2 * t + x;  // the lane's two columns
+    rp.lse2[x] = 0.f;
+    rp.inv[x] = 1.f;
+    rp.limit[x] = 0;
+    if (r < rows) {
+      const int j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
+      const float v = a.lse[(size_t)(q0 + j) * a.Hq + h * a.group + (r - j * a.group)];
+      rp.lse2[x] = v * 1.4426950408889634f;
+      rp.limit[x] = v == -__builtin_huge_valf() ? 0 : a.causal ? ctx - n_q + 1 + j : ctx;
     }
-    if (tid < R && r0 + tid < rows) slse[tid] = a.lse[(size_t)(q0 + (r0 + tid) / a.group) * a.Hq + h * a.group + (r0 + tid) % a.group] * 1.4426950408889634f;
-    __syncthreads();
-    if (!live) continue;
-    float acc[R] = {}, part[R];
-    for (int b = 0; b < a.D / 32; ++b) {
+  }
+}
+
+// 8 query rows as B fragments in their own 16-bit type, or an fp32 row as three bf16 terms (24 bits).
+template <int D, int QT>
+__device__ __forceinline__ void load_rows(const void* q, size_t at, bool live, int t, uint32_t (&w)[QT == CUDA_LLM_F32 ? 3 : 1][D / 32][4]) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) part[r] = 0.f;
-      for (int d = b * 32; d < b * 32 + 32; ++d) {
-        const size_t e = base + (size_t)d * a.page;
-        float k;
-        if (a.k_format == CUDA_LLM_KV_FP8_E4M3) k = f16x2_lo(e4m3x2_to_f16x2_lo(a.kc[e]));
-        else if (a.k_format == CUDA_LLM_KV_F16) k = __half2float(reinterpret_cast<const __half*>(a.kc)[e]);
-        else k = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.kc)[e]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) part[r] = fmaf(k, sq[r][d], part[r]);
+  for (int p = 0; p < D / 32; ++p) {
+    if (QT != CUDA_LLM_F32) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (live) u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at + p * 32 + 8 * t);
+      w[0][p][0] = u.x; w[0][p][1] = u.y; w[0][p][2] = u.z; w[0][p][3] = u.w;
+      rotate_words(w[0][p], t);
+    } else {
+      // fp32 as three bf16 terms: 24 bits
+      float f[8] = {};
+      if (live) {
+        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + p * 32 + 8 * t);
+        const float4 x = src[0], y = src[1];
+        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
       }
-      const float f = a.scale_mode == CUDA_LLM_SCALE_MX_E8M0 && a.ks
-                          ? e8m0_to_f32(a.ks[(((size_t)blk * a.Hkv + h) * (a.D / 32) + b) * a.page + off]) : 1.f;
 #pragma unroll
-      for (int r = 0; r < R; ++r) acc[r] = fmaf(part[r], f, acc[r]);
-    }
-    float f = a.scale_log2;
-    const float* ks = reinterpret_cast<const float*>(a.ks);
-    if (a.ks && a.scale_mode == CUDA_LLM_SCALE_PER_HEAD) f *= ks[h];
-    if (a.ks && a.scale_mode == CUDA_LLM_SCALE_PER_BLOCK) f *= ks[(size_t)blk * a.Hkv + h];
-    if (a.ks && a.scale_mode == CUDA_LLM_SCALE_PER_TOKEN) f *= ks[((size_t)blk * a.Hkv + h) * a.page + off];
+      for (int term = 0; term < (QT == CUDA_LLM_F32 ? 3 : 1); ++term) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int j = (r0 + r) / a.group;
-      if (r0 + r < rows && (!a.causal || t < ctx - n_q + 1 + j) && slse[r] != -__builtin_huge_valf())
-        sum += exp2f(fmaf(acc[r], f, -slse[r]));
+        for (int e = 0; e < 4; ++e) {
+          w[term][p][e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+          f[2 * e] -= __uint_as_float(w[term][p][e] << 16);
+          f[2 * e + 1] -= __uint_as_float(w[term][p][e] & 0xffff0000u);
+        }
+        rotate_words(w[term][p], t);
+      }
     }
   }
-  if (!live) return;
-  float* sp = a.scores + s * a.st_seq + h * a.st_head + t;
-  if (a.decay != 0.f && t < ctx - n_q) sum = fmaf(*sp, a.decay, sum);
-  *sp = sum;
+}
+
+// K fragments of 16 tokens: E4M3 codes widened to f16 (exact), or 16-bit elements as they are.  `row_bytes` is the distance of
+// head_dim rows in the slab.  Rows of the result: tokens 2g and 2g + 1 (8 bit) or g and g + 8 (16 bit).
+template <int D, int KF>
+__device__ __forceinline__ void load_keys(uint32_t slab, uint32_t row_bytes, int lane, uint32_t (&af)[D / 16][4]) {
+  if (KF == KF_E4M3) {
+    const int m = lane >> 3, i = lane & 7;
+    const uint32_t at = slab + (8 * (i >> 1) + 2 * ((m + (i >> 1)) & 3) + (i & 1)) * row_bytes;
+#pragma unroll
+    for (int p = 0; p < D / 32; ++p) {
+      uint32_t r[4];
+      ldmatrix_x4_trans(r, at + p * 32 * row_bytes);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        // bytes (token 2g, 2g + 1) of row 2t, then of row 2t + 1 -> (d, d + 1) of token 2g, then of token 2g + 1
+        const uint32_t b = prmt(r[x], 0, 0x3120);
+        af[2 * p + (x >> 1)][2 * (x & 1)] = e4m3x2_to_f16x2_lo(b);
+        af[2 * p + (x >> 1)][2 * (x & 1) + 1] = e4m3x2_to_f16x2_hi(b);
+      }
+    }
+  } else {
+    const int m = lane >> 3, i = lane & 7;  // matrices: (tokens 0..7, 8..15) x (first, second pair)
+#pragma unroll
+    for (int p = 0; p < D / 32; ++p) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t at = slab + (p * 32 + 8 * (i >> 1) + 2 * ((2 * x + (m >> 1) + (i >> 1)) & 3) + (i & 1)) * row_bytes + (m & 1) * 16;
+        ldmatrix_x4_trans(af[2 * p + x], at);
+      }
+    }
+  }
+}
+
+// fp32 rows of the queries of 8 columns, in f16: the row times 2^(14 - exponent of its largest element) keeps every bit of a
+// bf16 element down to 2^-30 of the largest; fp32 elements as hi + lo / 2^11.  `inv` undoes the power of two.
+template <int D, int QT, int NQ>
+__device__ __forceinline__ void load_rows_scaled(const void* q, size_t at, bool live, int t, uint32_t (&w)[NQ][D / 32][4], float (&inv)[2]) {
+  float f[D / 32][8], top = 0.f;
+#pragma unroll
+  for (int p = 0; p < D / 32; ++p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[p][e] = 0.f;
+    if (live && QT == CUDA_LLM_BF16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at + p * 32 + 8 * t);
+      const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[p][2 * e] = __uint_as_float(vv[e] << 16);
+        f[p][2 * e + 1] = __uint_as_float(vv[e] & 0xffff0000u);
+      }
+    } else if (live) {
+      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + p * 32 + 8 * t);
+      const float4 x = src[0], y = src[1];
+      f[p][0] = x.x; f[p][1] = x.y; f[p][2] = x.z; f[p][3] = x.w; f[p][4] = y.x; f[p][5] = y.y; f[p][6] = y.z; f[p][7] = y.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[p][e]));
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const uint32_t e2 = min(max(__float_as_uint(top) >> 23, 15u), 253u);
+  const float up = __uint_as_float(min(268u - e2, 254u) << 23), down = __uint_as_float((e2 - 14u) << 23);
+  inv[0] = __shfl_sync(0xffffffffu, down, 8 * t);      // columns 2t and 2t + 1 are the rows of lanes 8t and 8t + 4
+  inv[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+  for (int p = 0; p < D / 32; ++p) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = f[p][2 * e] * up, y = f[p][2 * e + 1] * up;
+      w[0][p][e] = pack_f16x2(x, y);
+      if (NQ == 2) w[NQ - 1][p][e] = pack_f16x2((x - f16x2_lo(w[0][p][e])) * 2048.f, (y - f16x2_hi(w[0][p][e])) * 2048.f);
+    }
+    rotate_words(w[0][p], t);
+    if (NQ == 2) rotate_words(w[NQ - 1][p], t);
+  }
+}
+
+// The plan of a CTA: its range of stages and the prefix sums to find sequences by.
+struct WeightsPlan {
+  const int *pre, *lens;
+  int w0, w1, s0;
+};
+template <int THREADS>
+__device__ __forceinline__ WeightsPlan make_plan(const WeightsArgs& a, const WeightsGeom& gm, int* pre, int* lens) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int cap = (int)min((long long)a.max_blocks * a.page, (long long)a.max_tokens);
+  for (int s = tid; s < a.S; s += THREADS) {
+    int n = a.ctx[s];
+    if (n > cap) {
+      if (a.status && blockIdx.x == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_CTX);
+      n = cap;
+    }
+    lens[s] = max(n, 0);
+  }
+  __syncthreads();
+  if (tid < 32) {
+    int sum = 0;
+    if (lane == 0) pre[0] = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 32) {
+      const int s = s0 + lane;
+      int x = s < a.S ? (lens[s] + gm.tok_stage - 1) / gm.tok_stage * gm.n_hg : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (s < a.S) pre[s + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+  WeightsPlan p;
+  p.pre = pre;
+  p.lens = lens;
+  const long long total = pre[a.S];
+  p.w0 = (int)(total * blockIdx.x / gridDim.x);
+  p.w1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+  int lo = 0, hi = a.S - 1;  // the last sequence with pre[s] <= w0
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= p.w0) lo = mid;
+    else hi = mid - 1;
+  }
+  p.s0 = lo;
+  return p;
+}
+
+// Producer warp: lane 0 issues the copies; the block-table entries of the next 32 / pages stages are fetched by all lanes.
+__device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom& gm, const WeightsPlan& pl, uint32_t full, uint32_t empty, uint32_t ring,
+                                        volatile int* fail_ptr) {
+  const int lane = threadIdx.x & 31, batch = 32 / gm.pages, pg_mask = gm.pages - 1, pg_shift = __popc(pg_mask);
+  bool ok = true;
+  int i = 0, s = pl.s0;
+  auto entry = [&](int w_first) -> int {
+    const int w = w_first + (lane >> pg_shift);
+    if (w >= pl.w1) return -1;
+    int sq = s;
+    while (w >= pl.pre[sq + 1]) ++sq;
+    const int per = (pl.pre[sq + 1] - pl.pre[sq]) / gm.n_hg, u = (w - pl.pre[sq]) % per;
+    const int page = u * gm.pages + (lane & pg_mask);
+    if ((long long)page * a.page >= pl.lens[sq]) return -1;  // behind the last token: nothing to copy
+    int blk = a.bt[(size_t)sq * a.max_blocks + page];
+    if (blk < 0 || blk >= a.num_blocks) {
+      if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
+      blk = -1;
+    }
+    return blk;
+  };
+  int next = entry(pl.w0);
+  for (int wb = pl.w0; ok && wb < pl.w1; wb += batch) {
+    const int mine = next;
+    while (wb >= pl.pre[s + 1]) ++s;
+    next = entry(wb + batch);
+    int sq = s;
+    for (int k = 0; k < batch && wb + k < pl.w1; ++k, ++i) {
+      const int st = i % gm.n_stages, w = wb + k;
+      const unsigned live = __ballot_sync(0xffffffffu, mine >= 0) >> (k << pg_shift) & (gm.pages == 32 ? 0xffffffffu : (1u << gm.pages) - 1);
+      if (i >= gm.n_stages) ok = tc_wait(empty + 8 * st, ((i / gm.n_stages) - 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      while (w >= pl.pre[sq + 1]) ++sq;
+      const int per = (pl.pre[sq + 1] - pl.pre[sq]) / gm.n_hg, h0 = (w - pl.pre[sq]) / per * gm.hg;
+      if (lane == 0) mbar_arrive_expect_tx(full + 8 * st, (uint32_t)__popc(live) * (gm.k_bytes + gm.s_bytes));
+      __syncwarp();
+      // the lanes that hold the stage's entries issue its copies
+      if ((lane >> pg_shift) == k && mine >= 0) {
+        const int pg = lane & pg_mask;
+        const size_t slab = (size_t)mine * a.Hkv + h0;
+        const uint32_t to = ring + st * gm.stage_bytes;
+        bulk_g2s(to + pg * gm.k_bytes, a.kc + slab * gm.k_head, gm.k_bytes, full + 8 * st);
+        if (gm.s_bytes) bulk_g2s(to + gm.pages * gm.k_bytes + pg * gm.s_bytes, a.ks + slab * gm.s_head, gm.s_bytes, full + 8 * st);
+      }
+    }
+  }
+  if (lane == 0) {
+    for (int x = max(0, i - gm.n_stages); x < i; ++x)  // copies in flight land before the CTA ends
+      if (!tc_wait(full + 8 * (x % gm.n_stages), (x / gm.n_stages) & 1)) ok = false;
+    if (a.status && (!ok || *fail_ptr)) atomicOr(a.status, CUDA_LLM_ST_TIMEOUT);
+  }
+}
+
+// NT > 0: the query fragments of 8 NT rows stay in registers from stage to stage (a decode step: all rows of a KV head).
+// NT == 0: many rows per KV head (a window of a prompt): a warp holds two 16-token units and streams the rows from L2, eight
+// at a time.
+template <int D, int KF, int QT, int NT>
+__global__ void __launch_bounds__(32 * ((NT ? kWgtWarps : 8) + 1), 1)
+kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm) {
+  constexpr bool F8 = KF == KF_E4M3;
+  constexpr int WARPS = NT ? kWgtWarps : 8, U = NT ? 1 : 2, ROWS = NT ? 8 * NT : 8;
+  // operand type of the products: f16, unless the cache or (streamed rows) the queries are bf16 / fp32
+  constexpr bool BF = KF == KF_BF16 || (NT == 0 && QT != CUDA_LLM_F16);
+  constexpr bool SCALED = NT > 0 && F8 && QT != CUDA_LLM_F16;
+  constexpr int TERMS = QT != CUDA_LLM_F32 ? 1 : NT ? 2 : 3;  // of an fp32 query: f16 hi + lo, or three bf16
+  constexpr int QN = NT ? NT : 1;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const uint32_t full = base, empty = base + 8 * kWgtMaxStages, ring = base + kWgtHeader;
+  int* pre = reinterpret_cast<int*>(smem + 192);  // [S + 1] stages before each sequence
+  int* lens = pre + kWgtSeqs + 4;                 // [S] context lengths
+  volatile int* fail_ptr = reinterpret_cast<volatile int*>(smem + 128);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < gm.n_stages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, WARPS);
+    }
+    *fail_ptr = 0;
+    mbar_fence_init();
+  }
+  const WeightsPlan pl = make_plan<32 * (WARPS + 1)>(a, gm, pre, lens);
+  if (pl.w0 >= pl.w1) return;
+  if (warp == WARPS) {
+    produce(a, gm, pl, full, empty, ring, fail_ptr);
+    return;
+  }
+
+  const int g = lane >> 2, t = lane & 3;
+  const int page_shift = 31 - __clz(a.page), groups_shift = page_shift - 4, hg_shift = 31 - __clz(gm.hg);
+  const uint32_t row_bytes = a.page * (F8 ? 1 : 2);
+  const bool is_mx = F8 && a.scale_mode == CUDA_LLM_SCALE_MX_E8M0;
+  uint32_t qf[QN][TERMS][D / 32][4];
+  RowPair rp[QN];
+  int s = pl.s0, cur_s = -1, cur_h = -1, cur_r = -1, q0 = 0, n_q = 0, rows = 0, ctx = 0, per = 1, hgi = 0, u = 0;
+  for (int w = pl.w0, i = 0; w < pl.w1; ++w, ++i) {
+    const int st = i % gm.n_stages;
+    while (w >= pl.pre[s + 1]) ++s;
+    if (s != cur_s) {
+      cur_s = s;
+      cur_h = -1;
+      ctx = pl.lens[s];
+      per = (pl.pre[s + 1] - pl.pre[s]) / gm.n_hg;
+      hgi = (w - pl.pre[s]) / per;
+      u = w - pl.pre[s] - hgi * per;
+      q0 = a.cuq ? a.cuq[s] : a.q_first + s;
+      const int q1 = a.cuq ? a.cuq[s + 1] : q0 + 1;
+      n_q = q1 - q0;
+      if (q0 < 0 || q1 < q0 || q1 > a.total_q) {
+        if (a.status && lane == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_QLEN);
+        q0 = n_q = 0;
+      }
+      rows = n_q * a.group;
+    } else if (++u == per) {
+      u = 0;
+      ++hgi;
+    }
+    bool waited = false;
+    // task of a stage: (token group(s), head), head innermost
+    for (int task = warp; task < gm.units / U; task += WARPS) {
+      const int hl = task & (gm.hg - 1), h = hgi * gm.hg + hl, tg0 = (task >> hg_shift) * U;
+      const int tok0 = u * gm.tok_stage + tg0 * 16;
+      if (tok0 >= ctx) break;
+      // lanes t = 0, 1 keep the scores of two tokens of a unit; the old ones are fetched ahead of the wait
+      float old[U], *sp[U];
+      bool writes[U];
+      int blk[U];
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        const int tok = tok0 + 16 * x + (F8 ? 2 * g + (t & 1) : g + 8 * (t & 1));
+        sp[x] = a.scores + s * a.st_seq + h * a.st_head + tok;
+        writes[x] = t < 2 && tok < ctx;
+        old[x] = 0.f;
+        if (writes[x] && a.decay != 0.f && tok < ctx - n_q) old[x] = *sp[x];
+        blk[x] = tok0 + 16 * x < ctx ? a.bt[(size_t)s * a.max_blocks + ((tok0 + 16 * x) >> page_shift)] : 0;
+      }
+      uint32_t af[U][D / 16][4], mx[U][D / 32];
+      float f_tok[U][2], sum[U][2];
+      auto load_tile = [&]() -> bool {
+        if (!waited) {
+          if (!tc_wait(full + 8 * st, (i / gm.n_stages) & 1)) return false;
+          waited = true;
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+          const int tg = tg0 + x, pg = tg >> groups_shift, sub = tg & ((1 << groups_shift) - 1);
+          const uint32_t stage = ring + st * gm.stage_bytes;
+          load_keys<D, KF>(stage + pg * gm.k_bytes + hl * gm.k_head + sub * (F8 ? 16 : 32), row_bytes, lane, af[x]);
+          if (F8 && BF) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) af[x][kk][e] = pack_bf16x2(f16x2_lo(af[x][kk][e]), f16x2_hi(af[x][kk][e]));
+          }
+          f_tok[x][0] = f_tok[x][1] = a.scale_log2;
+          sum[x][0] = sum[x][1] = 0.f;
+#pragma unroll
+          for (int p = 0; p < D / 32; ++p) mx[x][p] = 0;
+          if (F8) {
+            const uint32_t sc = stage + gm.pages * gm.k_bytes + pg * gm.s_bytes + hl * gm.s_head;
+            if (a.scale_mode == CUDA_LLM_SCALE_PER_TOKEN) {
+              const uint2 v = lds64(sc + (sub * 16 + 2 * g) * 4);
+              f_tok[x][0] *= __uint_as_float(v.x);
+              f_tok[x][1] *= __uint_as_float(v.y);
+            } else if (is_mx) {
+#pragma unroll
+              for (int p = 0; p < D / 32; ++p) mx[x][p] = lds16(sc + p * a.page + sub * 16 + 2 * g);
+            } else {
+              const float* ks = reinterpret_cast<const float*>(a.ks);
+              const bool bad = (unsigned)blk[x] >= (unsigned)a.num_blocks;
+              const float f = a.scale_mode == CUDA_LLM_SCALE_PER_HEAD ? ks[h] : bad ? 0.f : ks[(size_t)blk[x] * a.Hkv + h];
+              f_tok[x][0] *= f;
+              f_tok[x][1] *= f;
+            }
+          }
+        }
+        return true;
+      };
+      bool loaded = false;
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows || !loaded; r0 += ROWS) {
+        if (NT == 0 || h != cur_h || r0 != cur_r) {
+          cur_h = h;
+          cur_r = r0;
+#pragma unroll
+          for (int nt = 0; nt < QN; ++nt) {
+            const int r = r0 + nt * 8 + g, j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
+            const size_t at = ((size_t)(q0 + j) * a.Hq + h * a.group + (r - j * a.group)) * D;
+            row_pair(a, r0 + nt * 8, rows, q0, n_q, ctx, h, t, rp[nt]);
+            if constexpr (SCALED) load_rows_scaled<D, QT, TERMS>(a.q, at, r < rows, t, qf[nt], rp[nt].inv);
+            else load_rows<D, QT>(a.q, at, r < rows, t, qf[nt]);
+          }
+        }
+        if (!loaded) {
+          loaded = true;
+          if (!load_tile()) {
+            *fail_ptr = 1;
+            return;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+          const int tok_a = tok0 + 16 * x + (F8 ? 2 * g : g), tok_b = tok0 + 16 * x + (F8 ? 2 * g + 1 : g + 8);
+#pragma unroll
+          for (int nt = 0; nt < QN; ++nt) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = 0; p < D / 32; ++p) {
+              float part[4] = {0.f, 0.f, 0.f, 0.f};
+              if (NT > 0 && TERMS == 2) {
+                mma_any<BF>(part, af[x][2 * p], qf[nt][TERMS - 1][p][0], qf[nt][TERMS - 1][p][1]);
+                mma_any<BF>(part, af[x][2 * p + 1], qf[nt][TERMS - 1][p][2], qf[nt][TERMS - 1][p][3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[e] *= 1.f / 2048.f;
+              }
+#pragma unroll
+              for (int term = (NT > 0 ? 1 : TERMS) - 1; term >= 0; --term) {
+                mma_any<BF>(part, af[x][2 * p], qf[nt][term][p][0], qf[nt][term][p][1]);
+                mma_any<BF>(part, af[x][2 * p + 1], qf[nt][term][p][2], qf[nt][term][p][3]);
+              }
+              const float ea = is_mx ? e8m0_to_f32(mx[x][p] & 0xffu) : 1.f, eb = is_mx ? e8m0_to_f32(mx[x][p] >> 8) : 1.f;
+              c[0] = fmaf(part[0], ea, c[0]);
+              c[1] = fmaf(part[1], ea, c[1]);
+              c[2] = fmaf(part[2], eb, c[2]);
+              c[3] = fmaf(part[3], eb, c[3]);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              if (tok_a < rp[nt].limit[y]) sum[x][0] += fast_exp2(fmaf(c[y], f_tok[x][0] * rp[nt].inv[y], -rp[nt].lse2[y]));
+              if (tok_b < rp[nt].limit[y]) sum[x][1] += fast_exp2(fmaf(c[2 + y], f_tok[x][1] * rp[nt].inv[y], -rp[nt].lse2[y]));
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sum[x][e] += __shfl_xor_sync(0xffffffffu, sum[x][e], 1);
+          sum[x][e] += __shfl_xor_sync(0xffffffffu, sum[x][e], 2);
+        }
+        if (writes[x] && (unsigned)blk[x] < (unsigned)a.num_blocks) *sp[x] = fmaf(old[x], a.decay, (t & 1) ? sum[x][1] : sum[x][0]);
+      }
+    }
+    if (!waited && !tc_wait(full + 8 * st, (i / gm.n_stages) & 1)) {
+      *fail_ptr = 1;
+      return;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8 * st);
+  }
+}
+
+template <int D, int KF, int QT, int NT>
+static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cudaStream_t st) {
+  auto kern = kv_weights_kernel<D, KF, QT, NT>;
+  const size_t smem = kWgtHeader + (size_t)gm.n_stages * gm.stage_bytes;
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWgtBudget);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) configured[dev] = 1;
+  }
+  kern<<<grid, 32 * ((NT ? kWgtWarps : 8) + 1), smem, st>>>(a, gm);
+  return cudaGetLastError();
+}
+
+template <int D, int KF, int QT>
+static cudaError_t go_rows(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
+  if (nt == 1) return go<D, KF, QT, 1>(a, gm, grid, st);
+  if constexpr (QT != CUDA_LLM_F32)
+    if (nt == 2) return go<D, KF, QT, 2>(a, gm, grid, st);
+  return go<D, KF, QT, 0>(a, gm, grid, st);
+}
+template <int D>
+static cudaError_t go_types(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
+  if (a.k_format == CUDA_LLM_KV_F16) return go_rows<D, KF_F16, CUDA_LLM_F16>(a, gm, grid, nt, st);
+  if (a.k_format == CUDA_LLM_KV_BF16) return go_rows<D, KF_BF16, CUDA_LLM_BF16>(a, gm, grid, nt, st);
+  if (a.q_dtype == CUDA_LLM_F32) return go_rows<D, KF_E4M3, CUDA_LLM_F32>(a, gm, grid, nt, st);
+  if (a.q_dtype == CUDA_LLM_F16) return go_rows<D, KF_E4M3, CUDA_LLM_F16>(a, gm, grid, nt, st);
+  return go_rows<D, KF_E4M3, CUDA_LLM_BF16>(a, gm, grid, nt, st);
+}
+
+static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cudaStream_t st) {
+  const long long declared = (long long)a.group * (max_q_len < 1 ? 1 : max_q_len);
+  // rows that stay in registers: 8, 16 (16-bit queries), or none
+  const int nt = declared <= 8 ? 1 : declared <= 16 && a.q_dtype != CUDA_LLM_F32 ? 2 : 0;
+  const int eb = a.k_format == CUDA_LLM_KV_FP8_E4M3 ? 1 : 2, groups = a.page / 16;
+  // units of a stage: 32 KB of K (head_dim 128); with streamed rows at least two token groups of a head
+  const int want = nt ? 16 / eb : 16;
+  WeightsGeom gm;
+  gm.hg = nt ? 8 : 4;
+  while (a.Hkv % gm.hg || gm.hg * groups > want) gm.hg >>= 1;
+  gm.n_hg = a.Hkv / gm.hg;
+  gm.pages = want / (gm.hg * groups);
+  gm.tok_stage = gm.pages * a.page;
+  gm.units = gm.pages * groups * gm.hg;
+  gm.k_head = (uint32_t)a.D * a.page * eb;
+  gm.s_head = eb == 2 ? 0u : a.scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? (uint32_t)a.page * 4
+              : a.scale_mode == CUDA_LLM_SCALE_MX_E8M0 ? (uint32_t)(a.D / 32) * a.page : 0u;
+  gm.k_bytes = gm.hg * gm.k_head;
+  gm.s_bytes = gm.hg * gm.s_head;
+  gm.stage_bytes = ((gm.k_bytes + gm.s_bytes) * gm.pages + 127) / 128 * 128;
+  gm.n_stages = (int)((kWgtBudget - kWgtHeader) / gm.stage_bytes);
+  if (gm.n_stages > kWgtMaxStages) gm.n_stages = kWgtMaxStages;
+  const long long cap = (long long)a.max_blocks * a.page < a.max_tokens ? (long long)a.max_blocks * a.page : a.max_tokens;
+  a.group_shift = (a.group & (a.group - 1)) ? -1 : __builtin_ctz(a.group);
+  const int S = a.S;
+  for (int s0 = 0; s0 < S; s0 += kWgtSeqs) {
+    WeightsArgs x = a;
+    x.S = S - s0 < kWgtSeqs ? S - s0 : kWgtSeqs;
+    x.bt += (size_t)s0 * a.max_blocks;
+    x.ctx += s0;
+    if (x.cuq) x.cuq += s0;
+    x.q_first = s0;
+    x.scores += s0 * a.st_seq;
+    const long long most = (cap + gm.tok_stage - 1) / gm.tok_stage * gm.n_hg * x.S;
+    const int grid = (int)(most < sms ? most : sms);
+    const cudaError_t e = a.D == 64 ? go_types<64>(x, gm, grid, nt, st) : go_types<128>(x, gm, grid, nt, st);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace b200
@@ -140,7 +616,6 @@ extern "C" int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* p, v
   a.D = p->head_dim; a.page = p->page_size; a.max_blocks = p->max_blocks_per_seq; a.num_blocks = p->num_blocks;
   a.max_tokens = p->max_tokens; a.q_dtype = p->q_dtype; a.k_format = p->k_format; a.scale_mode = p->scale_mode;
   a.causal = p->is_causal ? 1 : 0; a.scale_log2 = p->softmax_scale * 1.4426950408889634f; a.decay = p->decay;
-  const long long cap = (long long)a.max_blocks * a.page < a.max_tokens ? (long long)a.max_blocks * a.page : a.max_tokens;
-  kv_weights_kernel<<<dim3((unsigned)((cap + 127) / 128), a.Hkv, a.S), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  return cuda_result(cudaGetLastError(), "kv_weights_kernel launch");
+  a.q_first = 0;
+  return cuda_result(launch_kv_weights(a, p->max_q_len, current_sm_count(), reinterpret_cast<cudaStream_t>(stream)), "kv_weights_kernel launch");
 }
