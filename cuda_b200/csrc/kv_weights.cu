@@ -26,10 +26,10 @@ struct WeightsArgs {
 // bulk copy per page: the heads of a page are contiguous) and their scales.  Its 16-token units, one head each, go to the
 // computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
 // ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
-constexpr int kWgtWarps = 16;         // computing warps, resident rows
+constexpr int kWgtWarps = 16;         // 16-token units of a stage, and computing warps (half of them with two units each)
 constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
-constexpr uint32_t kWgtHeader = 192 + 8 * kWgtSeqs + 64;  // barriers, flag, prefix sums, lengths: a multiple of 128
+constexpr uint32_t kWgtHeader = 192 + 8 * kWgtSeqs + 64;  // barriers, page masks, flag, prefix sums, lengths: a multiple of 128
 constexpr uint32_t kWgtBudget = 224 * 1024;
 
 struct WeightsGeom {
@@ -118,35 +118,30 @@ __device__ __forceinline__ void load_rows(const void* q, size_t at, bool live, i
   }
 }
 
-// K fragments of 16 tokens: E4M3 codes widened to f16 (exact), or 16-bit elements as they are.  `row_bytes` is the distance of
-// head_dim rows in the slab.  Rows of the result: tokens 2g and 2g + 1 (8 bit) or g and g + 8 (16 bit).
-template <int D, int KF>
-__device__ __forceinline__ void load_keys(uint32_t slab, uint32_t row_bytes, int lane, uint32_t (&af)[D / 16][4]) {
+// K fragments of 16 tokens and 32 elements of head_dim (two k-steps): E4M3 codes widened to f16 (exact), or 16-bit elements as
+// they are.  `at` comes from key_row().  Rows of the result: tokens 2g and 2g + 1 (8 bit) or g and g + 8 (16 bit).
+template <int KF>
+__device__ __forceinline__ uint32_t key_row(int lane, uint32_t row_bytes, int x) {
+  const int m = lane >> 3, i = lane & 7;
+  if (KF == KF_E4M3) return (8 * (i >> 1) + 2 * ((m + (i >> 1)) & 3) + (i & 1)) * row_bytes;
+  // matrices of k-step x: (tokens 0..7, 8..15) x (first, second pair of elements)
+  return (8 * (i >> 1) + 2 * ((2 * x + (m >> 1) + (i >> 1)) & 3) + (i & 1)) * row_bytes + (m & 1) * 16;
+}
+template <int KF>
+__device__ __forceinline__ void load_key_block(const uint32_t (&at)[2], uint32_t offset, uint32_t (&af)[2][4]) {
   if (KF == KF_E4M3) {
-    const int m = lane >> 3, i = lane & 7;
-    const uint32_t at = slab + (8 * (i >> 1) + 2 * ((m + (i >> 1)) & 3) + (i & 1)) * row_bytes;
+    uint32_t r[4];
+    ldmatrix_x4_trans(r, at[0] + offset);
 #pragma unroll
-    for (int p = 0; p < D / 32; ++p) {
-      uint32_t r[4];
-      ldmatrix_x4_trans(r, at + p * 32 * row_bytes);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        // bytes (token 2g, 2g + 1) of row 2t, then of row 2t + 1 -> (d, d + 1) of token 2g, then of token 2g + 1
-        const uint32_t b = prmt(r[x], 0, 0x3120);
-        af[2 * p + (x >> 1)][2 * (x & 1)] = e4m3x2_to_f16x2_lo(b);
-        af[2 * p + (x >> 1)][2 * (x & 1) + 1] = e4m3x2_to_f16x2_hi(b);
-      }
+    for (int x = 0; x < 4; ++x) {
+      // bytes (token 2g, 2g + 1) of row 2t, then of row 2t + 1 -> (d, d + 1) of token 2g, then of token 2g + 1
+      const uint32_t b = prmt(r[x], 0, 0x3120);
+      af[x >> 1][2 * (x & 1)] = e4m3x2_to_f16x2_lo(b);
+      af[x >> 1][2 * (x & 1) + 1] = e4m3x2_to_f16x2_hi(b);
     }
   } else {
-    const int m = lane >> 3, i = lane & 7;  // matrices: (tokens 0..7, 8..15) x (first, second pair)
-#pragma unroll
-    for (int p = 0; p < D / 32; ++p) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t at = slab + (p * 32 + 8 * (i >> 1) + 2 * ((2 * x + (m >> 1) + (i >> 1)) & 3) + (i & 1)) * row_bytes + (m & 1) * 16;
-        ldmatrix_x4_trans(af[2 * p + x], at);
-      }
-    }
+    ldmatrix_x4_trans(af[0], at[0] + offset);
+    ldmatrix_x4_trans(af[1], at[1] + offset);
   }
 }
 
@@ -245,11 +240,13 @@ __device__ __forceinline__ WeightsPlan make_plan(const WeightsArgs& a, const Wei
 }
 
 // Producer warp: lane 0 issues the copies; the block-table entries of the next 32 / pages stages are fetched by all lanes.
-__device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom& gm, const WeightsPlan& pl, uint32_t full, uint32_t empty, uint32_t ring,
-                                        volatile int* fail_ptr) {
+// Beside a stage lies a mask of the pages that were copied (bad block-table entries are not).
+__device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom& gm, const WeightsPlan& pl, uint32_t full, uint32_t empty, uint32_t live_at,
+                                        uint32_t ring, volatile int* fail_ptr) {
   const int lane = threadIdx.x & 31, batch = 32 / gm.pages, pg_mask = gm.pages - 1, pg_shift = __popc(pg_mask);
   bool ok = true;
-  int i = 0, s = pl.s0;
+  int i = 0, s = pl.s0, st = 0;
+  uint32_t free_par = 1;  // the first round finds every slot free
   auto entry = [&](int w_first) -> int {
     const int w = w_first + (lane >> pg_shift);
     if (w >= pl.w1) return -1;
@@ -272,16 +269,19 @@ __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom&
     next = entry(wb + batch);
     int sq = s;
     for (int k = 0; k < batch && wb + k < pl.w1; ++k, ++i) {
-      const int st = i % gm.n_stages, w = wb + k;
+      const int w = wb + k;
       const unsigned live = __ballot_sync(0xffffffffu, mine >= 0) >> (k << pg_shift) & (gm.pages == 32 ? 0xffffffffu : (1u << gm.pages) - 1);
-      if (i >= gm.n_stages) ok = tc_wait(empty + 8 * st, ((i / gm.n_stages) - 1) & 1);
+      ok = mbar_wait(empty + 8 * st, free_par, 0);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       while (w >= pl.pre[sq + 1]) ++sq;
       const int per = (pl.pre[sq + 1] - pl.pre[sq]) / gm.n_hg, h0 = (w - pl.pre[sq]) / per * gm.hg;
-      if (lane == 0) mbar_arrive_expect_tx(full + 8 * st, (uint32_t)__popc(live) * (gm.k_bytes + gm.s_bytes));
+      if (lane == 0) {
+        sts32(live_at + 4 * st, (int)live);
+        mbar_arrive_expect_tx(full + 8 * st, (uint32_t)__popc(live) * (gm.k_bytes + gm.s_bytes));
+      }
       __syncwarp();
       // the lanes that hold the stage's entries issue its copies
       if ((lane >> pg_shift) == k && mine >= 0) {
@@ -291,23 +291,29 @@ __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom&
         bulk_g2s(to + pg * gm.k_bytes, a.kc + slab * gm.k_head, gm.k_bytes, full + 8 * st);
         if (gm.s_bytes) bulk_g2s(to + gm.pages * gm.k_bytes + pg * gm.s_bytes, a.ks + slab * gm.s_head, gm.s_bytes, full + 8 * st);
       }
+      if (++st == gm.n_stages) {
+        st = 0;
+        free_par ^= 1;
+      }
     }
   }
   if (lane == 0) {
     for (int x = max(0, i - gm.n_stages); x < i; ++x)  // copies in flight land before the CTA ends
-      if (!tc_wait(full + 8 * (x % gm.n_stages), (x / gm.n_stages) & 1)) ok = false;
+      if (!mbar_wait(full + 8 * (x % gm.n_stages), (x / gm.n_stages) & 1, 0)) ok = false;
     if (a.status && (!ok || *fail_ptr)) atomicOr(a.status, CUDA_LLM_ST_TIMEOUT);
   }
 }
 
-// NT > 0: the query fragments of 8 NT rows stay in registers from stage to stage (a decode step: all rows of a KV head).
-// NT == 0: many rows per KV head (a window of a prompt): a warp holds two 16-token units and streams the rows from L2, eight
+// One stage is one task per computing warp: head warp % hg of the group, a run of 16-token units.
+// NT > 0: the query fragments of 8 NT rows stay in registers from stage to stage (a decode step: all rows of a KV head); a
+// sequence with more rows than that is right but reloads them.
+// NT == 0: many rows per KV head (a window of a prompt): a warp holds the keys of two units and streams the rows from L2, eight
 // at a time.
-template <int D, int KF, int QT, int NT>
-__global__ void __launch_bounds__(32 * ((NT ? kWgtWarps : 8) + 1), 1)
+template <int D, int KF, int QT, int NT, bool MX>
+__global__ void __launch_bounds__(32 * ((NT ? kWgtWarps : kWgtWarps / 2) + 1), 1)
 kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm) {
   constexpr bool F8 = KF == KF_E4M3;
-  constexpr int WARPS = NT ? kWgtWarps : 8, U = NT ? 1 : 2, ROWS = NT ? 8 * NT : 8;
+  constexpr int U = NT ? 1 : 2, WARPS = kWgtWarps / U, ROWS = NT ? 8 * NT : 8;
   // operand type of the products: f16, unless the cache or (streamed rows) the queries are bf16 / fp32
   constexpr bool BF = KF == KF_BF16 || (NT == 0 && QT != CUDA_LLM_F16);
   constexpr bool SCALED = NT > 0 && F8 && QT != CUDA_LLM_F16;
@@ -315,10 +321,10 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   constexpr int QN = NT ? NT : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t full = base, empty = base + 8 * kWgtMaxStages, ring = base + kWgtHeader;
+  const uint32_t full = base, empty = base + 8 * kWgtMaxStages, live_at = base + 128, ring = base + kWgtHeader;
   int* pre = reinterpret_cast<int*>(smem + 192);  // [S + 1] stages before each sequence
   int* lens = pre + kWgtSeqs + 4;                 // [S] context lengths
-  volatile int* fail_ptr = reinterpret_cast<volatile int*>(smem + 128);
+  volatile int* fail_ptr = reinterpret_cast<volatile int*>(smem + 160);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < gm.n_stages; ++i) {
@@ -331,23 +337,38 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   const WeightsPlan pl = make_plan<32 * (WARPS + 1)>(a, gm, pre, lens);
   if (pl.w0 >= pl.w1) return;
   if (warp == WARPS) {
-    produce(a, gm, pl, full, empty, ring, fail_ptr);
+    produce(a, gm, pl, full, empty, live_at, ring, fail_ptr);
     return;
   }
 
   const int g = lane >> 2, t = lane & 3;
-  const int page_shift = 31 - __clz(a.page), groups_shift = page_shift - 4, hg_shift = 31 - __clz(gm.hg);
+  const int groups = a.page >> 4;  // 16-token groups of a page
+  const int hl = warp & (gm.hg - 1), tg0 = warp / gm.hg * U, pg0 = tg0 / groups, sub0 = tg0 % groups;
   const uint32_t row_bytes = a.page * (F8 ? 1 : 2);
-  const bool is_mx = F8 && a.scale_mode == CUDA_LLM_SCALE_MX_E8M0;
+  // this lane's places in a stage: rows for ldmatrix, scales, page bit; unit 1 is the next group of the same or the next page
+  uint32_t key_at[U][2], scale_at[U];
+  int pg[U];
+#pragma unroll
+  for (int x = 0; x < U; ++x) {
+    const int sub = sub0 + x < groups ? sub0 + x : 0;
+    pg[x] = sub0 + x < groups ? pg0 : pg0 + 1;
+    const uint32_t slab = ring + pg[x] * gm.k_bytes + hl * gm.k_head + sub * (F8 ? 16 : 32);
+    key_at[x][0] = slab + key_row<KF>(lane, row_bytes, 0);
+    key_at[x][1] = slab + key_row<KF>(lane, row_bytes, 1);
+    scale_at[x] = ring + gm.pages * gm.k_bytes + pg[x] * gm.s_bytes + hl * gm.s_head + (sub * 16 + 2 * g) * (MX ? 1 : 4);
+  }
+  const int lane_tok = tg0 * 16 + (F8 ? 2 * g + (t & 1) : g + 8 * (t & 1));  // lanes t = 0, 1 keep the scores of two tokens of a unit
   uint32_t qf[QN][TERMS][D / 32][4];
   RowPair rp[QN];
-  int s = pl.s0, cur_s = -1, cur_h = -1, cur_r = -1, q0 = 0, n_q = 0, rows = 0, ctx = 0, per = 1, hgi = 0, u = 0;
-  for (int w = pl.w0, i = 0; w < pl.w1; ++w, ++i) {
-    const int st = i % gm.n_stages;
+
+  // the task one stage ahead: where it is, and its old scores, on their way while the stage in hand is worked on
+  int s = pl.s0, ctx = 0, per = 1, hgi = 0, u = -1, q0 = 0, n_q = 0, seq = -1;
+  float* sp = nullptr;
+  float old[U];
+  auto locate = [&](int w) {
     while (w >= pl.pre[s + 1]) ++s;
-    if (s != cur_s) {
-      cur_s = s;
-      cur_h = -1;
+    if (s != seq) {
+      seq = s;
       ctx = pl.lens[s];
       per = (pl.pre[s + 1] - pl.pre[s]) / gm.n_hg;
       hgi = (w - pl.pre[s]) / per;
@@ -359,125 +380,149 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
         if (a.status && lane == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_QLEN);
         q0 = n_q = 0;
       }
-      rows = n_q * a.group;
     } else if (++u == per) {
       u = 0;
       ++hgi;
     }
-    bool waited = false;
-    // task of a stage: (token group(s), head), head innermost
-    for (int task = warp; task < gm.units / U; task += WARPS) {
-      const int hl = task & (gm.hg - 1), h = hgi * gm.hg + hl, tg0 = (task >> hg_shift) * U;
-      const int tok0 = u * gm.tok_stage + tg0 * 16;
-      if (tok0 >= ctx) break;
-      // lanes t = 0, 1 keep the scores of two tokens of a unit; the old ones are fetched ahead of the wait
-      float old[U], *sp[U];
-      bool writes[U];
-      int blk[U];
+    const int tok = u * gm.tok_stage + lane_tok;
+    sp = a.scores + s * a.st_seq + (hgi * gm.hg + hl) * a.st_head + tok;
+#pragma unroll
+    for (int x = 0; x < U; ++x) old[x] = (t < 2 && a.decay != 0.f && tok + 16 * x < ctx - n_q) ? sp[16 * x] : 0.f;
+  };
+  locate(pl.w0);
+  int cur_s = -1, cur_h = -1, cur_r = -1, st = 0;
+  uint32_t par = 0, ring_off = 0;
+  for (int w = pl.w0; w < pl.w1; ++w) {
+    const int my_s = s, h = hgi * gm.hg + hl, tok0 = u * gm.tok_stage + tg0 * 16, my_ctx = ctx, my_q0 = q0, my_nq = n_q, rows = n_q * a.group;
+    float* const my_sp = sp;
+    float my_old[U];
+#pragma unroll
+    for (int x = 0; x < U; ++x) my_old[x] = old[x];
+    if (w + 1 < pl.w1) locate(w + 1);
+    if (tok0 < my_ctx) {
+      auto fetch_rows = [&](int r0) {
+        cur_s = my_s;
+        cur_h = h;
+        cur_r = r0;
+#pragma unroll
+        for (int nt = 0; nt < QN; ++nt) {
+          const int r = r0 + nt * 8 + g, j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
+          const size_t at = ((size_t)(my_q0 + j) * a.Hq + h * a.group + (r - j * a.group)) * D;
+          row_pair(a, r0 + nt * 8, rows, my_q0, my_nq, my_ctx, h, t, rp[nt]);
+          if constexpr (SCALED) load_rows_scaled<D, QT, TERMS>(a.q, at, r < rows, t, qf[nt], rp[nt].inv);
+          else load_rows<D, QT>(a.q, at, r < rows, t, qf[nt]);
+        }
+      };
+      if (NT > 0 && (my_s != cur_s || h != cur_h || cur_r != 0)) fetch_rows(0);
+      if (!mbar_wait(full + 8 * st, par, 0)) {
+        *fail_ptr = 1;
+        return;
+      }
+      const uint32_t live = lds32(live_at + 4 * st);
+      float f_tok[U][2], sum[U][2];
+      uint32_t mx[U][MX ? D / 32 : 1];
 #pragma unroll
       for (int x = 0; x < U; ++x) {
-        const int tok = tok0 + 16 * x + (F8 ? 2 * g + (t & 1) : g + 8 * (t & 1));
-        sp[x] = a.scores + s * a.st_seq + h * a.st_head + tok;
-        writes[x] = t < 2 && tok < ctx;
-        old[x] = 0.f;
-        if (writes[x] && a.decay != 0.f && tok < ctx - n_q) old[x] = *sp[x];
-        blk[x] = tok0 + 16 * x < ctx ? a.bt[(size_t)s * a.max_blocks + ((tok0 + 16 * x) >> page_shift)] : 0;
+        f_tok[x][0] = f_tok[x][1] = a.scale_log2;
+        sum[x][0] = sum[x][1] = 0.f;
+        if (MX) {
+#pragma unroll
+          for (int p = 0; p < D / 32; ++p) mx[x][p] = lds16(scale_at[x] + ring_off + p * a.page);
+        } else if (F8) {
+          float fa, fb;
+          if (a.scale_mode == CUDA_LLM_SCALE_PER_TOKEN) {
+            const uint2 v = lds64(scale_at[x] + ring_off);
+            fa = __uint_as_float(v.x);
+            fb = __uint_as_float(v.y);
+          } else {
+            const float* ks = reinterpret_cast<const float*>(a.ks);
+            fa = 0.f;
+            if (a.scale_mode == CUDA_LLM_SCALE_PER_HEAD) fa = ks[h];
+            else if (live >> pg[x] & 1) fa = ks[(size_t)a.bt[(size_t)my_s * a.max_blocks + (tok0 + 16 * x) / a.page] * a.Hkv + h];
+            fb = fa;
+          }
+          f_tok[x][0] *= fa;
+          f_tok[x][1] *= fb;
+        }
       }
-      uint32_t af[U][D / 16][4], mx[U][D / 32];
-      float f_tok[U][2], sum[U][2];
-      auto load_tile = [&]() -> bool {
-        if (!waited) {
-          if (!tc_wait(full + 8 * st, (i / gm.n_stages) & 1)) return false;
-          waited = true;
+      auto add_weights = [&](int x, const float (&c)[4], const RowPair& r) {
+        const int tok_a = tok0 + 16 * x + (F8 ? 2 * g : g), tok_b = tok_a + (F8 ? 1 : 8);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float wa = fast_exp2(fmaf(c[y], f_tok[x][0] * r.inv[y], -r.lse2[y])), wb = fast_exp2(fmaf(c[2 + y], f_tok[x][1] * r.inv[y], -r.lse2[y]));
+          sum[x][0] += tok_a < r.limit[y] ? wa : 0.f;
+          sum[x][1] += tok_b < r.limit[y] ? wb : 0.f;
+        }
+      };
+      // c += K block p of one unit times the rows of one 8-column block
+      auto dot_block = [&](float (&c)[4], const uint32_t (&af)[2][4], const uint32_t (&q)[TERMS][D / 32][4], int x, int p) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!MX && !(NT > 0 && TERMS == 2)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[e] = c[e];
+        }
+        if (NT > 0 && TERMS == 2) {
+          mma_any<BF>(part, af[0], q[TERMS - 1][p][0], q[TERMS - 1][p][1]);
+          mma_any<BF>(part, af[1], q[TERMS - 1][p][2], q[TERMS - 1][p][3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[e] = MX ? part[e] * (1.f / 2048.f) : fmaf(part[e], 1.f / 2048.f, c[e]);
         }
 #pragma unroll
-        for (int x = 0; x < U; ++x) {
-          const int tg = tg0 + x, pg = tg >> groups_shift, sub = tg & ((1 << groups_shift) - 1);
-          const uint32_t stage = ring + st * gm.stage_bytes;
-          load_keys<D, KF>(stage + pg * gm.k_bytes + hl * gm.k_head + sub * (F8 ? 16 : 32), row_bytes, lane, af[x]);
-          if (F8 && BF) {
+        for (int term = (NT > 0 ? 1 : TERMS) - 1; term >= 0; --term) {
+          mma_any<BF>(part, af[0], q[term][p][0], q[term][p][1]);
+          mma_any<BF>(part, af[1], q[term][p][2], q[term][p][3]);
+        }
+        if (MX) {
+          const float ea = e8m0_to_f32(mx[x][p] & 0xffu), eb = e8m0_to_f32(mx[x][p] >> 8);
+          c[0] = fmaf(part[0], ea, c[0]);
+          c[1] = fmaf(part[1], ea, c[1]);
+          c[2] = fmaf(part[2], eb, c[2]);
+          c[3] = fmaf(part[3], eb, c[3]);
+        } else {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
+          for (int e = 0; e < 4; ++e) c[e] = part[e];
+        }
+      };
+      if constexpr (NT > 0) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += ROWS) {
+          if (r0 > 0) fetch_rows(r0);
+          float c[NT][2][4] = {};  // two chains of products
 #pragma unroll
-              for (int e = 0; e < 4; ++e) af[x][kk][e] = pack_bf16x2(f16x2_lo(af[x][kk][e]), f16x2_hi(af[x][kk][e]));
+          for (int p = 0; p < D / 32; ++p) {
+            uint32_t af[2][4];
+            load_key_block<KF>(key_at[0], ring_off + p * 32 * row_bytes, af);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) dot_block(c[nt][p & 1], af, qf[nt], 0, p);
           }
-          f_tok[x][0] = f_tok[x][1] = a.scale_log2;
-          sum[x][0] = sum[x][1] = 0.f;
 #pragma unroll
-          for (int p = 0; p < D / 32; ++p) mx[x][p] = 0;
-          if (F8) {
-            const uint32_t sc = stage + gm.pages * gm.k_bytes + pg * gm.s_bytes + hl * gm.s_head;
-            if (a.scale_mode == CUDA_LLM_SCALE_PER_TOKEN) {
-              const uint2 v = lds64(sc + (sub * 16 + 2 * g) * 4);
-              f_tok[x][0] *= __uint_as_float(v.x);
-              f_tok[x][1] *= __uint_as_float(v.y);
-            } else if (is_mx) {
+          for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-              for (int p = 0; p < D / 32; ++p) mx[x][p] = lds16(sc + p * a.page + sub * 16 + 2 * g);
-            } else {
-              const float* ks = reinterpret_cast<const float*>(a.ks);
-              const bool bad = (unsigned)blk[x] >= (unsigned)a.num_blocks;
-              const float f = a.scale_mode == CUDA_LLM_SCALE_PER_HEAD ? ks[h] : bad ? 0.f : ks[(size_t)blk[x] * a.Hkv + h];
-              f_tok[x][0] *= f;
-              f_tok[x][1] *= f;
+            for (int e = 0; e < 4; ++e) c[nt][0][e] += c[nt][1][e];
+            add_weights(0, c[nt][0], rp[nt]);
+          }
+        }
+      } else {
+        uint32_t af[U][D / 32][2][4];
+#pragma unroll
+        for (int x = 0; x < U; ++x)
+#pragma unroll
+          for (int p = 0; p < D / 32; ++p) {
+            load_key_block<KF>(key_at[x], ring_off + p * 32 * row_bytes, af[x][p]);
+            if (F8 && BF) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) af[x][p][e >> 2][e & 3] = pack_bf16x2(f16x2_lo(af[x][p][e >> 2][e & 3]), f16x2_hi(af[x][p][e >> 2][e & 3]));
             }
           }
-        }
-        return true;
-      };
-      bool loaded = false;
 #pragma unroll 1
-      for (int r0 = 0; r0 < rows || !loaded; r0 += ROWS) {
-        if (NT == 0 || h != cur_h || r0 != cur_r) {
-          cur_h = h;
-          cur_r = r0;
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          fetch_rows(r0);
 #pragma unroll
-          for (int nt = 0; nt < QN; ++nt) {
-            const int r = r0 + nt * 8 + g, j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
-            const size_t at = ((size_t)(q0 + j) * a.Hq + h * a.group + (r - j * a.group)) * D;
-            row_pair(a, r0 + nt * 8, rows, q0, n_q, ctx, h, t, rp[nt]);
-            if constexpr (SCALED) load_rows_scaled<D, QT, TERMS>(a.q, at, r < rows, t, qf[nt], rp[nt].inv);
-            else load_rows<D, QT>(a.q, at, r < rows, t, qf[nt]);
-          }
-        }
-        if (!loaded) {
-          loaded = true;
-          if (!load_tile()) {
-            *fail_ptr = 1;
-            return;
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < U; ++x) {
-          const int tok_a = tok0 + 16 * x + (F8 ? 2 * g : g), tok_b = tok0 + 16 * x + (F8 ? 2 * g + 1 : g + 8);
-#pragma unroll
-          for (int nt = 0; nt < QN; ++nt) {
+          for (int x = 0; x < U; ++x) {
             float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int p = 0; p < D / 32; ++p) {
-              float part[4] = {0.f, 0.f, 0.f, 0.f};
-              if (NT > 0 && TERMS == 2) {
-                mma_any<BF>(part, af[x][2 * p], qf[nt][TERMS - 1][p][0], qf[nt][TERMS - 1][p][1]);
-                mma_any<BF>(part, af[x][2 * p + 1], qf[nt][TERMS - 1][p][2], qf[nt][TERMS - 1][p][3]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) part[e] *= 1.f / 2048.f;
-              }
-#pragma unroll
-              for (int term = (NT > 0 ? 1 : TERMS) - 1; term >= 0; --term) {
-                mma_any<BF>(part, af[x][2 * p], qf[nt][term][p][0], qf[nt][term][p][1]);
-                mma_any<BF>(part, af[x][2 * p + 1], qf[nt][term][p][2], qf[nt][term][p][3]);
-              }
-              const float ea = is_mx ? e8m0_to_f32(mx[x][p] & 0xffu) : 1.f, eb = is_mx ? e8m0_to_f32(mx[x][p] >> 8) : 1.f;
-              c[0] = fmaf(part[0], ea, c[0]);
-              c[1] = fmaf(part[1], ea, c[1]);
-              c[2] = fmaf(part[2], eb, c[2]);
-              c[3] = fmaf(part[3], eb, c[3]);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              if (tok_a < rp[nt].limit[y]) sum[x][0] += fast_exp2(fmaf(c[y], f_tok[x][0] * rp[nt].inv[y], -rp[nt].lse2[y]));
-              if (tok_b < rp[nt].limit[y]) sum[x][1] += fast_exp2(fmaf(c[2 + y], f_tok[x][1] * rp[nt].inv[y], -rp[nt].lse2[y]));
-            }
+            for (int p = 0; p < D / 32; ++p) dot_block(c, af[x][p], qf[0], x, p);
+            add_weights(x, c, rp[0]);
           }
         }
       }
@@ -488,21 +533,27 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
           sum[x][e] += __shfl_xor_sync(0xffffffffu, sum[x][e], 1);
           sum[x][e] += __shfl_xor_sync(0xffffffffu, sum[x][e], 2);
         }
-        if (writes[x] && (unsigned)blk[x] < (unsigned)a.num_blocks) *sp[x] = fmaf(old[x], a.decay, (t & 1) ? sum[x][1] : sum[x][0]);
+        if (t < 2 && (live >> pg[x] & 1) && tok0 - tg0 * 16 + lane_tok + 16 * x < my_ctx)
+          my_sp[16 * x] = fmaf(my_old[x], a.decay, (t & 1) ? sum[x][1] : sum[x][0]);
       }
-    }
-    if (!waited && !tc_wait(full + 8 * st, (i / gm.n_stages) & 1)) {
+    } else if (!mbar_wait(full + 8 * st, par, 0)) {
       *fail_ptr = 1;
       return;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + 8 * st);
+    ring_off += gm.stage_bytes;
+    if (++st == gm.n_stages) {
+      st = 0;
+      ring_off = 0;
+      par ^= 1;
+    }
   }
 }
 
-template <int D, int KF, int QT, int NT>
+template <int D, int KF, int QT, int NT, bool MX>
 static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cudaStream_t st) {
-  auto kern = kv_weights_kernel<D, KF, QT, NT>;
+  auto kern = kv_weights_kernel<D, KF, QT, NT, MX>;
   const size_t smem = kWgtHeader + (size_t)gm.n_stages * gm.stage_bytes;
   static int configured[64] = {0};
   int dev = 0;
@@ -513,16 +564,23 @@ static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cud
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = 1;
   }
-  kern<<<grid, 32 * ((NT ? kWgtWarps : 8) + 1), smem, st>>>(a, gm);
+  kern<<<grid, 32 * ((NT ? kWgtWarps : kWgtWarps / 2) + 1), smem, st>>>(a, gm);
   return cudaGetLastError();
 }
 
 template <int D, int KF, int QT>
 static cudaError_t go_rows(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
-  if (nt == 1) return go<D, KF, QT, 1>(a, gm, grid, st);
+  if constexpr (KF == KF_E4M3)
+    if (a.scale_mode == CUDA_LLM_SCALE_MX_E8M0) {
+      if (nt == 1) return go<D, KF, QT, 1, true>(a, gm, grid, st);
+      if constexpr (QT != CUDA_LLM_F32)
+        if (nt == 2) return go<D, KF, QT, 2, true>(a, gm, grid, st);
+      return go<D, KF, QT, 0, true>(a, gm, grid, st);
+    }
+  if (nt == 1) return go<D, KF, QT, 1, false>(a, gm, grid, st);
   if constexpr (QT != CUDA_LLM_F32)
-    if (nt == 2) return go<D, KF, QT, 2>(a, gm, grid, st);
-  return go<D, KF, QT, 0>(a, gm, grid, st);
+    if (nt == 2) return go<D, KF, QT, 2, false>(a, gm, grid, st);
+  return go<D, KF, QT, 0, false>(a, gm, grid, st);
 }
 template <int D>
 static cudaError_t go_types(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
@@ -538,8 +596,7 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   // rows that stay in registers: 8, 16 (16-bit queries), or none
   const int nt = declared <= 8 ? 1 : declared <= 16 && a.q_dtype != CUDA_LLM_F32 ? 2 : 0;
   const int eb = a.k_format == CUDA_LLM_KV_FP8_E4M3 ? 1 : 2, groups = a.page / 16;
-  // units of a stage: 32 KB of K (head_dim 128); with streamed rows at least two token groups of a head
-  const int want = nt ? 16 / eb : 16;
+  const int want = kWgtWarps;  // 16-token units of a stage: one per warp, or two (streamed rows: groups of one head side by side)
   WeightsGeom gm;
   gm.hg = nt ? 8 : 4;
   while (a.Hkv % gm.hg || gm.hg * groups > want) gm.hg >>= 1;
