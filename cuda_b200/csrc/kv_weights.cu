@@ -26,7 +26,7 @@ struct WeightsArgs {
 // bulk copy per page: the heads of a page are contiguous) and their scales.  Its 16-token units, one head each, go to the
 // computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
 // ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
-constexpr int kWgtWarps = 16;         // 16-token units of a stage, and computing warps (half of them with two units each)
+constexpr int kWgtWarps = 8, kWgtUnits = 2 * kWgtWarps;  // computing warps; 16-token units of a stage, two per warp
 constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
 constexpr uint32_t kWgtHeader = 192 + 8 * kWgtSeqs + 64;  // barriers, page masks, flag, prefix sums, lengths: a multiple of 128
@@ -307,13 +307,12 @@ __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom&
 // One stage is one task per computing warp: head warp % hg of the group, a run of 16-token units.
 // NT > 0: the query fragments of 8 NT rows stay in registers from stage to stage (a decode step: all rows of a KV head); a
 // sequence with more rows than that is right but reloads them.
-// NT == 0: many rows per KV head (a window of a prompt): a warp holds the keys of two units and streams the rows from L2, eight
-// at a time.
+// NT == 0: many rows per KV head (a window of a prompt): the warp holds the keys and streams the rows from L2, eight at a time.
 template <int D, int KF, int QT, int NT, bool MX>
-__global__ void __launch_bounds__(32 * ((NT ? kWgtWarps : kWgtWarps / 2) + 1), 1)
+__global__ void __launch_bounds__(32 * (kWgtWarps + 1), 1)
 kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm) {
   constexpr bool F8 = KF == KF_E4M3;
-  constexpr int U = NT ? 1 : 2, WARPS = kWgtWarps / U, ROWS = NT ? 8 * NT : 8;
+  constexpr int U = 2, WARPS = kWgtWarps, ROWS = NT ? 8 * NT : 8;
   // operand type of the products: f16, unless the cache or (streamed rows) the queries are bf16 / fp32
   constexpr bool BF = KF == KF_BF16 || (NT == 0 && QT != CUDA_LLM_F16);
   constexpr bool SCALED = NT > 0 && F8 && QT != CUDA_LLM_F16;
@@ -487,20 +486,20 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
 #pragma unroll 1
         for (int r0 = 0; r0 < rows; r0 += ROWS) {
           if (r0 > 0) fetch_rows(r0);
-          float c[NT][2][4] = {};  // two chains of products
+          float c[U][NT][4] = {};
 #pragma unroll
-          for (int p = 0; p < D / 32; ++p) {
-            uint32_t af[2][4];
-            load_key_block<KF>(key_at[0], ring_off + p * 32 * row_bytes, af);
+          for (int p = 0; p < D / 32; ++p)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) dot_block(c[nt][p & 1], af, qf[nt], 0, p);
-          }
+            for (int x = 0; x < U; ++x) {
+              uint32_t af[2][4];
+              load_key_block<KF>(key_at[x], ring_off + p * 32 * row_bytes, af);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
+              for (int nt = 0; nt < NT; ++nt) dot_block(c[x][nt], af, qf[nt], x, p);
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[nt][0][e] += c[nt][1][e];
-            add_weights(0, c[nt][0], rp[nt]);
-          }
+          for (int x = 0; x < U; ++x)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) add_weights(x, c[x][nt], rp[nt]);
         }
       } else {
         uint32_t af[U][D / 32][2][4];
@@ -564,7 +563,7 @@ static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cud
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = 1;
   }
-  kern<<<grid, 32 * ((NT ? kWgtWarps : kWgtWarps / 2) + 1), smem, st>>>(a, gm);
+  kern<<<grid, 32 * (kWgtWarps + 1), smem, st>>>(a, gm);
   return cudaGetLastError();
 }
 
@@ -596,9 +595,9 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   // rows that stay in registers: 8, 16 (16-bit queries), or none
   const int nt = declared <= 8 ? 1 : declared <= 16 && a.q_dtype != CUDA_LLM_F32 ? 2 : 0;
   const int eb = a.k_format == CUDA_LLM_KV_FP8_E4M3 ? 1 : 2, groups = a.page / 16;
-  const int want = kWgtWarps;  // 16-token units of a stage: one per warp, or two (streamed rows: groups of one head side by side)
+  const int want = kWgtUnits;  // two units of a warp are 16-token groups side by side of one head: at most 8 heads
   WeightsGeom gm;
-  gm.hg = nt ? 8 : 4;
+  gm.hg = 8;
   while (a.Hkv % gm.hg || gm.hg * groups > want) gm.hg >>= 1;
   gm.n_hg = a.Hkv / gm.hg;
   gm.pages = want / (gm.hg * groups);
