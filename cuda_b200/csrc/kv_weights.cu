@@ -26,7 +26,7 @@ struct WeightsArgs {
 // bulk copy per page: the heads of a page are contiguous) and their scales.  Its 16-token units, one head each, go to the
 // computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
 // ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
-constexpr int kWgtWarps = 8, kWgtUnits = 2 * kWgtWarps;  // computing warps; 16-token units of a stage, two per warp
+constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each
 constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
 constexpr uint32_t kWgtHeader = 192 + 8 * kWgtSeqs + 64;  // barriers, page masks, flag, prefix sums, lengths: a multiple of 128
@@ -74,14 +74,14 @@ __device__ __forceinline__ void row_pair(const WeightsArgs& a, int r0, int rows,
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int r = r0 + 2 * t + x;  // the lane's two columns
-    rp.lse2[x] = 0.f;
+    rp.lse2[x] = __builtin_huge_valf();  // no such row, or a row that saw nothing: weights of zero
     rp.inv[x] = 1.f;
     rp.limit[x] = 0;
     if (r < rows) {
       const int j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
       const float v = a.lse[(size_t)(q0 + j) * a.Hq + h * a.group + (r - j * a.group)];
-      rp.lse2[x] = v * 1.4426950408889634f;
-      rp.limit[x] = v == -__builtin_huge_valf() ? 0 : a.causal ? ctx - n_q + 1 + j : ctx;
+      if (v != -__builtin_huge_valf()) rp.lse2[x] = v * 1.4426950408889634f;
+      rp.limit[x] = a.causal ? ctx - n_q + 1 + j : ctx;
     }
   }
 }
@@ -304,15 +304,20 @@ __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom&
   }
 }
 
+// Four units per warp and stage share more of what a stage costs a warp, where three such stages fit and the fragments leave
+// registers: 8-bit caches, or 16-bit ones of head_dim 64.
+template <int D, int KF, int QT>
+constexpr bool kFourUnits = QT != CUDA_LLM_F32 && (KF == KF_E4M3 || D == 64);
+
 // One stage is one task per computing warp: head warp % hg of the group, a run of 16-token units.
 // NT > 0: the query fragments of 8 NT rows stay in registers from stage to stage (a decode step: all rows of a KV head); a
 // sequence with more rows than that is right but reloads them.
 // NT == 0: many rows per KV head (a window of a prompt): the warp holds the keys and streams the rows from L2, eight at a time.
-template <int D, int KF, int QT, int NT, bool MX>
+template <int D, int KF, int QT, int NT, bool MX, int U>
 __global__ void __launch_bounds__(32 * (kWgtWarps + 1), 1)
 kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm) {
   constexpr bool F8 = KF == KF_E4M3;
-  constexpr int U = 2, WARPS = kWgtWarps, ROWS = NT ? 8 * NT : 8;
+  constexpr int WARPS = kWgtWarps, ROWS = NT ? 8 * NT : 8;
   // operand type of the products: f16, unless the cache or (streamed rows) the queries are bf16 / fp32
   constexpr bool BF = KF == KF_BF16 || (NT == 0 && QT != CUDA_LLM_F16);
   constexpr bool SCALED = NT > 0 && F8 && QT != CUDA_LLM_F16;
@@ -344,13 +349,13 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   const int groups = a.page >> 4;  // 16-token groups of a page
   const int hl = warp & (gm.hg - 1), tg0 = warp / gm.hg * U, pg0 = tg0 / groups, sub0 = tg0 % groups;
   const uint32_t row_bytes = a.page * (F8 ? 1 : 2);
-  // this lane's places in a stage: rows for ldmatrix, scales, page bit; unit 1 is the next group of the same or the next page
+  // this lane's places in a stage: rows for ldmatrix, scales, page bit; a warp's units are neighbouring groups of one head
   uint32_t key_at[U][2], scale_at[U];
   int pg[U];
 #pragma unroll
   for (int x = 0; x < U; ++x) {
-    const int sub = sub0 + x < groups ? sub0 + x : 0;
-    pg[x] = sub0 + x < groups ? pg0 : pg0 + 1;
+    const int sub = (sub0 + x) % groups;
+    pg[x] = pg0 + (sub0 + x) / groups;
     const uint32_t slab = ring + pg[x] * gm.k_bytes + hl * gm.k_head + sub * (F8 ? 16 : 32);
     key_at[x][0] = slab + key_row<KF>(lane, row_bytes, 0);
     key_at[x][1] = slab + key_row<KF>(lane, row_bytes, 1);
@@ -361,32 +366,37 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   RowPair rp[QN];
 
   // the task one stage ahead: where it is, and its old scores, on their way while the stage in hand is worked on
-  int s = pl.s0, ctx = 0, per = 1, hgi = 0, u = -1, q0 = 0, n_q = 0, seq = -1;
+  int s = pl.s0, ctx = 0, per = 1, hgi = 0, u = 0, left = 0, q0 = 0, n_q = 0, seq = -1, no_old = 0;
   float* sp = nullptr;
   float old[U];
   auto locate = [&](int w) {
-    while (w >= pl.pre[s + 1]) ++s;
-    if (s != seq) {
-      seq = s;
-      ctx = pl.lens[s];
-      per = (pl.pre[s + 1] - pl.pre[s]) / gm.n_hg;
+    if (left == 0) {  // another sequence or head group
+      while (w >= pl.pre[s + 1]) ++s;
+      if (s != seq) {
+        seq = s;
+        ctx = pl.lens[s];
+        per = (pl.pre[s + 1] - pl.pre[s]) / gm.n_hg;
+        q0 = a.cuq ? a.cuq[s] : a.q_first + s;
+        const int q1 = a.cuq ? a.cuq[s + 1] : q0 + 1;
+        n_q = q1 - q0;
+        if (q0 < 0 || q1 < q0 || q1 > a.total_q) {
+          if (a.status && lane == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_QLEN);
+          q0 = n_q = 0;
+        }
+        no_old = (t < 2 && a.decay != 0.f) ? ctx - n_q : 0;  // scores from here on start at zero
+      }
       hgi = (w - pl.pre[s]) / per;
       u = w - pl.pre[s] - hgi * per;
-      q0 = a.cuq ? a.cuq[s] : a.q_first + s;
-      const int q1 = a.cuq ? a.cuq[s + 1] : q0 + 1;
-      n_q = q1 - q0;
-      if (q0 < 0 || q1 < q0 || q1 > a.total_q) {
-        if (a.status && lane == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_QLEN);
-        q0 = n_q = 0;
-      }
-    } else if (++u == per) {
-      u = 0;
-      ++hgi;
+      left = per - u;
+      sp = a.scores + s * a.st_seq + (hgi * gm.hg + hl) * a.st_head + u * gm.tok_stage + lane_tok;
+    } else {
+      ++u;
+      sp += gm.tok_stage;
     }
+    --left;
     const int tok = u * gm.tok_stage + lane_tok;
-    sp = a.scores + s * a.st_seq + (hgi * gm.hg + hl) * a.st_head + tok;
 #pragma unroll
-    for (int x = 0; x < U; ++x) old[x] = (t < 2 && a.decay != 0.f && tok + 16 * x < ctx - n_q) ? sp[16 * x] : 0.f;
+    for (int x = 0; x < U; ++x) old[x] = tok + 16 * x < no_old ? sp[16 * x] : 0.f;
   };
   locate(pl.w0);
   int cur_s = -1, cur_h = -1, cur_r = -1, st = 0;
@@ -399,6 +409,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
     for (int x = 0; x < U; ++x) my_old[x] = old[x];
     if (w + 1 < pl.w1) locate(w + 1);
     if (tok0 < my_ctx) {
+      const bool edge = tok0 + 16 * U > my_ctx - my_nq;  // some row may not see some token
       auto fetch_rows = [&](int r0) {
         cur_s = my_s;
         cur_h = h;
@@ -449,8 +460,8 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const float wa = fast_exp2(fmaf(c[y], f_tok[x][0] * r.inv[y], -r.lse2[y])), wb = fast_exp2(fmaf(c[2 + y], f_tok[x][1] * r.inv[y], -r.lse2[y]));
-          sum[x][0] += tok_a < r.limit[y] ? wa : 0.f;
-          sum[x][1] += tok_b < r.limit[y] ? wb : 0.f;
+          sum[x][0] += !edge || tok_a < r.limit[y] ? wa : 0.f;
+          sum[x][1] += !edge || tok_b < r.limit[y] ? wb : 0.f;
         }
       };
       // c += K block p of one unit times the rows of one 8-column block
@@ -550,9 +561,9 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   }
 }
 
-template <int D, int KF, int QT, int NT, bool MX>
+template <int D, int KF, int QT, int NT, bool MX, int U>
 static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cudaStream_t st) {
-  auto kern = kv_weights_kernel<D, KF, QT, NT, MX>;
+  auto kern = kv_weights_kernel<D, KF, QT, NT, MX, U>;
   const size_t smem = kWgtHeader + (size_t)gm.n_stages * gm.stage_bytes;
   static int configured[64] = {0};
   int dev = 0;
@@ -567,27 +578,28 @@ static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cud
   return cudaGetLastError();
 }
 
-template <int D, int KF, int QT>
+template <int D, int KF, int QT, bool MX>
 static cudaError_t go_rows(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
-  if constexpr (KF == KF_E4M3)
-    if (a.scale_mode == CUDA_LLM_SCALE_MX_E8M0) {
-      if (nt == 1) return go<D, KF, QT, 1, true>(a, gm, grid, st);
-      if constexpr (QT != CUDA_LLM_F32)
-        if (nt == 2) return go<D, KF, QT, 2, true>(a, gm, grid, st);
-      return go<D, KF, QT, 0, true>(a, gm, grid, st);
-    }
-  if (nt == 1) return go<D, KF, QT, 1, false>(a, gm, grid, st);
+  if constexpr (kFourUnits<D, KF, QT>)
+    if (nt == 1 && gm.units == 4 * kWgtWarps) return go<D, KF, QT, 1, MX, 4>(a, gm, grid, st);
+  if (nt == 1) return go<D, KF, QT, 1, MX, 2>(a, gm, grid, st);
   if constexpr (QT != CUDA_LLM_F32)
-    if (nt == 2) return go<D, KF, QT, 2, false>(a, gm, grid, st);
-  return go<D, KF, QT, 0, false>(a, gm, grid, st);
+    if (nt == 2) return go<D, KF, QT, 2, MX, 2>(a, gm, grid, st);
+  return go<D, KF, QT, 0, MX, 2>(a, gm, grid, st);
+}
+template <int D, int KF, int QT>
+static cudaError_t go_scales(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
+  if constexpr (KF == KF_E4M3)
+    if (a.scale_mode == CUDA_LLM_SCALE_MX_E8M0) return go_rows<D, KF, QT, true>(a, gm, grid, nt, st);
+  return go_rows<D, KF, QT, false>(a, gm, grid, nt, st);
 }
 template <int D>
 static cudaError_t go_types(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
-  if (a.k_format == CUDA_LLM_KV_F16) return go_rows<D, KF_F16, CUDA_LLM_F16>(a, gm, grid, nt, st);
-  if (a.k_format == CUDA_LLM_KV_BF16) return go_rows<D, KF_BF16, CUDA_LLM_BF16>(a, gm, grid, nt, st);
-  if (a.q_dtype == CUDA_LLM_F32) return go_rows<D, KF_E4M3, CUDA_LLM_F32>(a, gm, grid, nt, st);
-  if (a.q_dtype == CUDA_LLM_F16) return go_rows<D, KF_E4M3, CUDA_LLM_F16>(a, gm, grid, nt, st);
-  return go_rows<D, KF_E4M3, CUDA_LLM_BF16>(a, gm, grid, nt, st);
+  if (a.k_format == CUDA_LLM_KV_F16) return go_scales<D, KF_F16, CUDA_LLM_F16>(a, gm, grid, nt, st);
+  if (a.k_format == CUDA_LLM_KV_BF16) return go_scales<D, KF_BF16, CUDA_LLM_BF16>(a, gm, grid, nt, st);
+  if (a.q_dtype == CUDA_LLM_F32) return go_scales<D, KF_E4M3, CUDA_LLM_F32>(a, gm, grid, nt, st);
+  if (a.q_dtype == CUDA_LLM_F16) return go_scales<D, KF_E4M3, CUDA_LLM_F16>(a, gm, grid, nt, st);
+  return go_scales<D, KF_E4M3, CUDA_LLM_BF16>(a, gm, grid, nt, st);
 }
 
 static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cudaStream_t st) {
@@ -595,7 +607,10 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   // rows that stay in registers: 8, 16 (16-bit queries), or none
   const int nt = declared <= 8 ? 1 : declared <= 16 && a.q_dtype != CUDA_LLM_F32 ? 2 : 0;
   const int eb = a.k_format == CUDA_LLM_KV_FP8_E4M3 ? 1 : 2, groups = a.page / 16;
-  const int want = kWgtUnits;  // two units of a warp are 16-token groups side by side of one head: at most 8 heads
+  const long long cap = (long long)a.max_blocks * a.page < a.max_tokens ? (long long)a.max_blocks * a.page : a.max_tokens;
+  // units of a stage; the larger stage only where there are stages for every SM a few times over
+  const bool four = nt == 1 && a.q_dtype != CUDA_LLM_F32 && (eb == 1 || a.D == 64) && cap * a.Hkv * a.S / 16 >= 4ll * 4 * kWgtWarps * sms;
+  const int want = (four ? 4 : 2) * kWgtWarps;
   WeightsGeom gm;
   gm.hg = 8;
   while (a.Hkv % gm.hg || gm.hg * groups > want) gm.hg >>= 1;
@@ -611,7 +626,6 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   gm.stage_bytes = ((gm.k_bytes + gm.s_bytes) * gm.pages + 127) / 128 * 128;
   gm.n_stages = (int)((kWgtBudget - kWgtHeader) / gm.stage_bytes);
   if (gm.n_stages > kWgtMaxStages) gm.n_stages = kWgtMaxStages;
-  const long long cap = (long long)a.max_blocks * a.page < a.max_tokens ? (long long)a.max_blocks * a.page : a.max_tokens;
   a.group_shift = (a.group & (a.group - 1)) ? -1 : __builtin_ctz(a.group);
   const int S = a.S;
   for (int s0 = 0; s0 < S; s0 += kWgtSeqs) {
