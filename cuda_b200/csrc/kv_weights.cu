@@ -29,15 +29,31 @@ struct WeightsArgs {
 constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each
 constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
-constexpr uint32_t kWgtHeader = 192 + 8 * kWgtSeqs + 64;  // barriers, page masks, flag, prefix sums, lengths: a multiple of 128
+constexpr uint32_t kWgtHeader = 9 * 1024;  // barriers, page masks, flag, prefix sums, lengths
+static_assert(192 + 4 * (2 * kWgtSeqs + 4) <= kWgtHeader, "header");
+constexpr int kWgtRows = 128;         // query rows of a KV head kept in shared memory
 constexpr uint32_t kWgtBudget = 224 * 1024;
 
 struct WeightsGeom {
   int hg, n_hg, pages, tok_stage, units;   // pages, tokens and units (head x 16 tokens) of a stage
   int n_stages;
+  int box_rows;                            // pages as swizzled TMA boxes of this many head_dim rows; 0: as bulk copies
+  uint32_t q_off, smem;                    // where streamed rows are kept in shared memory; bytes of it in all
   uint32_t k_head, s_head;                 // bytes of one head of one page, K / scales
   uint32_t k_bytes, s_bytes, stage_bytes;  // of the head group of one page; of a stage
 };
+
+// Pages with rows of 64 or 128 bytes arrive as TMA boxes with the swizzle of that width, which spreads the eight rows of an
+// ldmatrix over all banks; shorter rows do that by themselves (16 bytes) or conflict in pairs (32).
+struct alignas(64) WeightsMap {
+  CUtensorMap k;  // [num_blocks][Hkv * D][page]
+};
+__device__ __forceinline__ void tma_box_3d(uint32_t dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
 
 // B fragments of mma.m16n8k16 for 8 query rows: lane (g, t) holds 8 consecutive elements of every 32 of row g, d = 32 p + 8 t ..
 // 8 t + 7.  Word w of them meets matrix (w - t) & 3 of the ldmatrix below, which for lane t brings K at d = 32 p + 8 t +
@@ -120,12 +136,19 @@ __device__ __forceinline__ void load_rows(const void* q, size_t at, bool live, i
 
 // K fragments of 16 tokens and 32 elements of head_dim (two k-steps): E4M3 codes widened to f16 (exact), or 16-bit elements as
 // they are.  `at` comes from key_row().  Rows of the result: tokens 2g and 2g + 1 (8 bit) or g and g + 8 (16 bit).
+// `chunk`: which 16 bytes of a row hold the unit's tokens (its first 8 tokens, 16 bit).
 template <int KF>
-__device__ __forceinline__ uint32_t key_row(int lane, uint32_t row_bytes, int x) {
+__device__ __forceinline__ uint32_t key_row(int lane, uint32_t row_bytes, int chunk, int x) {
   const int m = lane >> 3, i = lane & 7;
-  if (KF == KF_E4M3) return (8 * (i >> 1) + 2 * ((m + (i >> 1)) & 3) + (i & 1)) * row_bytes;
-  // matrices of k-step x: (tokens 0..7, 8..15) x (first, second pair of elements)
-  return (8 * (i >> 1) + 2 * ((2 * x + (m >> 1) + (i >> 1)) & 3) + (i & 1)) * row_bytes + (m & 1) * 16;
+  uint32_t row;
+  if (KF == KF_E4M3) {
+    row = 8 * (i >> 1) + 2 * ((m + (i >> 1)) & 3) + (i & 1);
+  } else {  // matrices of k-step x: (tokens 0..7, 8..15) x (first, second pair of elements)
+    row = 8 * (i >> 1) + 2 * ((2 * x + (m >> 1) + (i >> 1)) & 3) + (i & 1);
+    chunk += m & 1;
+  }
+  const uint32_t swizzle = row_bytes == 128 ? row & 7 : row_bytes == 64 ? (row >> 1) & 3 : 0;
+  return row * row_bytes + ((chunk ^ swizzle) << 4);
 }
 template <int KF>
 __device__ __forceinline__ void load_key_block(const uint32_t (&at)[2], uint32_t offset, uint32_t (&af)[2][4]) {
@@ -241,7 +264,7 @@ __device__ __forceinline__ WeightsPlan make_plan(const WeightsArgs& a, const Wei
 
 // Producer warp: lane 0 issues the copies; the block-table entries of the next 32 / pages stages are fetched by all lanes.
 // Beside a stage lies a mask of the pages that were copied (bad block-table entries are not).
-__device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom& gm, const WeightsPlan& pl, uint32_t full, uint32_t empty, uint32_t live_at,
+__device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, const WeightsPlan& pl, uint32_t full, uint32_t empty, uint32_t live_at,
                                         uint32_t ring, volatile int* fail_ptr) {
   const int lane = threadIdx.x & 31, batch = 32 / gm.pages, pg_mask = gm.pages - 1, pg_shift = __popc(pg_mask);
   bool ok = true;
@@ -288,7 +311,13 @@ __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom&
         const int pg = lane & pg_mask;
         const size_t slab = (size_t)mine * a.Hkv + h0;
         const uint32_t to = ring + st * gm.stage_bytes;
-        bulk_g2s(to + pg * gm.k_bytes, a.kc + slab * gm.k_head, gm.k_bytes, full + 8 * st);
+        if (gm.box_rows) {
+          const int rows = gm.hg * a.D;
+          for (int r = 0; r < rows; r += gm.box_rows)
+            tma_box_3d(to + pg * gm.k_bytes + r * (gm.k_head / a.D), &map.k, 0, h0 * a.D + r, mine, full + 8 * st);
+        } else {
+          bulk_g2s(to + pg * gm.k_bytes, a.kc + slab * gm.k_head, gm.k_bytes, full + 8 * st);
+        }
         if (gm.s_bytes) bulk_g2s(to + gm.pages * gm.k_bytes + pg * gm.s_bytes, a.ks + slab * gm.s_head, gm.s_bytes, full + 8 * st);
       }
       if (++st == gm.n_stages) {
@@ -315,7 +344,7 @@ constexpr bool kFourUnits = QT != CUDA_LLM_F32 && (KF == KF_E4M3 || D == 64);
 // NT == 0: many rows per KV head (a window of a prompt): the warp holds the keys and streams the rows from L2, eight at a time.
 template <int D, int KF, int QT, int NT, bool MX, int U>
 __global__ void __launch_bounds__(32 * (kWgtWarps + 1), 1)
-kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm) {
+kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm, const __grid_constant__ WeightsMap map) {
   constexpr bool F8 = KF == KF_E4M3;
   constexpr int WARPS = kWgtWarps, ROWS = NT ? 8 * NT : 8;
   // operand type of the products: f16, unless the cache or (streamed rows) the queries are bf16 / fp32
@@ -323,7 +352,12 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   constexpr bool SCALED = NT > 0 && F8 && QT != CUDA_LLM_F16;
   constexpr int TERMS = QT != CUDA_LLM_F32 ? 1 : NT ? 2 : 3;  // of an fp32 query: f16 hi + lo, or three bf16
   constexpr int QN = NT ? NT : 1;
-  extern __shared__ __align__(128) uint8_t smem[];
+  // Block scales of streamed rows go into the keys: bf16 holds code x 2^(block exponent - the token's largest) exactly down to
+  // 2^-117 of the largest block; the largest exponent scales the whole dot product.
+  constexpr bool FOLD = MX && NT == 0 && BF;
+  constexpr bool KEPT = NT == 0 && QT != CUDA_LLM_F32;  // up to kWgtRows streamed rows lie in shared memory
+  constexpr int QCH = D / 8;                            // 16-byte chunks of a row there
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t full = base, empty = base + 8 * kWgtMaxStages, live_at = base + 128, ring = base + kWgtHeader;
   int* pre = reinterpret_cast<int*>(smem + 192);  // [S + 1] stages before each sequence
@@ -341,7 +375,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   const WeightsPlan pl = make_plan<32 * (WARPS + 1)>(a, gm, pre, lens);
   if (pl.w0 >= pl.w1) return;
   if (warp == WARPS) {
-    produce(a, gm, pl, full, empty, live_at, ring, fail_ptr);
+    produce(a, gm, map, pl, full, empty, live_at, ring, fail_ptr);
     return;
   }
 
@@ -356,9 +390,9 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   for (int x = 0; x < U; ++x) {
     const int sub = (sub0 + x) % groups;
     pg[x] = pg0 + (sub0 + x) / groups;
-    const uint32_t slab = ring + pg[x] * gm.k_bytes + hl * gm.k_head + sub * (F8 ? 16 : 32);
-    key_at[x][0] = slab + key_row<KF>(lane, row_bytes, 0);
-    key_at[x][1] = slab + key_row<KF>(lane, row_bytes, 1);
+    const uint32_t slab = ring + pg[x] * gm.k_bytes + hl * gm.k_head;
+    key_at[x][0] = slab + key_row<KF>(lane, row_bytes, sub * (F8 ? 1 : 2), 0);
+    key_at[x][1] = slab + key_row<KF>(lane, row_bytes, sub * (F8 ? 1 : 2), 1);
     scale_at[x] = ring + gm.pages * gm.k_bytes + pg[x] * gm.s_bytes + hl * gm.s_head + (sub * 16 + 2 * g) * (MX ? 1 : 4);
   }
   const int lane_tok = tg0 * 16 + (F8 ? 2 * g + (t & 1) : g + 8 * (t & 1));  // lanes t = 0, 1 keep the scores of two tokens of a unit
@@ -401,6 +435,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
   locate(pl.w0);
   int cur_s = -1, cur_h = -1, cur_r = -1, st = 0;
   uint32_t par = 0, ring_off = 0;
+  bool dead = false;
   for (int w = pl.w0; w < pl.w1; ++w) {
     const int my_s = s, h = hgi * gm.hg + hl, tok0 = u * gm.tok_stage + tg0 * 16, my_ctx = ctx, my_q0 = q0, my_nq = n_q, rows = n_q * a.group;
     float* const my_sp = sp;
@@ -408,7 +443,34 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
 #pragma unroll
     for (int x = 0; x < U; ++x) my_old[x] = old[x];
     if (w + 1 < pl.w1) locate(w + 1);
-    if (tok0 < my_ctx) {
+    if (KEPT && rows <= kWgtRows && (my_s != cur_s || h != cur_h)) {
+      // another sequence or head (of all warps alike): its rows, words already rotated for the lanes that will read them, and
+      // {log-sum-exp, first token not seen} of every row
+      cur_s = my_s;
+      cur_h = h;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      for (int e = tid; e < ((rows + 7) & ~7) * QCH; e += 32 * WARPS) {
+        const int r = e / QCH, c = e % QCH, j = r / a.group;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows)
+          v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + ((size_t)(my_q0 + j) * a.Hq + h * a.group + (r - j * a.group)) * D + c * 8);
+        uint32_t x[4] = {v.x, v.y, v.z, v.w};
+        rotate_words(x, c & 3);
+        sts128(base + gm.q_off + (r * QCH + (c ^ ((r & 1) << 2))) * 16, x[0], x[1], x[2], x[3]);
+      }
+      for (int r = tid; r < ((rows + 7) & ~7); r += 32 * WARPS) {
+        RowPair x;
+        row_pair(a, r, rows, my_q0, my_nq, my_ctx, h, 0, x);
+        sts32(base + gm.q_off + kWgtRows * QCH * 16 + r * 8, __float_as_int(x.lse2[0]));
+        sts32(base + gm.q_off + kWgtRows * QCH * 16 + r * 8 + 4, x.limit[0]);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (!dead && !mbar_wait(full + 8 * st, par, 0)) {  // the warp goes on without work: others may wait for it at the barrier above
+      dead = true;
+      *fail_ptr = 1;
+    }
+    if (tok0 < my_ctx && !dead) {
       const bool edge = tok0 + 16 * U > my_ctx - my_nq;  // some row may not see some token
       auto fetch_rows = [&](int r0) {
         cur_s = my_s;
@@ -424,10 +486,6 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
         }
       };
       if (NT > 0 && (my_s != cur_s || h != cur_h || cur_r != 0)) fetch_rows(0);
-      if (!mbar_wait(full + 8 * st, par, 0)) {
-        *fail_ptr = 1;
-        return;
-      }
       const uint32_t live = lds32(live_at + 4 * st);
       float f_tok[U][2], sum[U][2];
       uint32_t mx[U][MX ? D / 32 : 1];
@@ -438,6 +496,19 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
         if (MX) {
 #pragma unroll
           for (int p = 0; p < D / 32; ++p) mx[x][p] = lds16(scale_at[x] + ring_off + p * a.page);
+          if (FOLD) {
+            uint32_t ea = 0, eb = 0;
+#pragma unroll
+            for (int p = 0; p < D / 32; ++p) {
+              ea = max(ea, mx[x][p] & 0xffu);
+              eb = max(eb, mx[x][p] >> 8);
+            }
+            f_tok[x][0] *= e8m0_to_f32(ea);
+            f_tok[x][1] *= e8m0_to_f32(eb);
+#pragma unroll
+            for (int p = 0; p < D / 32; ++p)  // biased exponents of 2^(block - largest), 0 (a factor of zero) below 2^-126
+              mx[x][p] = (uint32_t)max(0, 127 + (int)(mx[x][p] & 0xffu) - (int)ea) | (uint32_t)max(0, 127 + (int)(mx[x][p] >> 8) - (int)eb) << 8;
+          }
         } else if (F8) {
           float fa, fb;
           if (a.scale_mode == CUDA_LLM_SCALE_PER_TOKEN) {
@@ -467,7 +538,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
       // c += K block p of one unit times the rows of one 8-column block
       auto dot_block = [&](float (&c)[4], const uint32_t (&af)[2][4], const uint32_t (&q)[TERMS][D / 32][4], int x, int p) {
         float part[4] = {0.f, 0.f, 0.f, 0.f};
-        if (!MX && !(NT > 0 && TERMS == 2)) {
+        if ((!MX || FOLD) && !(NT > 0 && TERMS == 2)) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) part[e] = c[e];
         }
@@ -482,7 +553,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
           mma_any<BF>(part, af[0], q[term][p][0], q[term][p][1]);
           mma_any<BF>(part, af[1], q[term][p][2], q[term][p][3]);
         }
-        if (MX) {
+        if (MX && !FOLD) {
           const float ea = e8m0_to_f32(mx[x][p] & 0xffu), eb = e8m0_to_f32(mx[x][p] >> 8);
           c[0] = fmaf(part[0], ea, c[0]);
           c[1] = fmaf(part[1], ea, c[1]);
@@ -521,18 +592,37 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
             load_key_block<KF>(key_at[x], ring_off + p * 32 * row_bytes, af[x][p]);
             if (F8 && BF) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) af[x][p][e >> 2][e & 3] = pack_bf16x2(f16x2_lo(af[x][p][e >> 2][e & 3]), f16x2_hi(af[x][p][e >> 2][e & 3]));
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t v = af[x][p][e >> 2][e & 3];
+                const float up = !FOLD ? 1.f : __uint_as_float((e & 1 ? mx[x][p] >> 8 : mx[x][p] & 0xffu) << 23);
+                af[x][p][e >> 2][e & 3] = pack_bf16x2(f16x2_lo(v) * up, f16x2_hi(v) * up);
+              }
             }
           }
 #pragma unroll 1
         for (int r0 = 0; r0 < rows; r0 += 8) {
-          fetch_rows(r0);
+          if (KEPT && rows <= kWgtRows) {
+            const uint32_t row_at = base + gm.q_off + (r0 + g) * QCH * 16;
+#pragma unroll
+            for (int p = 0; p < D / 32; ++p) {
+              const uint4 v = lds128(row_at + (((p * 4 + t) ^ ((g & 1) << 2)) << 4));
+              qf[0][0][p][0] = v.x; qf[0][0][p][1] = v.y; qf[0][0][p][2] = v.z; qf[0][0][p][3] = v.w;
+            }
+            const uint4 v = lds128(base + gm.q_off + kWgtRows * QCH * 16 + (r0 + 2 * t) * 8);
+            rp[0].lse2[0] = __uint_as_float(v.x); rp[0].limit[0] = (int)v.y;
+            rp[0].lse2[1] = __uint_as_float(v.z); rp[0].limit[1] = (int)v.w;
+            rp[0].inv[0] = rp[0].inv[1] = 1.f;
+          } else {
+            fetch_rows(r0);
+          }
 #pragma unroll
           for (int x = 0; x < U; ++x) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            float c[2][4] = {};  // two chains of products
 #pragma unroll
-            for (int p = 0; p < D / 32; ++p) dot_block(c, af[x][p], qf[0], x, p);
-            add_weights(x, c, rp[0]);
+            for (int p = 0; p < D / 32; ++p) dot_block(c[p & 1], af[x][p], qf[0], x, p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[0][e] += c[1][e];
+            add_weights(x, c[0], rp[0]);
           }
         }
       }
@@ -546,9 +636,6 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
         if (t < 2 && (live >> pg[x] & 1) && tok0 - tg0 * 16 + lane_tok + 16 * x < my_ctx)
           my_sp[16 * x] = fmaf(my_old[x], a.decay, (t & 1) ? sum[x][1] : sum[x][0]);
       }
-    } else if (!mbar_wait(full + 8 * st, par, 0)) {
-      *fail_ptr = 1;
-      return;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + 8 * st);
@@ -562,9 +649,8 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
 }
 
 template <int D, int KF, int QT, int NT, bool MX, int U>
-static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cudaStream_t st) {
+static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, int grid, cudaStream_t st) {
   auto kern = kv_weights_kernel<D, KF, QT, NT, MX, U>;
-  const size_t smem = kWgtHeader + (size_t)gm.n_stages * gm.stage_bytes;
   static int configured[64] = {0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -574,32 +660,32 @@ static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, int grid, cud
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = 1;
   }
-  kern<<<grid, 32 * (kWgtWarps + 1), smem, st>>>(a, gm);
+  kern<<<grid, 32 * (kWgtWarps + 1), gm.smem, st>>>(a, gm, map);
   return cudaGetLastError();
 }
 
 template <int D, int KF, int QT, bool MX>
-static cudaError_t go_rows(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
+static cudaError_t go_rows(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, int grid, int nt, cudaStream_t st) {
   if constexpr (kFourUnits<D, KF, QT>)
-    if (nt == 1 && gm.units == 4 * kWgtWarps) return go<D, KF, QT, 1, MX, 4>(a, gm, grid, st);
-  if (nt == 1) return go<D, KF, QT, 1, MX, 2>(a, gm, grid, st);
+    if (nt == 1 && gm.units == 4 * kWgtWarps) return go<D, KF, QT, 1, MX, 4>(a, gm, map, grid, st);
+  if (nt == 1) return go<D, KF, QT, 1, MX, 2>(a, gm, map, grid, st);
   if constexpr (QT != CUDA_LLM_F32)
-    if (nt == 2) return go<D, KF, QT, 2, MX, 2>(a, gm, grid, st);
-  return go<D, KF, QT, 0, MX, 2>(a, gm, grid, st);
+    if (nt == 2) return go<D, KF, QT, 2, MX, 2>(a, gm, map, grid, st);
+  return go<D, KF, QT, 0, MX, 2>(a, gm, map, grid, st);
 }
 template <int D, int KF, int QT>
-static cudaError_t go_scales(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
+static cudaError_t go_scales(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, int grid, int nt, cudaStream_t st) {
   if constexpr (KF == KF_E4M3)
-    if (a.scale_mode == CUDA_LLM_SCALE_MX_E8M0) return go_rows<D, KF, QT, true>(a, gm, grid, nt, st);
-  return go_rows<D, KF, QT, false>(a, gm, grid, nt, st);
+    if (a.scale_mode == CUDA_LLM_SCALE_MX_E8M0) return go_rows<D, KF, QT, true>(a, gm, map, grid, nt, st);
+  return go_rows<D, KF, QT, false>(a, gm, map, grid, nt, st);
 }
 template <int D>
-static cudaError_t go_types(const WeightsArgs& a, const WeightsGeom& gm, int grid, int nt, cudaStream_t st) {
-  if (a.k_format == CUDA_LLM_KV_F16) return go_scales<D, KF_F16, CUDA_LLM_F16>(a, gm, grid, nt, st);
-  if (a.k_format == CUDA_LLM_KV_BF16) return go_scales<D, KF_BF16, CUDA_LLM_BF16>(a, gm, grid, nt, st);
-  if (a.q_dtype == CUDA_LLM_F32) return go_scales<D, KF_E4M3, CUDA_LLM_F32>(a, gm, grid, nt, st);
-  if (a.q_dtype == CUDA_LLM_F16) return go_scales<D, KF_E4M3, CUDA_LLM_F16>(a, gm, grid, nt, st);
-  return go_scales<D, KF_E4M3, CUDA_LLM_BF16>(a, gm, grid, nt, st);
+static cudaError_t go_types(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, int grid, int nt, cudaStream_t st) {
+  if (a.k_format == CUDA_LLM_KV_F16) return go_scales<D, KF_F16, CUDA_LLM_F16>(a, gm, map, grid, nt, st);
+  if (a.k_format == CUDA_LLM_KV_BF16) return go_scales<D, KF_BF16, CUDA_LLM_BF16>(a, gm, map, grid, nt, st);
+  if (a.q_dtype == CUDA_LLM_F32) return go_scales<D, KF_E4M3, CUDA_LLM_F32>(a, gm, map, grid, nt, st);
+  if (a.q_dtype == CUDA_LLM_F16) return go_scales<D, KF_E4M3, CUDA_LLM_F16>(a, gm, map, grid, nt, st);
+  return go_scales<D, KF_E4M3, CUDA_LLM_BF16>(a, gm, map, grid, nt, st);
 }
 
 static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cudaStream_t st) {
@@ -612,7 +698,7 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   const bool four = nt == 1 && a.q_dtype != CUDA_LLM_F32 && (eb == 1 || a.D == 64) && cap * a.Hkv * a.S / 16 >= 4ll * 4 * kWgtWarps * sms;
   const int want = (four ? 4 : 2) * kWgtWarps;
   WeightsGeom gm;
-  gm.hg = 8;
+  gm.hg = nt ? 8 : 1;
   while (a.Hkv % gm.hg || gm.hg * groups > want) gm.hg >>= 1;
   gm.n_hg = a.Hkv / gm.hg;
   gm.pages = want / (gm.hg * groups);
@@ -623,9 +709,26 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
               : a.scale_mode == CUDA_LLM_SCALE_MX_E8M0 ? (uint32_t)(a.D / 32) * a.page : 0u;
   gm.k_bytes = gm.hg * gm.k_head;
   gm.s_bytes = gm.hg * gm.s_head;
-  gm.stage_bytes = ((gm.k_bytes + gm.s_bytes) * gm.pages + 127) / 128 * 128;
-  gm.n_stages = (int)((kWgtBudget - kWgtHeader) / gm.stage_bytes);
+  gm.stage_bytes = ((gm.k_bytes + gm.s_bytes) * gm.pages + 1023) / 1024 * 1024;
+  const uint32_t q_bytes = nt || a.q_dtype == CUDA_LLM_F32 ? 0u : (uint32_t)kWgtRows * (a.D * 2 + 8);
+  gm.n_stages = (int)((kWgtBudget - kWgtHeader - q_bytes) / gm.stage_bytes);
   if (gm.n_stages > kWgtMaxStages) gm.n_stages = kWgtMaxStages;
+  gm.q_off = kWgtHeader + gm.n_stages * gm.stage_bytes;
+  gm.smem = gm.q_off + q_bytes;
+  WeightsMap map = {};
+  gm.box_rows = 0;
+  if (a.page * eb >= 64) {
+    EncodeTiledFn enc = tensor_map_encoder();
+    if (!enc) return cudaErrorNotSupported;
+    gm.box_rows = gm.hg * a.D < 256 ? gm.hg * a.D : 256;
+    const cuuint64_t dims[3] = {(cuuint64_t)a.page, (cuuint64_t)a.Hkv * a.D, (cuuint64_t)a.num_blocks};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.page * eb, (cuuint64_t)a.Hkv * a.D * a.page * eb};
+    const cuuint32_t box[3] = {(cuuint32_t)a.page, (cuuint32_t)gm.box_rows, 1}, estr[3] = {1, 1, 1};
+    if (enc(&map.k, eb == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(a.kc), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, a.page * eb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  }
   a.group_shift = (a.group & (a.group - 1)) ? -1 : __builtin_ctz(a.group);
   const int S = a.S;
   for (int s0 = 0; s0 < S; s0 += kWgtSeqs) {
@@ -638,7 +741,7 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
     x.scores += s0 * a.st_seq;
     const long long most = (cap + gm.tok_stage - 1) / gm.tok_stage * gm.n_hg * x.S;
     const int grid = (int)(most < sms ? most : sms);
-    const cudaError_t e = a.D == 64 ? go_types<64>(x, gm, grid, nt, st) : go_types<128>(x, gm, grid, nt, st);
+    const cudaError_t e = a.D == 64 ? go_types<64>(x, gm, map, grid, nt, st) : go_types<128>(x, gm, map, grid, nt, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
