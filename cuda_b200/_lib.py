@@ -67,7 +67,7 @@ class KvWeightsParams(C.Structure):
     ]
 
 
-EVICT_MAX_TOKENS = 786432
+EVICT_MAX_TOKENS = 393216
 
 
 class KvEvictParams(C.Structure):

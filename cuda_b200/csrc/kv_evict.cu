@@ -34,145 +34,427 @@ __device__ __forceinline__ uint32_t rank_key(float x, bool is_protected) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
+// ---- selection ------------------------------------------------------------------------------------------------------
+// A thread-block cluster per (KV head, sequence); each CTA holds its part of the score row in shared memory.  The budget-th
+// largest key comes from four passes over its bytes: a histogram per CTA (lanes with the same byte add once), summed over the
+// cluster through distributed shared memory.  Then each warp counts, and afterwards writes, the kept tokens of its own run
+// of positions, so that the order needs one prefix sum.  The row is read once, before anything is written: new_scores may be
+// scores.
+constexpr int kSelMaxPart = 49152;  // scores per CTA: 192 KB
 
-// One CTA per (KV head, sequence): the budget-th largest key by four passes over its bytes (histograms in shared memory),
-// then the kept positions in order by a running prefix sum.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t s_prefix, s_left;
-  __shared__ uint32_t warp_gt[32], warp_eq[32];
-  const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int ctx = evict_ctx(a, s, h == 0 && tid == 0);
+__device__ __forceinline__ uint32_t sel_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t sel_parts() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void sel_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t sel_remote(const uint32_t* p, uint32_t rank) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.u32 %0, [ra];\n\t}"
+               : "=r"(v) : "r"(smem_u32(p)), "r"(rank) : "memory");
+  return v;
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a) {
+  constexpr int WARPS = THREADS / 32;
+  extern __shared__ float row[];
+  __shared__ uint32_t hist[4][256], digit_sum[256];
+  __shared__ uint32_t counts[2];             // kept for sure, on the edge: of this CTA
+  __shared__ uint32_t warp_gt[WARPS], warp_eq[WARPS], found[2];
+  const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = sel_rank(), parts = sel_parts();
+  const int ctx = evict_ctx(a, s, h == 0 && rank == 0 && tid == 0);
   const int n_keep = min(ctx, a.budget);
   const float* sc = a.scores + s * a.st_seq + h * a.st_head;
   float* ns = a.new_scores ? a.new_scores + s * a.nst_seq + h * a.nst_head : nullptr;
   int32_t* kept = a.kept + ((size_t)s * a.Hkv + h) * a.budget;
-  if (h == 0 && tid == 0) a.new_ctx[s] = n_keep;
-  for (int i = n_keep + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
-  auto key_at = [&](int t) { return rank_key(sc[t], t < a.sink || t >= ctx - a.recent); };
-  if (ctx <= a.budget) {
-    for (int t = tid; t < ctx; t += kSelThreads) {
+  if (h == 0 && rank == 0 && tid == 0) a.new_ctx[s] = n_keep;
+  for (int i = n_keep + (int)rank * THREADS + tid; i < a.budget; i += parts * THREADS) kept[i] = -1;
+  if (ctx <= a.budget) {  // of the whole cluster
+    for (int t = (int)rank * THREADS + tid; t < ctx; t += parts * THREADS) {
       kept[t] = t;
-      if (ns) ns[t] = sc[t];
+      if (ns && ns != sc) ns[t] = sc[t];
     }
     return;
   }
-  if (tid == 0) {
-    s_prefix = 0;
-    s_left = (uint32_t)n_keep;
-  }
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int t = tid; t < ctx; t += kSelThreads) {
-      const uint32_t k = key_at(t);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+  const int t0 = (int)((long long)ctx * rank / parts), n = (int)((long long)ctx * (rank + 1) / parts) - t0;
+  for (int i = tid; i < 4 * 256; i += THREADS) (&hist[0][0])[i] = 0;
+#pragma unroll 4
+  for (int i = tid; i < n; i += THREADS) row[i] = sc[t0 + i];
+  __syncthreads();
+  auto key_at = [&](int i) { return rank_key(row[i], t0 + i < a.sink || t0 + i >= ctx - a.recent); };
+  uint32_t prefix = 0, left = (uint32_t)n_keep;
+#pragma unroll 1
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
+    for (int i0 = 0; i0 < n; i0 += THREADS) {
+      const int i = i0 + tid;
+      const uint32_t k = i < n ? key_at(i) : 0u;
+      const bool in = i < n && (k & mask) == prefix;
+      const uint32_t digit = (k >> shift) & 255;
+      const uint32_t same = __match_any_sync(0xffffffffu, in ? digit : 256u);
+      if (in && lane == __ffs(same) - 1) atomicAdd(&hist[pass][digit], (uint32_t)__popc(same));
     }
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t left = s_left;
-      int b = 255;
-      while (b > 0 && hist[b] < left) left -= hist[b--];
-      s_left = left;
-      s_prefix = prefix | ((uint32_t)b << shift);
-    }
-    __syncthreads();
-  }
-  const uint32_t edge = s_prefix, n_edge = s_left;  // keep all above the edge and the first n_edge on it
-  uint32_t base_gt = 0, base_eq = 0;
-  for (int t0 = 0; t0 < ctx; t0 += kSelThreads) {
-    const int t = t0 + tid;
-    const uint32_t k = t < ctx ? key_at(t) : 0u;
-    const float x = t < ctx ? sc[t] : 0.f;
-    const bool gt = t < ctx && k > edge, eq = t < ctx && k == edge;
-    const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      warp_gt[warp] = __popc(bg);
-      warp_eq[warp] = __popc(be);
-    }
-    __syncthreads();  // and every score of this tile is read: new_scores may be scores
-    uint32_t g = base_gt, e = base_eq;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) {
-        g += warp_gt[w];
-        e += warp_eq[w];
+    if (parts > 1) sel_cluster_sync();
+    else __syncthreads();
+    if (tid < 256) {
+      uint32_t sum = hist[pass][tid];
+      if (parts > 1) {
+        sum = 0;
+        for (uint32_t q = 0; q < parts; ++q) sum += sel_remote(&hist[pass][tid], q);
       }
-      base_gt += warp_gt[w];
-      base_eq += warp_eq[w];
-    }
-    g += __popc(bg & ((1u << lane) - 1));
-    e += __popc(be & ((1u << lane) - 1));
-    if (gt || (eq && e < n_edge)) {
-      const uint32_t i = g + min(e, n_edge);
-      kept[i] = t;
-      if (ns) ns[i] = x;
+      digit_sum[tid] = sum;
     }
     __syncthreads();
+    if (warp == 0) {  // the largest digit d with (keys above d) < left <= (keys from d up)
+      uint32_t c[8], mine = 0;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        c[x] = digit_sum[255 - (lane * 8 + x)];
+        mine += c[x];
+      }
+      uint32_t before = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      before -= mine;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        if (before < left && left <= before + c[x]) {
+          found[0] = 255 - (lane * 8 + x);
+          found[1] = left - before;
+        }
+        before += c[x];
+      }
+    }
+    __syncthreads();
+    prefix |= found[0] << shift;
+    left = found[1];
   }
+  // keep all keys above `prefix` and the first `left` that equal it
+  const uint32_t edge = prefix;
+  const int per = ((n + WARPS - 1) / WARPS + 31) & ~31, b0 = min(n, warp * per), b1 = min(n, b0 + per);
+  uint32_t gt = 0, eq = 0;
+  for (int i0 = b0; i0 < b1; i0 += 32) {
+    const uint32_t k = i0 + lane < b1 ? key_at(i0 + lane) : 0u;
+    gt += __popc(__ballot_sync(0xffffffffu, i0 + lane < b1 && k > edge));
+    eq += __popc(__ballot_sync(0xffffffffu, i0 + lane < b1 && k == edge));
+  }
+  if (lane == 0) {
+    warp_gt[warp] = gt;
+    warp_eq[warp] = eq;
+  }
+  __syncthreads();
+  if (warp == 0) {  // exclusive prefix sums over the warps, totals of the CTA
+    uint32_t x = lane < WARPS ? warp_gt[lane] : 0u, y = lane < WARPS ? warp_eq[lane] : 0u;
+    const uint32_t x0 = x, y0 = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) {
+        x += u;
+        y += v;
+      }
+    }
+    if (lane < WARPS) {
+      warp_gt[lane] = x - x0;
+      warp_eq[lane] = y - y0;
+    }
+    if (lane == 31) {
+      counts[0] = x;
+      counts[1] = y;
+    }
+  }
+  if (parts > 1) sel_cluster_sync();
+  else __syncthreads();
+  uint32_t at_gt = warp_gt[warp], at_eq = warp_eq[warp];
+  for (uint32_t q = 0; q < rank; ++q) {
+    at_gt += sel_remote(&counts[0], q);
+    at_eq += sel_remote(&counts[1], q);
+  }
+  for (int i0 = b0; i0 < b1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t k = i < b1 ? key_at(i) : 0u;
+    const bool is_gt = i < b1 && k > edge, is_eq = i < b1 && k == edge;
+    const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq), below = (1u << lane) - 1;
+    const uint32_t e = at_eq + __popc(be & below);
+    if (is_gt || (is_eq && e < left)) {
+      const uint32_t to = at_gt + __popc(bg & below) + min(e, left);
+      kept[to] = t0 + i;
+      if (ns) ns[to] = row[i];
+    }
+    at_gt += __popc(bg);
+    at_eq += __popc(be);
+  }
+  if (parts > 1) sel_cluster_sync();  // nobody leaves while its counts may still be read
 }
+
+// ---- move -----------------------------------------------------------------------------------------------------------
+// A (page, head) is rows of `page` elements (head_dim rows of K, ..), so a kept token is one element in every row and moving it
+// shifts bytes inside rows.  The unit is 16 bytes of a row (a group of 16, 8 or 4 tokens): a lane owns a row, loads the old
+// groups that hold kept tokens one after another (each once) and assembles the new groups with byte permutes.  Which bytes go
+// where is the same for every row of the KV head: a CTA works that out once for a run of new positions, as a list of old
+// groups ("entries") and, for every 32-bit word of a new group, the pieces it takes from them.  Bound by DRAM: whole
+// groups are read for the tokens kept in them.
+//
+// In place: a kept token never moves upwards, so when a lane writes new group g, every old group that it still has to read
+// lies above g; rows are owned by lanes, so no other order matters.  One CTA then takes all positions of a KV head in
+// turn; into other pages every run of positions is a CTA of its own.
+constexpr int kMoveThreads = 256, kMoveRun = 2048, kMoveRing = 8;
 
 struct MoveTensor {
   void* p;
-  int rows;     // rows of a (page, head): head_dim, head_dim / 2, head_dim / 32 or 1
-  int task0;    // first 32-row slice of this tensor among all slices of a head
+  int rows;  // rows of a (page, head)
 };
 struct MoveArgs {
   EvictArgs e;
-  MoveTensor t[4];
-  int n_tensors, slices;
+  MoveTensor t[2];      // K, V
+  MoveTensor sc[2];     // their scales: rows 1 of 4 bytes, or head_dim / 32 of 1 byte; rows 0: none
+  int slices[2];        // 32-row slices of K and V
+  int run;              // new positions a CTA works out at a time
 };
 
-// One warp per (sequence, KV head, 32 rows of one tensor): it walks the new positions in groups of 16 tokens, a lane
-// takes the group's 16 elements of one row.  Within a row old positions never lie before new ones, so walking
-// upwards is safe in place, and no two warps touch the same row.
-template <typename E>
-__device__ __forceinline__ void move_rows(const EvictArgs& a, const MoveTensor& mt, int s, int h, int row, int g0, int g_step) {
-  const int ctx = evict_ctx(a, s, false), n = min(ctx, a.budget);
-  if (a.in_place && ctx <= a.budget) return;
-  const int32_t* kept = a.kept + ((size_t)s * a.Hkv + h) * a.budget;
-  const int32_t* bt = a.bt + (size_t)s * a.max_blocks;
-  const int32_t* nbt = a.new_bt + (size_t)s * a.new_max_blocks;
-  E* p = static_cast<E*>(mt.p);
-  for (int g = g0; g * 16 < n; g += g_step) {
-    E x[16];
-    uint32_t have = 0;
-    for (int k = 0; k < 16; ++k) {
-      const int i = g * 16 + k;
-      if (i >= n) break;
-      const int t = kept[i];
-      if (t < 0 || t >= ctx) continue;
-      const int blk = bt[t / a.page];
+struct MovePlan {           // of one run of new positions, in shared memory
+  int2 entry[kMoveRun];     // page (or -1) and 16-byte group of the page of an old group
+  uint2 piece[kMoveRun];    // selectors {lo 8 source bytes | hi 8 << 16, which of the two | keep or take << 16}, bit 31: next entry
+  uint16_t word[kMoveRun + 4];  // first piece of every word
+  uint16_t gentry[kMoveRun / 4 + 2];  // first entry of every new group
+  int to[kMoveRun / 4];     // new page of every group
+  uint32_t have[kMoveRun / 4];  // which of a group's tokens there are
+  uint32_t scan[2][kMoveThreads / 32];
+};
+
+template <int EB>
+__device__ void plan_run(const EvictArgs& a, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx) {
+  constexpr int G = 16 / EB, WT = 4 / EB > 0 ? 4 / EB : 1;  // tokens of a group, of a word
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t base_e = 0, base_p = 0;
+  for (int j0 = 0; j0 < n; j0 += kMoveThreads) {
+    const int j = j0 + tid;
+    const int t = j < n ? kept[p0 + j] : -1, prev = j > 0 && j < n ? kept[p0 + j - 1] : -1;
+    const bool first_e = j < n && (j % G == 0 || t / G != prev / G);
+    const bool first_p = j < n && (first_e || j % WT == 0);
+    uint32_t e = first_e, p = first_p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, e, o), y = __shfl_up_sync(0xffffffffu, p, o);
+      if (lane >= o) {
+        e += x;
+        p += y;
+      }
+    }
+    if (lane == 31) {
+      pl.scan[0][warp] = e;
+      pl.scan[1][warp] = p;
+    }
+    __syncthreads();
+    uint32_t be = base_e, bp = base_p;
+#pragma unroll
+    for (int w = 0; w < kMoveThreads / 32; ++w) {
+      if (w < warp) {
+        be += pl.scan[0][w];
+        bp += pl.scan[1][w];
+      }
+      base_e += pl.scan[0][w];
+      base_p += pl.scan[1][w];
+    }
+    e += be - 1;  // index of the entry and the piece of this position
+    p += bp - 1;
+    if (first_e) {
+      int blk = (t >= 0 && t < ctx) ? bt[t / a.page] : -1;
       if (blk < 0 || blk >= a.num_blocks) {
         if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
-        continue;
+        blk = -1;
       }
-      x[k] = p[(((size_t)blk * a.Hkv + h) * mt.rows + row) * a.page + t % a.page];
-      have |= 1u << k;
+      pl.entry[e] = make_int2(blk, t % a.page / G);
     }
-    const int to = nbt[g * 16 / a.page];
-    if (to < 0 || to >= a.num_blocks) {
-      if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
-      continue;
+    if (first_p) {  // the tokens of this piece: same word, same old group
+      uint32_t lo = 0, hi = 0, pick = 0, take = 0x3210;
+      for (int k = j; k < n && (k == j || (k % WT != 0 && k % G != 0)); ++k) {
+        const int tk = kept[p0 + k];
+        if (tk / G != t / G) break;
+#pragma unroll
+        for (int x = 0; x < EB; ++x) {
+          const int to = (k % WT) * EB + x, from = (tk % G) * EB + x;
+          if (from < 8) lo |= (uint32_t)from << (4 * to);
+          else hi |= (uint32_t)(from - 8) << (4 * to);
+          pick |= (uint32_t)(from < 8 ? to : 4 + to) << (4 * to);
+          take |= 4u << (4 * to);
+        }
+      }
+      pl.piece[p] = make_uint2(lo | hi << 16, pick | take << 16 | (first_e ? 0x80000000u : 0u));
     }
-    E* dst = p + (((size_t)to * a.Hkv + h) * mt.rows + row) * a.page + g * 16 % a.page;
-    for (int k = 0; k < 16; ++k)
-      if (have >> k & 1) dst[k] = x[k];
+    if (j < n && j % WT == 0) pl.word[j / WT] = (uint16_t)p;
+    if (j < n && j % G == 0) {
+      const int to = nbt[(p0 + j) / a.page];
+      const bool fine = to >= 0 && to < a.num_blocks;
+      if (!fine && a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
+      pl.to[j / G] = fine ? to : -1;
+      pl.gentry[j / G] = (uint16_t)e;
+      uint32_t have = 0;
+      for (int k = 0; k < G && j + k < n; ++k) {
+        const int tk = kept[p0 + j + k];
+        const int blk = (tk >= 0 && tk < ctx) ? bt[tk / a.page] : -1;
+        if (blk >= 0 && blk < a.num_blocks) have |= 1u << k;
+      }
+      pl.have[j / G] = fine ? have : 0u;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    const int words = (n + WT - 1) / WT, groups = (n + G - 1) / G;
+    for (int w = words; w < groups * 4; ++w) pl.word[w] = (uint16_t)base_p;
+    pl.word[groups * 4] = (uint16_t)base_p;
+    pl.gentry[groups] = (uint16_t)base_e;
+  }
+  __syncthreads();
+}
+
+template <int EB>
+__device__ __forceinline__ void move_slice(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int row, int h, int n, int p0, uint32_t ring) {
+  constexpr int G = 16 / EB;
+  const int groups = (n + G - 1) / G, n_entries = pl.gentry[groups];
+  const bool live = row < mt.rows;
+  const long long head_bytes = (long long)mt.rows * a.page * EB, row_at = (long long)row * a.page * EB;
+  uint8_t* const base = static_cast<uint8_t*>(mt.p) + h * head_bytes + row_at;
+  const long long page_bytes = head_bytes * a.Hkv;
+  const uint32_t mine = ring + (threadIdx.x & 31) * 16;
+  auto request = [&](int e) {
+    if (e < n_entries) {
+      const int2 src = pl.entry[e];
+      if (live && src.x >= 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (e % kMoveRing) * 512), "l"(base + src.x * page_bytes + src.y * 16) : "memory");
+    }
+    cp_async_commit();
+  };
+#pragma unroll 1
+  for (int e = 0; e < kMoveRing - 1; ++e) request(e);
+  int e = -1;
+  uint4 src = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int g = 0; g < groups; ++g) {
+    uint32_t out[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int q1 = pl.word[g * 4 + w + 1];
+#pragma unroll 1
+      for (int q = pl.word[g * 4 + w]; q < q1; ++q) {
+        const uint2 pc = pl.piece[q];
+        if (pc.y >> 31) {
+          ++e;
+          request(e + kMoveRing - 1);
+          cp_async_wait<kMoveRing - 1>();
+          src = lds128(mine + (e % kMoveRing) * 512);
+        }
+        const uint32_t lo = prmt(src.x, src.y, pc.x), hi = prmt(src.z, src.w, pc.x >> 16);
+        out[w] = prmt(out[w], prmt(lo, hi, pc.y), (pc.y >> 16) & 0x7fffu);
+      }
+    }
+    const uint32_t have = pl.have[g];
+    if (live && have) {
+      uint8_t* dst = base + pl.to[g] * page_bytes + ((p0 + g * G) % a.page) * EB;
+      if (have == (1u << G) - 1) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < G; ++k)
+          if (have >> k & 1) {
+            if (EB == 1) dst[k] = (uint8_t)(out[k >> 2] >> (8 * (k & 3)));
+            else if (EB == 2) reinterpret_cast<uint16_t*>(dst)[k] = (uint16_t)(out[k >> 1] >> (16 * (k & 1)));
+            else reinterpret_cast<uint32_t*>(dst)[k] = out[k & 3];
+          }
+      }
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// scales: a lane takes a token
+template <typename E>
+__device__ __forceinline__ void move_scales(const EvictArgs& a, const MoveTensor& mt, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int h,
+                                            int n, int p0, int ctx) {
+  const int lane = threadIdx.x & 31;
+  E* const p = static_cast<E*>(mt.p);
+  for (int j0 = 0; j0 < n; j0 += 32) {
+    const int j = j0 + lane;
+    const int t = j < n ? kept[p0 + j] : -1;
+    const int blk = (t >= 0 && t < ctx) ? bt[t / a.page] : -1, to = j < n ? nbt[(p0 + j) / a.page] : -1;
+    const bool fine = blk >= 0 && blk < a.num_blocks && to >= 0 && to < a.num_blocks;
+    for (int r = 0; r < mt.rows; ++r) {
+      E x = 0;
+      if (fine) x = p[(((size_t)blk * a.Hkv + h) * mt.rows + r) * a.page + t % a.page];
+      __syncwarp();
+      if (fine) p[(((size_t)to * a.Hkv + h) * mt.rows + r) * a.page + (p0 + j) % a.page] = x;
+      __syncwarp();
+    }
   }
 }
 
-template <typename EK, typename EV>
-__global__ void __launch_bounds__(128) evict_move_kernel(const MoveArgs m) {
-  const int task = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, h = blockIdx.y % m.e.Hkv, s = blockIdx.y / m.e.Hkv;
-  if (task >= m.slices) return;
-  int i = 0;
-  while (i + 1 < m.n_tensors && task >= m.t[i + 1].task0) ++i;
-  const int row = (task - m.t[i].task0) * 32 + lane;
-  if (row >= m.t[i].rows) return;
-  if (i == 0) move_rows<EK>(m.e, m.t[i], s, h, row, blockIdx.z, gridDim.z);
-  else if (i == 1) move_rows<EK>(m.e, m.t[i], s, h, row, blockIdx.z, gridDim.z);
-  else move_rows<EV>(m.e, m.t[i], s, h, row, blockIdx.z, gridDim.z);
+template <int EB, typename ES>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const MoveArgs m) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  MovePlan& pl = *reinterpret_cast<MovePlan*>(smem);
+  const EvictArgs& a = m.e;
+  const int h = blockIdx.y, s = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctx = evict_ctx(a, s, false), total = min(ctx, a.budget);
+  if (a.in_place && ctx <= a.budget) return;
+  const uint32_t ring = smem_u32(smem) + (uint32_t)((sizeof(MovePlan) + 15) & ~15) + warp * (kMoveRing * 512);
+  const int32_t* kept = a.kept + ((size_t)s * a.Hkv + h) * a.budget;
+  const int32_t* bt = a.bt + (size_t)s * a.max_blocks;
+  const int32_t* nbt = a.new_bt + (size_t)s * a.new_max_blocks;
+  for (int p0 = blockIdx.x * m.run; p0 < total; p0 += gridDim.x * m.run) {
+    const int n = min(m.run, total - p0);
+    plan_run<EB>(a, pl, kept, bt, nbt, p0, n, ctx);
+    const int slices = m.slices[0] + m.slices[1];
+    for (int task = warp; task < slices + 2; task += kMoveThreads / 32) {
+      if (task < m.slices[0]) move_slice<EB>(a, pl, m.t[0], task * 32 + lane, h, n, p0, ring);
+      else if (task < slices) move_slice<EB>(a, pl, m.t[1], (task - m.slices[0]) * 32 + lane, h, n, p0, ring);
+      else if (m.sc[task - slices].rows) move_scales<ES>(a, m.sc[task - slices], kept, bt, nbt, h, n, p0, ctx);
+    }
+    __syncthreads();
+  }
+}
+
+template <int EB, typename ES>
+static cudaError_t launch_move(const MoveArgs& m, cudaStream_t st) {
+  auto kern = evict_move_kernel<EB, ES>;
+  const int smem = (int)((sizeof(MovePlan) + 15) & ~15) + kMoveThreads / 32 * kMoveRing * 512;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const unsigned runs = m.e.in_place ? 1u : (unsigned)((m.e.budget + m.run - 1) / m.run);
+  kern<<<dim3(runs, m.e.Hkv, m.e.S), kMoveThreads, smem, st>>>(m);
+  return cudaGetLastError();
+}
+
+template <int THREADS>
+static cudaError_t launch_select(const EvictArgs& a, int parts, int most, cudaStream_t st) {
+  auto kern = evict_select_kernel<THREADS>;
+  const int smem = ((most + parts - 1) / parts + 1) * 4;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelMaxPart * 4 + 64);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(parts, a.Hkv, a.S);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 }  // namespace b200
@@ -205,7 +487,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   if (p->num_seqs == 0) return CUDA_LLM_OK;
   if (p->max_blocks_per_seq < 0 || p->new_max_blocks_per_seq < 0 || p->num_blocks <= 0)
     return refuse(CUDA_LLM_EINVAL, "block tables and pool must not be empty");
-  if ((long long)p->num_seqs * p->num_kv_heads > 65535) return refuse(CUDA_LLM_EINVAL, "more than 65535 (sequence, KV head) pairs");
+  if (p->num_seqs > 65535 || p->num_kv_heads > 65535) return refuse(CUDA_LLM_EINVAL, "more than 65535 sequences or KV heads");
   const bool scaled = !wide && p->scale_mode != CUDA_LLM_SCALE_PER_HEAD;
   if (!p->scores || !p->key_cache || !p->value_cache || !p->block_tables || !p->new_block_tables || !p->context_lens ||
       !p->new_context_lens || !p->kept || (scaled && (!p->k_scale || !p->v_scale)))
@@ -235,28 +517,25 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   a.new_max_blocks = p->new_max_blocks_per_seq; a.num_blocks = p->num_blocks; a.max_tokens = p->max_tokens; a.budget = p->budget;
   a.sink = p->sink; a.recent = p->recent; a.in_place = in_place;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  evict_select_kernel<<<dim3(a.Hkv, a.S), kSelThreads, 0, st>>>(a);
-  rc = cuda_result(cudaGetLastError(), "evict_select_kernel launch");
+  // the score row over as many CTAs as leave each at least 4096 scores
+  long long row_most = (long long)a.max_blocks * a.page;
+  if (row_most > a.max_tokens) row_most = a.max_tokens;
+  int parts = 1;
+  while (parts < 8 && row_most > 8192ll * parts) parts *= 2;
+  rc = cuda_result(row_most > 4096 ? launch_select<1024>(a, parts, (int)row_most, st) : launch_select<256>(a, parts, (int)row_most, st),
+                   "evict_select_kernel launch");
   if (rc != CUDA_LLM_OK) return rc;
-  const int D = p->head_dim;
-  m.n_tensors = 0;
-  m.slices = 0;
-  auto add = [&](void* t, int rows) {
-    m.t[m.n_tensors++] = MoveTensor{t, rows, m.slices};
-    m.slices += (rows + 31) / 32;
-  };
-  add(p->key_cache, D);
-  add(p->value_cache, p->v_format == CUDA_LLM_KV_FP4_E2M1 ? D / 2 : D);
-  if (scaled) {
-    const int rows = p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? 1 : D / 32;
-    add(p->k_scale, rows);
-    add(p->v_scale, rows);
-  }
-  const dim3 grid((m.slices + 3) / 4, a.Hkv * a.S, in_place ? 1 : 16);
+  const int D = p->head_dim, v_rows = p->v_format == CUDA_LLM_KV_FP4_E2M1 ? D / 2 : D;
+  const int sc_rows = !scaled ? 0 : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? 1 : D / 32;
+  m.t[0] = MoveTensor{p->key_cache, D};
+  m.t[1] = MoveTensor{p->value_cache, v_rows};
+  m.sc[0] = MoveTensor{p->k_scale, sc_rows};
+  m.sc[1] = MoveTensor{p->v_scale, sc_rows};
+  m.slices[0] = D / 32;
+  m.slices[1] = v_rows / 32;
+  m.run = in_place ? kMoveRun : 256;
   const int eb = format_bytes(p->k_format);
-  if (eb == 4) evict_move_kernel<uint32_t, uint32_t><<<grid, 128, 0, st>>>(m);
-  else if (eb == 2) evict_move_kernel<uint16_t, uint16_t><<<grid, 128, 0, st>>>(m);
-  else if (p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN) evict_move_kernel<uint8_t, uint32_t><<<grid, 128, 0, st>>>(m);
-  else evict_move_kernel<uint8_t, uint8_t><<<grid, 128, 0, st>>>(m);
-  return cuda_result(cudaGetLastError(), "evict_move_kernel launch");
+  const cudaError_t e = eb == 4 ? launch_move<4, uint32_t>(m, st) : eb == 2 ? launch_move<2, uint32_t>(m, st)
+                        : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move<1, uint32_t>(m, st) : launch_move<1, uint8_t>(m, st);
+  return cuda_result(e, "evict_move_kernel launch");
 }

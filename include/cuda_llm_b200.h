@@ -453,7 +453,7 @@ typedef struct CudaLlmKvEvictParams {
   int32_t sink;
   int32_t recent;
 } CudaLlmKvEvictParams;
-#define CUDA_LLM_EVICT_MAX_TOKENS 786432
+#define CUDA_LLM_EVICT_MAX_TOKENS 393216
 
 int cuda_llm_kv_evict(const CudaLlmKvEvictParams* params, void* stream);
 

@@ -107,7 +107,7 @@ EVICT_BAD = [
     (dict(k_format=L.KV_BF16), L.EINVAL), (dict(v_format=L.KV_F16), L.EINVAL), (dict(v_format=L.KV_FP4_E2M1), L.EINVAL),
     (dict(scale_mode=L.SCALE_PER_BLOCK), L.EINVAL), (dict(scale_mode=-1), L.EINVAL), (dict(budget=0), L.EINVAL), (dict(budget=-3), L.EINVAL),
     (dict(sink=-1), L.EINVAL), (dict(recent=-1), L.EINVAL), (dict(sink=40, recent=40), L.EINVAL), (dict(budget=2 ** 31 - 1, sink=2 ** 31 - 1, recent=1), L.EINVAL),
-    (dict(max_tokens=L.EVICT_MAX_TOKENS + 1), L.EINVAL), (dict(num_blocks=0), L.EINVAL), (dict(num_seqs=40000), L.EINVAL),
+    (dict(max_tokens=L.EVICT_MAX_TOKENS + 1), L.EINVAL), (dict(num_blocks=0), L.EINVAL), (dict(num_seqs=70000), L.EINVAL),
     (dict(scores=None), L.EINVAL), (dict(kept=None), L.EINVAL), (dict(k_scale=None), L.EINVAL), (dict(new_context_lens=0x7000), L.EINVAL),
     (dict(new_max_blocks_per_seq=3), L.EINVAL), (dict(new_block_tables=0xa000, new_max_blocks_per_seq=3), L.EINVAL),
     (dict(key_cache=0x2004), L.EALIGN), (dict(kept=0x9002), L.EALIGN),
