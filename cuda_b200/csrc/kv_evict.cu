@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
 // In place: a kept token never moves upwards, so when a lane writes new group g, every old group that it still has to read
 // lies above g; rows are owned by lanes, so no other order matters.  One CTA then takes all positions of a KV head in
 // turn; into other pages every run of positions is a CTA of its own.
-constexpr int kMoveThreads = 256, kMoveRun = 2048, kMoveRing = 8;
+constexpr int kMoveThreads = 256, kMoveRun = 2048, kMoveRing = 16;
 
 struct MoveTensor {
   void* p;
@@ -226,25 +226,41 @@ struct MoveArgs {
 };
 
 struct MovePlan {           // of one run of new positions, in shared memory
-  int2 entry[kMoveRun];     // page (or -1) and 16-byte group of the page of an old group
-  uint2 piece[kMoveRun];    // selectors {lo 8 source bytes | hi 8 << 16, which of the two | keep or take << 16}, bit 31: next entry
-  uint16_t word[kMoveRun + 4];  // first piece of every word
-  uint16_t gentry[kMoveRun / 4 + 2];  // first entry of every new group
-  int to[kMoveRun / 4];     // new page of every group
+  int2 entry[kMoveRun + kMoveRing];  // page (or -1) and 16-byte group of the page of an old group
+  uint2 piece[kMoveRun + 2];  // selectors {of the low 8 source bytes | high 8 << 16, which of the two | keep or take << 16} + flags
+  int to[kMoveRun / 4];     // new page of every new group
   uint32_t have[kMoveRun / 4];  // which of a group's tokens there are
+  int kept[kMoveRun];
   uint32_t scan[2][kMoveThreads / 32];
+  int n_entries, n_pieces;
 };
+// flags of a piece, in bits that no selector uses
+constexpr uint32_t kNewEntry = 0x80000000u, kWordEnd = 0x8000u;
 
 template <int EB>
 __device__ void plan_run(const EvictArgs& a, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx) {
-  constexpr int G = 16 / EB, WT = 4 / EB > 0 ? 4 / EB : 1;  // tokens of a group, of a word
+  constexpr int G = 16 / EB, WT = 4 / EB;  // tokens of a group, of a word
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int j = tid; j < n; j += kMoveThreads) pl.kept[j] = kept[p0 + j];
+  __syncthreads();
   uint32_t base_e = 0, base_p = 0;
   for (int j0 = 0; j0 < n; j0 += kMoveThreads) {
     const int j = j0 + tid;
-    const int t = j < n ? kept[p0 + j] : -1, prev = j > 0 && j < n ? kept[p0 + j - 1] : -1;
+    const int t = j < n ? pl.kept[j] : -1, prev = j > 0 && j < n ? pl.kept[j - 1] : -1;
     const bool first_e = j < n && (j % G == 0 || t / G != prev / G);
     const bool first_p = j < n && (first_e || j % WT == 0);
+    int blk = (t >= 0 && t < ctx) ? bt[t / a.page] : -1;
+    int to = j < n ? nbt[(p0 + j) / a.page] : -1;
+    if (blk >= a.num_blocks || to >= a.num_blocks || ((blk < 0 || to < 0) && j < n)) {
+      if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
+      if (blk >= a.num_blocks) blk = -1;
+      if (to >= a.num_blocks) to = -1;
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0 && to >= 0);
+    if (j < n && j % G == 0) {
+      pl.to[j / G] = to;
+      pl.have[j / G] = there >> lane & ((1u << G) - 1);
+    }
     uint32_t e = first_e, p = first_p;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -269,115 +285,110 @@ __device__ void plan_run(const EvictArgs& a, MovePlan& pl, const int32_t* kept, 
       base_e += pl.scan[0][w];
       base_p += pl.scan[1][w];
     }
-    e += be - 1;  // index of the entry and the piece of this position
-    p += bp - 1;
-    if (first_e) {
-      int blk = (t >= 0 && t < ctx) ? bt[t / a.page] : -1;
-      if (blk < 0 || blk >= a.num_blocks) {
-        if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
-        blk = -1;
-      }
-      pl.entry[e] = make_int2(blk, t % a.page / G);
-    }
+    if (first_e) pl.entry[e + be - 1] = make_int2(blk, t % a.page / G);
     if (first_p) {  // the tokens of this piece: same word, same old group
       uint32_t lo = 0, hi = 0, pick = 0, take = 0x3210;
-      for (int k = j; k < n && (k == j || (k % WT != 0 && k % G != 0)); ++k) {
-        const int tk = kept[p0 + k];
-        if (tk / G != t / G) break;
+      int k = j;
+      do {
+        const int from0 = pl.kept[k] % G * EB, to0 = k % WT * EB;
 #pragma unroll
         for (int x = 0; x < EB; ++x) {
-          const int to = (k % WT) * EB + x, from = (tk % G) * EB + x;
-          if (from < 8) lo |= (uint32_t)from << (4 * to);
-          else hi |= (uint32_t)(from - 8) << (4 * to);
-          pick |= (uint32_t)(from < 8 ? to : 4 + to) << (4 * to);
-          take |= 4u << (4 * to);
+          const int from = from0 + x, at = 4 * (to0 + x);
+          if (from < 8) lo |= (uint32_t)from << at;
+          else hi |= (uint32_t)(from - 8) << at;
+          pick |= (uint32_t)((from < 8 ? 0 : 4) + to0 + x) << at;
+          take |= 4u << at;
         }
-      }
-      pl.piece[p] = make_uint2(lo | hi << 16, pick | take << 16 | (first_e ? 0x80000000u : 0u));
-    }
-    if (j < n && j % WT == 0) pl.word[j / WT] = (uint16_t)p;
-    if (j < n && j % G == 0) {
-      const int to = nbt[(p0 + j) / a.page];
-      const bool fine = to >= 0 && to < a.num_blocks;
-      if (!fine && a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
-      pl.to[j / G] = fine ? to : -1;
-      pl.gentry[j / G] = (uint16_t)e;
-      uint32_t have = 0;
-      for (int k = 0; k < G && j + k < n; ++k) {
-        const int tk = kept[p0 + j + k];
-        const int blk = (tk >= 0 && tk < ctx) ? bt[tk / a.page] : -1;
-        if (blk >= 0 && blk < a.num_blocks) have |= 1u << k;
-      }
-      pl.have[j / G] = fine ? have : 0u;
+        ++k;
+      } while (k < n && k % WT != 0 && pl.kept[k] / G == t / G);
+      pl.piece[p + bp - 1] = make_uint2(lo | hi << 16, pick | take << 16 | (first_e ? kNewEntry : 0u) | (k % WT == 0 || k == n ? kWordEnd : 0u));
     }
     __syncthreads();
   }
   if (tid == 0) {
-    const int words = (n + WT - 1) / WT, groups = (n + G - 1) / G;
-    for (int w = words; w < groups * 4; ++w) pl.word[w] = (uint16_t)base_p;
-    pl.word[groups * 4] = (uint16_t)base_p;
-    pl.gentry[groups] = (uint16_t)base_e;
+    pl.n_entries = (int)base_e;
+    pl.n_pieces = (int)base_p;
   }
+  for (int x = tid; x < kMoveRing; x += kMoveThreads) pl.entry[base_e + x] = make_int2(-1, 0);
+  if (tid < 2) pl.piece[base_p + tid] = make_uint2(0, 0);
   __syncthreads();
 }
 
 template <int EB>
-__device__ __forceinline__ void move_slice(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int row, int h, int n, int p0, uint32_t ring) {
+__device__ __forceinline__ void move_slice(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int row, int h, int p0, uint32_t ring) {
   constexpr int G = 16 / EB;
-  const int groups = (n + G - 1) / G, n_entries = pl.gentry[groups];
+  const int n_pieces = pl.n_pieces;
   const bool live = row < mt.rows;
-  const long long head_bytes = (long long)mt.rows * a.page * EB, row_at = (long long)row * a.page * EB;
-  uint8_t* const base = static_cast<uint8_t*>(mt.p) + h * head_bytes + row_at;
-  const long long page_bytes = head_bytes * a.Hkv;
+  const uint32_t row_bytes = a.page * EB;
+  const long long head_bytes = (long long)mt.rows * row_bytes, page_bytes = head_bytes * a.Hkv;
+  uint8_t* const base = static_cast<uint8_t*>(mt.p) + h * head_bytes + (long long)row * row_bytes;
   const uint32_t mine = ring + (threadIdx.x & 31) * 16;
-  auto request = [&](int e) {
-    if (e < n_entries) {
-      const int2 src = pl.entry[e];
-      if (live && src.x >= 0)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (e % kMoveRing) * 512), "l"(base + src.x * page_bytes + src.y * 16) : "memory");
-    }
+  auto request = [&](int e, int slot) {  // (behind the last entry lie kMoveRing that copy nothing)
+    const int2 src = pl.entry[e];
+    if (live && src.x >= 0)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(mine + slot * 512), "l"(base + src.x * page_bytes + src.y * 16) : "memory");
     cp_async_commit();
   };
 #pragma unroll 1
-  for (int e = 0; e < kMoveRing - 1; ++e) request(e);
-  int e = -1;
-  uint4 src = make_uint4(0, 0, 0, 0);
+  for (int e = 0; e < kMoveRing - 1; ++e) request(e < pl.n_entries ? e : pl.n_entries, e);
+  int e = -1, slot = kMoveRing - 1, words = 0, g = 0;  // `slot`: where entry e + kMoveRing goes
+  uint4 src = make_uint4(0, 0, 0, 0), ahead;
+  cp_async_wait<kMoveRing - 2>();
+  ahead = lds128(mine);
+  uint32_t cur = 0, o0 = 0, o1 = 0, o2 = 0, o3 = 0;
+  uint2 next = pl.piece[0];
 #pragma unroll 1
-  for (int g = 0; g < groups; ++g) {
-    uint32_t out[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int q1 = pl.word[g * 4 + w + 1];
-#pragma unroll 1
-      for (int q = pl.word[g * 4 + w]; q < q1; ++q) {
-        const uint2 pc = pl.piece[q];
-        if (pc.y >> 31) {
-          ++e;
-          request(e + kMoveRing - 1);
-          cp_async_wait<kMoveRing - 1>();
-          src = lds128(mine + (e % kMoveRing) * 512);
-        }
-        const uint32_t lo = prmt(src.x, src.y, pc.x), hi = prmt(src.z, src.w, pc.x >> 16);
-        out[w] = prmt(out[w], prmt(lo, hi, pc.y), (pc.y >> 16) & 0x7fffu);
-      }
+  for (int q = 0; q < n_pieces; ++q) {
+    const uint2 pc = next;
+    next = pl.piece[q + 1];
+    if (pc.y & kNewEntry) {
+      ++e;
+      src = ahead;
+      // the slot of the entry before this one is free; the entry after this one is needed next
+      const int want = e + kMoveRing - 1;
+      request(want < pl.n_entries ? want : pl.n_entries, slot);
+      slot = (slot + 1) & (kMoveRing - 1);
+      cp_async_wait<kMoveRing - 2>();
+      ahead = lds128(mine + ((slot + 1) & (kMoveRing - 1)) * 512);
     }
-    const uint32_t have = pl.have[g];
-    if (live && have) {
-      uint8_t* dst = base + pl.to[g] * page_bytes + ((p0 + g * G) % a.page) * EB;
-      if (have == (1u << G) - 1) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-      } else {
+    const uint32_t lo = prmt(src.x, src.y, pc.x), hi = prmt(src.z, src.w, pc.x >> 16);
+    cur = prmt(cur, prmt(lo, hi, pc.y & 0x7777u), (pc.y >> 16) & 0x7777u);
+    if (pc.y & kWordEnd) {
+      o0 = o1;
+      o1 = o2;
+      o2 = o3;
+      o3 = cur;
+      if (++words == 4 || q + 1 == n_pieces) {
+        while (words < 4) {  // the last group of a sequence may end early
+          o0 = o1;
+          o1 = o2;
+          o2 = o3;
+          o3 = 0;
+          ++words;
+        }
+        words = 0;
+        const uint32_t have = pl.have[g];
+        if (live && have) {
+          uint8_t* dst = base + pl.to[g] * page_bytes + ((p0 + g * G) & (a.page - 1)) * EB;
+          if (have == (1u << G) - 1) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(o0, o1, o2, o3);
+          } else {
+            const uint32_t out[4] = {o0, o1, o2, o3};
 #pragma unroll
-        for (int k = 0; k < G; ++k)
-          if (have >> k & 1) {
-            if (EB == 1) dst[k] = (uint8_t)(out[k >> 2] >> (8 * (k & 3)));
-            else if (EB == 2) reinterpret_cast<uint16_t*>(dst)[k] = (uint16_t)(out[k >> 1] >> (16 * (k & 1)));
-            else reinterpret_cast<uint32_t*>(dst)[k] = out[k & 3];
+            for (int k = 0; k < G; ++k)
+              if (have >> k & 1) {
+                if (EB == 1) dst[k] = (uint8_t)(out[k >> 2] >> (8 * (k & 3)));
+                else if (EB == 2) reinterpret_cast<uint16_t*>(dst)[k] = (uint16_t)(out[k >> 1] >> (16 * (k & 1)));
+                else reinterpret_cast<uint32_t*>(dst)[k] = out[k & 3];
+              }
           }
+        }
+        ++g;
       }
     }
   }
   cp_async_wait<0>();
+  __syncwarp();
 }
 
 // scales: a lane takes a token
@@ -418,8 +429,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const MoveArgs
     plan_run<EB>(a, pl, kept, bt, nbt, p0, n, ctx);
     const int slices = m.slices[0] + m.slices[1];
     for (int task = warp; task < slices + 2; task += kMoveThreads / 32) {
-      if (task < m.slices[0]) move_slice<EB>(a, pl, m.t[0], task * 32 + lane, h, n, p0, ring);
-      else if (task < slices) move_slice<EB>(a, pl, m.t[1], (task - m.slices[0]) * 32 + lane, h, n, p0, ring);
+      if (task < m.slices[0]) move_slice<EB>(a, pl, m.t[0], task * 32 + lane, h, p0, ring);
+      else if (task < slices) move_slice<EB>(a, pl, m.t[1], (task - m.slices[0]) * 32 + lane, h, p0, ring);
       else if (m.sc[task - slices].rows) move_scales<ES>(a, m.sc[task - slices], kept, bt, nbt, h, n, p0, ctx);
     }
     __syncthreads();
