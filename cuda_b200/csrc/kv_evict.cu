@@ -1,7 +1,7 @@
 // Eviction from a paged KV cache: which tokens stay (a selection by rank per sequence and KV head), and their move to the
 // front of the same or of other pages.
 #include "host_common.cuh"
-#include "sm100_primitives.cuh"
+#include "tcgen05_primitives.cuh"
 
 namespace b200 {
 
@@ -101,8 +101,12 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
       const uint32_t k = i < n ? key_at(i) : 0u;
       const bool in = i < n && (k & mask) == prefix;
       const uint32_t digit = (k >> shift) & 255;
-      const uint32_t same = __match_any_sync(0xffffffffu, in ? digit : 256u);
-      if (in && lane == __ffs(same) - 1) atomicAdd(&hist[pass][digit], (uint32_t)__popc(same));
+      if (pass == 0) {  // sign and exponent: few different bytes, lanes with the same one add once
+        const uint32_t same = __match_any_sync(0xffffffffu, in ? digit : 256u);
+        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[0][digit], (uint32_t)__popc(same));
+      } else if (in) {
+        atomicAdd(&hist[pass][digit], 1u);
+      }
     }
     if (parts > 1) sel_cluster_sync();
     else __syncthreads();
@@ -201,250 +205,256 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
 }
 
 // ---- move -----------------------------------------------------------------------------------------------------------
-// A (page, head) is rows of `page` elements (head_dim rows of K, ..), so a kept token is one element in every row and moving it
-// shifts bytes inside rows.  The unit is 16 bytes of a row (a group of 16, 8 or 4 tokens): a lane owns a row, loads the old
-// groups that hold kept tokens one after another (each once) and assembles the new groups with byte permutes.  Which bytes go
-// where is the same for every row of the KV head: a CTA works that out once for a run of new positions, as a list of old
-// groups ("entries") and, for every 32-bit word of a new group, the pieces it takes from them.  Bound by DRAM: whole
-// groups are read for the tokens kept in them.
+// A (page, head) is a slab of rows (head_dim rows of K, ..) of `page` elements, contiguous in memory; a kept token is one element
+// in every row.  A CTA owns some rows of K and V of one (sequence, KV head) and walks the new positions in groups of 16 bytes of
+// a row: a producer thread brings in the slabs that hold kept tokens, each once, by bulk copies into a ring that always holds
+// all slabs a group can need; each warp, with rows of its own, gathers the group's elements from them, a lane one 32-bit
+// word of a row, and writes the words out.  Bound by DRAM: whole slabs are read for the tokens kept in them.
 //
-// In place: a kept token never moves upwards, so when a lane writes new group g, every old group that it still has to read
-// lies above g; rows are owned by lanes, so no other order matters.  One CTA then takes all positions of a KV head in
-// turn; into other pages every run of positions is a CTA of its own.
-constexpr int kMoveThreads = 256, kMoveRun = 2048, kMoveRing = 16;
+// In place: a kept token never moves upwards, so every page that is still to be read, however far ahead the copies run, lies
+// above the group that is written, or is in the ring already; rows belong to warps, so no other order matters.  The tokens of a head are then one
+// CTA's work, and with few (sequence, head) pairs the rows are split over more CTAs; into other pages every run of new
+// positions is a CTA of its own.
+constexpr int kMoveWarps = 8, kMoveThreads = 32 * (kMoveWarps + 2), kMoveRun = 2048, kMoveMaxRing = 32;
 
 struct MoveTensor {
-  void* p;
+  uint8_t* p;
   int rows;  // rows of a (page, head)
 };
 struct MoveArgs {
   EvictArgs e;
-  MoveTensor t[2];      // K, V
-  MoveTensor sc[2];     // their scales: rows 1 of 4 bytes, or head_dim / 32 of 1 byte; rows 0: none
-  int slices[2];        // 32-row slices of K and V
-  int run;              // new positions a CTA works out at a time
+  MoveTensor t[2];   // K, V
+  MoveTensor sc[2];  // their scales: 1 row of 4 bytes or head_dim / 32 rows of 1 byte; 0 rows: none
+  int split;         // CTAs that share the rows of a KV head
+  int run;           // new positions that a CTA plans at a time
+  int ring;          // slabs in flight
+  uint32_t slot_bytes, ring_at, smem;
 };
 
-struct MovePlan {           // of one run of new positions, in shared memory
-  int2 entry[kMoveRun + kMoveRing];  // page (or -1) and 16-byte group of the page of an old group
-  uint2 piece[kMoveRun + 2];  // selectors {of the low 8 source bytes | high 8 << 16, which of the two | keep or take << 16} + flags
-  int to[kMoveRun / 4];     // new page of every new group
-  uint32_t have[kMoveRun / 4];  // which of a group's tokens there are
-  int kept[kMoveRun];
-  uint32_t scan[2][kMoveThreads / 32];
-  int n_entries, n_pieces;
+struct MovePlan {                 // of one run of new positions
+  uint32_t tok[kMoveRun + 16];    // a token's page in the list below << 8 | its place in that page
+  int page_blk[kMoveRun];         // pages that hold kept tokens, in order; -1: not in the pool
+  int to[kMoveRun / 16];          // new pages, -1: not in the pool
+  uint32_t there[kMoveRun / 32];  // which new positions have a token to move
+  uint32_t scan[kMoveThreads / 32];
+  int n_pages;
 };
-// flags of a piece, in bits that no selector uses
-constexpr uint32_t kNewEntry = 0x80000000u, kWordEnd = 0x8000u;
 
-template <int EB>
 __device__ void plan_run(const EvictArgs& a, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx) {
-  constexpr int G = 16 / EB, WT = 4 / EB;  // tokens of a group, of a word
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int j = tid; j < n; j += kMoveThreads) pl.kept[j] = kept[p0 + j];
-  __syncthreads();
-  uint32_t base_e = 0, base_p = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, shift = 31 - __clz(a.page);
+  uint32_t base = 0;
   for (int j0 = 0; j0 < n; j0 += kMoveThreads) {
     const int j = j0 + tid;
-    const int t = j < n ? pl.kept[j] : -1, prev = j > 0 && j < n ? pl.kept[j - 1] : -1;
-    const bool first_e = j < n && (j % G == 0 || t / G != prev / G);
-    const bool first_p = j < n && (first_e || j % WT == 0);
-    int blk = (t >= 0 && t < ctx) ? bt[t / a.page] : -1;
-    int to = j < n ? nbt[(p0 + j) / a.page] : -1;
-    if (blk >= a.num_blocks || to >= a.num_blocks || ((blk < 0 || to < 0) && j < n)) {
-      if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
-      if (blk >= a.num_blocks) blk = -1;
-      if (to >= a.num_blocks) to = -1;
-    }
+    const int t = j < n ? kept[p0 + j] : -1, prev = j > 0 && j < n ? kept[p0 + j - 1] : -1;
+    const bool first = j < n && (j == 0 || (t >> shift) != (prev >> shift));
+    int blk = (t >= 0 && t < ctx) ? bt[t >> shift] : -1, to = j < n ? nbt[(p0 + j) >> shift] : -1;
+    if (blk >= a.num_blocks) blk = -1;
+    if (to >= a.num_blocks) to = -1;
+    if (j < n && (blk < 0 || to < 0) && a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
     const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0 && to >= 0);
-    if (j < n && j % G == 0) {
-      pl.to[j / G] = to;
-      pl.have[j / G] = there >> lane & ((1u << G) - 1);
-    }
-    uint32_t e = first_e, p = first_p;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, e, o), y = __shfl_up_sync(0xffffffffu, p, o);
-      if (lane >= o) {
-        e += x;
-        p += y;
-      }
-    }
-    if (lane == 31) {
-      pl.scan[0][warp] = e;
-      pl.scan[1][warp] = p;
+    const uint32_t starts = __ballot_sync(0xffffffffu, first);
+    if (lane == 0) {
+      pl.scan[warp] = __popc(starts);
+      if (j < n) pl.there[j >> 5] = there;
     }
     __syncthreads();
-    uint32_t be = base_e, bp = base_p;
+    uint32_t u = base + __popc(starts & ((2u << lane) - 1)) - 1;
 #pragma unroll
     for (int w = 0; w < kMoveThreads / 32; ++w) {
-      if (w < warp) {
-        be += pl.scan[0][w];
-        bp += pl.scan[1][w];
-      }
-      base_e += pl.scan[0][w];
-      base_p += pl.scan[1][w];
+      if (w < warp) u += pl.scan[w];
+      base += pl.scan[w];
     }
-    if (first_e) pl.entry[e + be - 1] = make_int2(blk, t % a.page / G);
-    if (first_p) {  // the tokens of this piece: same word, same old group
-      uint32_t lo = 0, hi = 0, pick = 0, take = 0x3210;
-      int k = j;
-      do {
-        const int from0 = pl.kept[k] % G * EB, to0 = k % WT * EB;
-#pragma unroll
-        for (int x = 0; x < EB; ++x) {
-          const int from = from0 + x, at = 4 * (to0 + x);
-          if (from < 8) lo |= (uint32_t)from << at;
-          else hi |= (uint32_t)(from - 8) << at;
-          pick |= (uint32_t)((from < 8 ? 0 : 4) + to0 + x) << at;
-          take |= 4u << at;
-        }
-        ++k;
-      } while (k < n && k % WT != 0 && pl.kept[k] / G == t / G);
-      pl.piece[p + bp - 1] = make_uint2(lo | hi << 16, pick | take << 16 | (first_e ? kNewEntry : 0u) | (k % WT == 0 || k == n ? kWordEnd : 0u));
+    if (j < n) {
+      pl.tok[j] = u << 8 | (uint32_t)(t & (a.page - 1));
+      if (first) pl.page_blk[u] = blk;
+      if ((j & (a.page - 1)) == 0) pl.to[j >> shift] = to;
     }
     __syncthreads();
   }
-  if (tid == 0) {
-    pl.n_entries = (int)base_e;
-    pl.n_pieces = (int)base_p;
-  }
-  for (int x = tid; x < kMoveRing; x += kMoveThreads) pl.entry[base_e + x] = make_int2(-1, 0);
-  if (tid < 2) pl.piece[base_p + tid] = make_uint2(0, 0);
+  if (tid == 0) pl.n_pages = (int)base;
+  if (tid < 16) pl.tok[n + tid] = (base - 1) << 8;  // the last group read whole
   __syncthreads();
 }
 
-template <int EB>
-__device__ __forceinline__ void move_slice(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int row, int h, int p0, uint32_t ring) {
-  constexpr int G = 16 / EB;
-  const int n_pieces = pl.n_pieces;
-  const bool live = row < mt.rows;
-  const uint32_t row_bytes = a.page * EB;
-  const long long head_bytes = (long long)mt.rows * row_bytes, page_bytes = head_bytes * a.Hkv;
-  uint8_t* const base = static_cast<uint8_t*>(mt.p) + h * head_bytes + (long long)row * row_bytes;
-  const uint32_t mine = ring + (threadIdx.x & 31) * 16;
-  auto request = [&](int e, int slot) {  // (behind the last entry lie kMoveRing that copy nothing)
-    const int2 src = pl.entry[e];
-    if (live && src.x >= 0)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(mine + slot * 512), "l"(base + src.x * page_bytes + src.y * 16) : "memory");
-    cp_async_commit();
-  };
-#pragma unroll 1
-  for (int e = 0; e < kMoveRing - 1; ++e) request(e < pl.n_entries ? e : pl.n_entries, e);
-  int e = -1, slot = kMoveRing - 1, words = 0, g = 0;  // `slot`: where entry e + kMoveRing goes
-  uint4 src = make_uint4(0, 0, 0, 0), ahead;
-  cp_async_wait<kMoveRing - 2>();
-  ahead = lds128(mine);
-  uint32_t cur = 0, o0 = 0, o1 = 0, o2 = 0, o3 = 0;
-  uint2 next = pl.piece[0];
-#pragma unroll 1
-  for (int q = 0; q < n_pieces; ++q) {
-    const uint2 pc = next;
-    next = pl.piece[q + 1];
-    if (pc.y & kNewEntry) {
-      ++e;
-      src = ahead;
-      // the slot of the entry before this one is free; the entry after this one is needed next
-      const int want = e + kMoveRing - 1;
-      request(want < pl.n_entries ? want : pl.n_entries, slot);
-      slot = (slot + 1) & (kMoveRing - 1);
-      cp_async_wait<kMoveRing - 2>();
-      ahead = lds128(mine + ((slot + 1) & (kMoveRing - 1)) * 512);
-    }
-    const uint32_t lo = prmt(src.x, src.y, pc.x), hi = prmt(src.z, src.w, pc.x >> 16);
-    cur = prmt(cur, prmt(lo, hi, pc.y & 0x7777u), (pc.y >> 16) & 0x7777u);
-    if (pc.y & kWordEnd) {
-      o0 = o1;
-      o1 = o2;
-      o2 = o3;
-      o3 = cur;
-      if (++words == 4 || q + 1 == n_pieces) {
-        while (words < 4) {  // the last group of a sequence may end early
-          o0 = o1;
-          o1 = o2;
-          o2 = o3;
-          o3 = 0;
-          ++words;
-        }
-        words = 0;
-        const uint32_t have = pl.have[g];
-        if (live && have) {
-          uint8_t* dst = base + pl.to[g] * page_bytes + ((p0 + g * G) & (a.page - 1)) * EB;
-          if (have == (1u << G) - 1) {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(o0, o1, o2, o3);
-          } else {
-            const uint32_t out[4] = {o0, o1, o2, o3};
-#pragma unroll
-            for (int k = 0; k < G; ++k)
-              if (have >> k & 1) {
-                if (EB == 1) dst[k] = (uint8_t)(out[k >> 2] >> (8 * (k & 3)));
-                else if (EB == 2) reinterpret_cast<uint16_t*>(dst)[k] = (uint16_t)(out[k >> 1] >> (16 * (k & 1)));
-                else reinterpret_cast<uint32_t*>(dst)[k] = out[k & 3];
-              }
-          }
-        }
-        ++g;
-      }
-    }
-  }
-  cp_async_wait<0>();
-  __syncwarp();
-}
-
-// scales: a lane takes a token
+// scales: a lane takes a token, 8 of them at a time (all loads before the stores: in place)
 template <typename E>
 __device__ __forceinline__ void move_scales(const EvictArgs& a, const MoveTensor& mt, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int h,
                                             int n, int p0, int ctx) {
-  const int lane = threadIdx.x & 31;
-  E* const p = static_cast<E*>(mt.p);
-  for (int j0 = 0; j0 < n; j0 += 32) {
-    const int j = j0 + lane;
-    const int t = j < n ? kept[p0 + j] : -1;
-    const int blk = (t >= 0 && t < ctx) ? bt[t / a.page] : -1, to = j < n ? nbt[(p0 + j) / a.page] : -1;
-    const bool fine = blk >= 0 && blk < a.num_blocks && to >= 0 && to < a.num_blocks;
+  const int lane = threadIdx.x & 31, shift = 31 - __clz(a.page);
+  E* const p = reinterpret_cast<E*>(mt.p);
+  for (int j0 = 0; j0 < n; j0 += 256) {
+    long long from[8], to[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int j = j0 + x * 32 + lane, t = j < n ? kept[p0 + j] : -1;
+      const int blk = (t >= 0 && t < ctx) ? bt[t >> shift] : -1, nb = j < n ? nbt[(p0 + j) >> shift] : -1;
+      const bool fine = blk >= 0 && blk < a.num_blocks && nb >= 0 && nb < a.num_blocks;
+      from[x] = fine ? ((long long)blk * a.Hkv + h) * mt.rows * a.page + (t & (a.page - 1)) : -1;
+      to[x] = ((long long)nb * a.Hkv + h) * mt.rows * a.page + ((p0 + j) & (a.page - 1));
+    }
     for (int r = 0; r < mt.rows; ++r) {
-      E x = 0;
-      if (fine) x = p[(((size_t)blk * a.Hkv + h) * mt.rows + r) * a.page + t % a.page];
+      E v[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = from[x] >= 0 ? p[from[x] + r * a.page] : (E)0;
       __syncwarp();
-      if (fine) p[(((size_t)to * a.Hkv + h) * mt.rows + r) * a.page + (p0 + j) % a.page] = x;
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (from[x] >= 0) p[to[x] + r * a.page] = v[x];
       __syncwarp();
     }
   }
 }
 
-template <int EB, typename ES>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const MoveArgs m) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  MovePlan& pl = *reinterpret_cast<MovePlan*>(smem);
+template <typename E>
+__device__ __forceinline__ E lds_elem(uint32_t at);
+template <>
+__device__ __forceinline__ uint8_t lds_elem<uint8_t>(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=h"(v) : "r"(at));
+  return (uint8_t)v;
+}
+template <>
+__device__ __forceinline__ uint16_t lds_elem<uint16_t>(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+  return v;
+}
+template <>
+__device__ __forceinline__ uint32_t lds_elem<uint32_t>(uint32_t at) { return lds32(at); }
+
+// E: an element of K and V, ES: of their scales
+template <typename E, typename ES>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ MoveArgs m) {
+  constexpr int EB = sizeof(E), G = 16 / EB, WT = 4 / EB;  // tokens of a group, of a word
+  extern __shared__ __align__(128) uint8_t smem[];
+  MovePlan& pl = *reinterpret_cast<MovePlan*>(smem + 1024);
   const EvictArgs& a = m.e;
-  const int h = blockIdx.y, s = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = smem_u32(smem), full = base, empty = base + 8 * kMoveMaxRing, ring = base + m.ring_at;
+  volatile int* fail_ptr = reinterpret_cast<volatile int*>(smem + 16 * kMoveMaxRing);
+  const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int part = blockIdx.x % m.split, run0 = blockIdx.x / m.split;
   const int ctx = evict_ctx(a, s, false), total = min(ctx, a.budget);
-  if (a.in_place && ctx <= a.budget) return;
-  const uint32_t ring = smem_u32(smem) + (uint32_t)((sizeof(MovePlan) + 15) & ~15) + warp * (kMoveRing * 512);
+  if (a.in_place ? ctx <= a.budget : run0 * m.run >= total) return;
   const int32_t* kept = a.kept + ((size_t)s * a.Hkv + h) * a.budget;
   const int32_t* bt = a.bt + (size_t)s * a.max_blocks;
   const int32_t* nbt = a.new_bt + (size_t)s * a.new_max_blocks;
-  for (int p0 = blockIdx.x * m.run; p0 < total; p0 += gridDim.x * m.run) {
+  if (tid == 0) {
+    for (int i = 0; i < m.ring; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, kMoveWarps);
+    }
+    *fail_ptr = 0;
+    mbar_fence_init();
+  }
+  const int row_bytes = a.page * EB, shift = 31 - __clz(a.page);
+  const int k_rows = m.t[0].rows / m.split, v_rows = m.t[1].rows / m.split, rows = k_rows + v_rows;  // of this CTA
+  const long long k_page = (long long)a.Hkv * m.t[0].rows * row_bytes, v_page = (long long)a.Hkv * m.t[1].rows * row_bytes;
+  uint8_t* const k_base = m.t[0].p + ((long long)h * m.t[0].rows + part * k_rows) * row_bytes;
+  uint8_t* const v_base = m.t[1].p + ((long long)h * m.t[1].rows + part * v_rows) * row_bytes;
+  int st = 0;          // ring slot and its phase, carried on from run to run by producer and warps alike
+  uint32_t par = 0;
+  auto step = [&]() {
+    if (++st == m.ring) {
+      st = 0;
+      par ^= 1;
+    }
+  };
+  bool dead = false;   // a wait ran out: nothing is moved any more, but the barriers of the block are kept
+  // in place: all runs of the head, one after another; else one
+  for (int p0 = run0 * m.run; p0 < total; p0 += a.in_place ? m.run : total) {
     const int n = min(m.run, total - p0);
-    plan_run<EB>(a, pl, kept, bt, nbt, p0, n, ctx);
-    const int slices = m.slices[0] + m.slices[1];
-    for (int task = warp; task < slices + 2; task += kMoveThreads / 32) {
-      if (task < m.slices[0]) move_slice<EB>(a, pl, m.t[0], task * 32 + lane, h, p0, ring);
-      else if (task < slices) move_slice<EB>(a, pl, m.t[1], (task - m.slices[0]) * 32 + lane, h, p0, ring);
-      else if (m.sc[task - slices].rows) move_scales<ES>(a, m.sc[task - slices], kept, bt, nbt, h, n, p0, ctx);
+    plan_run(a, pl, kept, bt, nbt, p0, n, ctx);
+    const int n_pages = pl.n_pages;
+    if (warp == kMoveWarps) {
+      if (lane == 0) {
+        for (int u = 0; u < n_pages; ++u) {
+          if (!dead && !tc_wait(empty + 8 * st, par ^ 1)) dead = true;
+          if (dead) break;
+          const int blk = pl.page_blk[u];
+          mbar_arrive_expect_tx(full + 8 * st, blk >= 0 ? (uint32_t)rows * row_bytes : 0u);
+          if (blk >= 0) {
+            bulk_g2s(ring + st * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * row_bytes, full + 8 * st);
+            bulk_g2s(ring + st * m.slot_bytes + k_rows * row_bytes, v_base + blk * v_page, (uint32_t)v_rows * row_bytes, full + 8 * st);
+          }
+          step();
+        }
+        if (dead) *fail_ptr = 1;
+      }
+    } else if (warp == kMoveWarps + 1) {
+      if (part == 0) {
+        if (m.sc[0].rows) move_scales<ES>(a, m.sc[0], kept, bt, nbt, h, n, p0, ctx);
+        if (m.sc[1].rows) move_scales<ES>(a, m.sc[1], kept, bt, nbt, h, n, p0, ctx);
+      }
+    } else {
+      const int r0 = rows * warp / kMoveWarps, r1 = rows * (warp + 1) / kMoveWarps;
+      const int my_row = r0 + (lane >> 2), w = lane & 3;
+      int ready = 0, first = 0, first_st = st;  // pages that have arrived; the first one still held, and its slot
+      for (int j0 = 0; j0 < n; j0 += G) {
+        const int last = (int)(pl.tok[min(j0 + G, n) - 1] >> 8);
+        while (ready <= last) {
+          if (!dead && !tc_wait(full + 8 * st, par)) {
+            dead = true;
+            *fail_ptr = 1;
+          }
+          ++ready;
+          step();
+        }
+        const int d = j0 >> shift, to = pl.to[d];
+        const uint32_t have = pl.there[j0 >> 5] >> (j0 & 31) & ((1u << G) - 1), mine = have >> (w * WT) & ((1u << WT) - 1);
+        uint32_t from[WT];
+#pragma unroll
+        for (int k = 0; k < WT; ++k) {
+          const uint32_t x = pl.tok[j0 + w * WT + k];
+          int slot = first_st + (int)(x >> 8) - first;
+          if (slot >= m.ring) slot -= m.ring;
+          from[k] = ring + slot * m.slot_bytes + (x & 255u) * EB;
+        }
+        uint8_t* const k_to = k_base + to * k_page + (j0 & (a.page - 1)) * EB + 4 * w;
+        uint8_t* const v_to = v_base + to * v_page + (j0 & (a.page - 1)) * EB + 4 * w - (long long)k_rows * row_bytes;
+        if (!dead) {
+#pragma unroll 4
+          for (int r = my_row; r < r1; r += 8) {
+            E x[WT];
+#pragma unroll
+            for (int k = 0; k < WT; ++k) x[k] = lds_elem<E>(from[k] + r * row_bytes);
+            uint8_t* const dst = (r < k_rows ? k_to : v_to) + r * row_bytes;
+            uint32_t word = x[0];
+#pragma unroll
+            for (int k = 1; k < WT; ++k) word |= (uint32_t)x[k] << (8 * EB * k);
+            if (mine == (1u << WT) - 1) {
+              *reinterpret_cast<uint32_t*>(dst) = word;
+            } else {
+#pragma unroll
+              for (int k = 0; k < WT; ++k)
+                if (mine >> k & 1) reinterpret_cast<E*>(dst)[k] = x[k];
+            }
+          }
+        }
+        // pages that the next group does not need any more
+        const int next = j0 + G < n ? (int)(pl.tok[j0 + G] >> 8) : n_pages;
+        if (first < next) __syncwarp();
+        for (; first < next; ++first) {
+          if (lane == 0) mbar_arrive(empty + 8 * first_st);
+          if (++first_st == m.ring) first_st = 0;
+        }
+      }
     }
     __syncthreads();
+    if (*fail_ptr) break;  // uniform: written before the barrier
+  }
+  if (tid == kMoveWarps * 32 && *fail_ptr) {
+    for (int i = 0; i < m.ring; ++i) mbar_wait(full + 8 * i, par ^ (i < st ? 0 : 1), 1);  // copies in flight land before the CTA ends
+    if (a.status) atomicOr(a.status, CUDA_LLM_ST_TIMEOUT);
   }
 }
 
-template <int EB, typename ES>
+template <typename E, typename ES>
 static cudaError_t launch_move(const MoveArgs& m, cudaStream_t st) {
-  auto kern = evict_move_kernel<EB, ES>;
-  const int smem = (int)((sizeof(MovePlan) + 15) & ~15) + kMoveThreads / 32 * kMoveRing * 512;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  auto kern = evict_move_kernel<E, ES>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)m.smem);
   if (e != cudaSuccess) return e;
   const unsigned runs = m.e.in_place ? 1u : (unsigned)((m.e.budget + m.run - 1) / m.run);
-  kern<<<dim3(runs, m.e.Hkv, m.e.S), kMoveThreads, smem, st>>>(m);
+  kern<<<dim3(runs * m.split, m.e.Hkv, m.e.S), kMoveThreads, m.smem, st>>>(m);
   return cudaGetLastError();
 }
 
@@ -538,15 +548,31 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   if (rc != CUDA_LLM_OK) return rc;
   const int D = p->head_dim, v_rows = p->v_format == CUDA_LLM_KV_FP4_E2M1 ? D / 2 : D;
   const int sc_rows = !scaled ? 0 : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? 1 : D / 32;
-  m.t[0] = MoveTensor{p->key_cache, D};
-  m.t[1] = MoveTensor{p->value_cache, v_rows};
-  m.sc[0] = MoveTensor{p->k_scale, sc_rows};
-  m.sc[1] = MoveTensor{p->v_scale, sc_rows};
-  m.slices[0] = D / 32;
-  m.slices[1] = v_rows / 32;
-  m.run = in_place ? kMoveRun : 256;
-  const int eb = format_bytes(p->k_format);
-  const cudaError_t e = eb == 4 ? launch_move<4, uint32_t>(m, st) : eb == 2 ? launch_move<2, uint32_t>(m, st)
-                        : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move<1, uint32_t>(m, st) : launch_move<1, uint8_t>(m, st);
+  m.t[0] = MoveTensor{(uint8_t*)p->key_cache, D};
+  m.t[1] = MoveTensor{(uint8_t*)p->value_cache, v_rows};
+  m.sc[0] = MoveTensor{(uint8_t*)p->k_scale, sc_rows};
+  m.sc[1] = MoveTensor{(uint8_t*)p->v_scale, sc_rows};
+  const int eb = format_bytes(p->k_format), row_bytes = a.page * eb;
+  const long long pairs = (long long)a.S * a.Hkv;
+  const int sms = current_sm_count(), group = 16 / eb;
+  auto slot = [&](int split) { return (uint32_t)(((D + v_rows) / split * row_bytes + 127) / 128 * 128); };
+  m.ring_at = (1024 + sizeof(MovePlan) + 127) / 128 * 128;
+  // The ring holds one slab more than a group has tokens, and about 64 KB.  Rows are split until two such rings fit an SM and,
+  // in place, until every SM has work; elsewhere there are runs of positions for that, as long as pays for their plan.
+  m.split = 1;
+  while (m.split < 8 && m.ring_at + (group + 1) * slot(m.split) > 112 * 1024) m.split *= 2;
+  m.run = kMoveRun;
+  if (in_place) {
+    while (m.split < 8 && pairs * m.split * 2 <= 2 * sms) m.split *= 2;
+  } else {
+    while (m.run > 256 && pairs * m.split * ((a.budget + m.run - 1) / m.run) < 2 * sms) m.run /= 2;
+  }
+  m.slot_bytes = slot(m.split);
+  m.ring = (int)(64 * 1024 / m.slot_bytes);
+  if (m.ring < group + 1) m.ring = group + 1;
+  if (m.ring > kMoveMaxRing) m.ring = kMoveMaxRing;
+  m.smem = m.ring_at + m.ring * m.slot_bytes;
+  const cudaError_t e = eb == 4 ? launch_move<uint32_t, uint32_t>(m, st) : eb == 2 ? launch_move<uint16_t, uint32_t>(m, st)
+                        : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move<uint8_t, uint32_t>(m, st) : launch_move<uint8_t, uint8_t>(m, st);
   return cuda_result(e, "evict_move_kernel launch");
 }
