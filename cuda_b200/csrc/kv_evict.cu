@@ -232,20 +232,29 @@ struct MoveArgs {
 };
 
 struct MovePlan {                 // of one run of new positions
-  uint32_t tok[kMoveRun + 16];    // a token's page in the list below << 8 | its place in that page
+  uint32_t addr[kMoveRun + 16];   // where in the ring a token's elements lie (those of the first row)
+  uint16_t page[kMoveRun];        // a token's page in the list below
+  uint8_t off[kMoveRun];          // its place in that page
   int page_blk[kMoveRun];         // pages that hold kept tokens, in order; -1: not in the pool
+  int4 group[kMoveRun / 4];       // 16 bytes of a row: last page needed, pages done with it, new page, tokens that there are
   int to[kMoveRun / 16];          // new pages, -1: not in the pool
   uint32_t there[kMoveRun / 32];  // which new positions have a token to move
   uint32_t scan[kMoveThreads / 32];
   int n_pages;
 };
 
-__device__ void plan_run(const EvictArgs& a, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx) {
+// `slot0`: ring slot of the run's first page
+template <int EB>
+__device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx, int slot0,
+                         uint32_t ring) {
+  constexpr int G = 16 / EB;
+  const EvictArgs& a = m.e;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, shift = 31 - __clz(a.page);
   uint32_t base = 0;
+  int t = tid < n ? kept[p0 + tid] : -1, prev = tid > 0 && tid < n ? kept[p0 + tid - 1] : -1;
   for (int j0 = 0; j0 < n; j0 += kMoveThreads) {
-    const int j = j0 + tid;
-    const int t = j < n ? kept[p0 + j] : -1, prev = j > 0 && j < n ? kept[p0 + j - 1] : -1;
+    const int j = j0 + tid, jn = j + kMoveThreads;
+    const int t_next = jn < n ? kept[p0 + jn] : -1, prev_next = jn < n ? kept[p0 + jn - 1] : -1;
     const bool first = j < n && (j == 0 || (t >> shift) != (prev >> shift));
     int blk = (t >= 0 && t < ctx) ? bt[t >> shift] : -1, to = j < n ? nbt[(p0 + j) >> shift] : -1;
     if (blk >= a.num_blocks) blk = -1;
@@ -265,32 +274,42 @@ __device__ void plan_run(const EvictArgs& a, MovePlan& pl, const int32_t* kept, 
       base += pl.scan[w];
     }
     if (j < n) {
-      pl.tok[j] = u << 8 | (uint32_t)(t & (a.page - 1));
+      pl.addr[j] = ring + (slot0 + u) % (uint32_t)m.ring * m.slot_bytes + (uint32_t)(t & (a.page - 1)) * EB;
+      pl.page[j] = (uint16_t)u;
+      pl.off[j] = (uint8_t)(t & (a.page - 1));
       if (first) pl.page_blk[u] = blk;
       if ((j & (a.page - 1)) == 0) pl.to[j >> shift] = to;
     }
+    t = t_next;
+    prev = prev_next;
     __syncthreads();
   }
+  if (tid < 16) pl.addr[n + tid] = ring;  // the last group is read whole
   if (tid == 0) pl.n_pages = (int)base;
-  if (tid < 16) pl.tok[n + tid] = (base - 1) << 8;  // the last group read whole
+  for (int g = tid; g * G < n; g += kMoveThreads) {
+    const int j = g * G;
+    pl.group[g] = make_int4(pl.page[min(j + G, n) - 1], j + G < n ? pl.page[j + G] : (int)base, pl.to[j >> shift],
+                            (int)(pl.there[j >> 5] >> (j & 31) & ((1u << G) - 1)));
+  }
   __syncthreads();
 }
 
 // scales: a lane takes a token, 8 of them at a time (all loads before the stores: in place)
 template <typename E>
-__device__ __forceinline__ void move_scales(const EvictArgs& a, const MoveTensor& mt, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int h,
-                                            int n, int p0, int ctx) {
+__device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int h, int n, int p0) {
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.page);
   E* const p = reinterpret_cast<E*>(mt.p);
   for (int j0 = 0; j0 < n; j0 += 256) {
     long long from[8], to[8];
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      const int j = j0 + x * 32 + lane, t = j < n ? kept[p0 + j] : -1;
-      const int blk = (t >= 0 && t < ctx) ? bt[t >> shift] : -1, nb = j < n ? nbt[(p0 + j) >> shift] : -1;
-      const bool fine = blk >= 0 && blk < a.num_blocks && nb >= 0 && nb < a.num_blocks;
-      from[x] = fine ? ((long long)blk * a.Hkv + h) * mt.rows * a.page + (t & (a.page - 1)) : -1;
-      to[x] = ((long long)nb * a.Hkv + h) * mt.rows * a.page + ((p0 + j) & (a.page - 1));
+      const int j = j0 + x * 32 + lane;
+      from[x] = -1;
+      to[x] = 0;
+      if (j < n && (pl.there[j >> 5] >> (j & 31) & 1)) {
+        from[x] = ((long long)pl.page_blk[pl.page[j]] * a.Hkv + h) * mt.rows * a.page + pl.off[j];
+        to[x] = ((long long)pl.to[j >> shift] * a.Hkv + h) * mt.rows * a.page + ((p0 + j) & (a.page - 1));
+      }
     }
     for (int r = 0; r < mt.rows; ++r) {
       E v[8];
@@ -305,27 +324,26 @@ __device__ __forceinline__ void move_scales(const EvictArgs& a, const MoveTensor
   }
 }
 
-template <typename E>
-__device__ __forceinline__ E lds_elem(uint32_t at);
-template <>
-__device__ __forceinline__ uint8_t lds_elem<uint8_t>(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=h"(v) : "r"(at));
-  return (uint8_t)v;
+// 4 bytes of a new row: 4, 2 or 1 elements from their places in the ring
+template <int EB>
+__device__ __forceinline__ uint32_t gather_word(const uint32_t (&from)[4 / EB], uint32_t offset) {
+  if constexpr (EB == 4) {
+    return lds32(from[0] + offset);
+  } else if constexpr (EB == 2) {
+    return prmt(lds16(from[0] + offset), lds16(from[1] + offset), 0x5410);
+  } else {
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x[k]) : "r"(from[k] + offset));
+    return prmt(prmt(x[0], x[1], 0x0040), prmt(x[2], x[3], 0x0040), 0x5410);
+  }
 }
-template <>
-__device__ __forceinline__ uint16_t lds_elem<uint16_t>(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
-  return v;
-}
-template <>
-__device__ __forceinline__ uint32_t lds_elem<uint32_t>(uint32_t at) { return lds32(at); }
 
 // E: an element of K and V, ES: of their scales
-template <typename E, typename ES>
+template <typename E, typename ES, int PAGE>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ MoveArgs m) {
   constexpr int EB = sizeof(E), G = 16 / EB, WT = 4 / EB;  // tokens of a group, of a word
+  constexpr int ROW = PAGE * EB;                           // bytes of a row
   extern __shared__ __align__(128) uint8_t smem[];
   MovePlan& pl = *reinterpret_cast<MovePlan*>(smem + 1024);
   const EvictArgs& a = m.e;
@@ -346,12 +364,11 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     *fail_ptr = 0;
     mbar_fence_init();
   }
-  const int row_bytes = a.page * EB, shift = 31 - __clz(a.page);
-  const int k_rows = m.t[0].rows / m.split, v_rows = m.t[1].rows / m.split, rows = k_rows + v_rows;  // of this CTA
-  const long long k_page = (long long)a.Hkv * m.t[0].rows * row_bytes, v_page = (long long)a.Hkv * m.t[1].rows * row_bytes;
-  uint8_t* const k_base = m.t[0].p + ((long long)h * m.t[0].rows + part * k_rows) * row_bytes;
-  uint8_t* const v_base = m.t[1].p + ((long long)h * m.t[1].rows + part * v_rows) * row_bytes;
-  int st = 0;          // ring slot and its phase, carried on from run to run by producer and warps alike
+  const int k_rows = m.t[0].rows / m.split, v_rows = m.t[1].rows / m.split;  // of this CTA
+  const long long k_page = (long long)a.Hkv * m.t[0].rows * ROW, v_page = (long long)a.Hkv * m.t[1].rows * ROW;
+  uint8_t* const k_base = m.t[0].p + ((long long)h * m.t[0].rows + part * k_rows) * ROW;
+  uint8_t* const v_base = m.t[1].p + ((long long)h * m.t[1].rows + part * v_rows) * ROW;
+  int st = 0, slot0 = 0;  // ring slot and its phase, carried on from run to run by producer and warps alike
   uint32_t par = 0;
   auto step = [&]() {
     if (++st == m.ring) {
@@ -359,22 +376,23 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
       par ^= 1;
     }
   };
-  bool dead = false;   // a wait ran out: nothing is moved any more, but the barriers of the block are kept
+  bool dead = false;      // a wait ran out: nothing is moved any more, but the barriers of the block are kept
   // in place: all runs of the head, one after another; else one
   for (int p0 = run0 * m.run; p0 < total; p0 += a.in_place ? m.run : total) {
     const int n = min(m.run, total - p0);
-    plan_run(a, pl, kept, bt, nbt, p0, n, ctx);
+    plan_run<EB>(m, pl, kept, bt, nbt, p0, n, ctx, slot0, ring);
     const int n_pages = pl.n_pages;
+    slot0 = (slot0 + n_pages) % m.ring;
     if (warp == kMoveWarps) {
       if (lane == 0) {
         for (int u = 0; u < n_pages; ++u) {
-          if (!dead && !tc_wait(empty + 8 * st, par ^ 1)) dead = true;
+          if (!dead && !mbar_wait(empty + 8 * st, par ^ 1, 0)) dead = true;
           if (dead) break;
           const int blk = pl.page_blk[u];
-          mbar_arrive_expect_tx(full + 8 * st, blk >= 0 ? (uint32_t)rows * row_bytes : 0u);
+          mbar_arrive_expect_tx(full + 8 * st, blk >= 0 ? (uint32_t)(k_rows + v_rows) * ROW : 0u);
           if (blk >= 0) {
-            bulk_g2s(ring + st * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * row_bytes, full + 8 * st);
-            bulk_g2s(ring + st * m.slot_bytes + k_rows * row_bytes, v_base + blk * v_page, (uint32_t)v_rows * row_bytes, full + 8 * st);
+            bulk_g2s(ring + st * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * ROW, full + 8 * st);
+            bulk_g2s(ring + st * m.slot_bytes + k_rows * ROW, v_base + blk * v_page, (uint32_t)v_rows * ROW, full + 8 * st);
           }
           step();
         }
@@ -382,60 +400,54 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
       }
     } else if (warp == kMoveWarps + 1) {
       if (part == 0) {
-        if (m.sc[0].rows) move_scales<ES>(a, m.sc[0], kept, bt, nbt, h, n, p0, ctx);
-        if (m.sc[1].rows) move_scales<ES>(a, m.sc[1], kept, bt, nbt, h, n, p0, ctx);
+        if (m.sc[0].rows) move_scales<ES>(a, pl, m.sc[0], h, n, p0);
+        if (m.sc[1].rows) move_scales<ES>(a, pl, m.sc[1], h, n, p0);
       }
     } else {
-      const int r0 = rows * warp / kMoveWarps, r1 = rows * (warp + 1) / kMoveWarps;
-      const int my_row = r0 + (lane >> 2), w = lane & 3;
+      // rows of this warp, the same share of K and of V; a lane owns one word of every eighth row
+      const int row = lane >> 2, w = lane & 3;
+      const int k0 = k_rows * warp / kMoveWarps + row, k1 = k_rows * (warp + 1) / kMoveWarps;
+      const int v0 = v_rows * warp / kMoveWarps + row, v1 = v_rows * (warp + 1) / kMoveWarps;
       int ready = 0, first = 0, first_st = st;  // pages that have arrived; the first one still held, and its slot
       for (int j0 = 0; j0 < n; j0 += G) {
-        const int last = (int)(pl.tok[min(j0 + G, n) - 1] >> 8);
-        while (ready <= last) {
+        const int4 grp = pl.group[j0 / G];
+        uint32_t from[WT];
+#pragma unroll
+        for (int k = 0; k < WT; ++k) from[k] = pl.addr[j0 + w * WT + k];
+        for (; ready <= grp.x; ++ready) {
           if (!dead && !tc_wait(full + 8 * st, par)) {
             dead = true;
             *fail_ptr = 1;
           }
-          ++ready;
           step();
         }
-        const int d = j0 >> shift, to = pl.to[d];
-        const uint32_t have = pl.there[j0 >> 5] >> (j0 & 31) & ((1u << G) - 1), mine = have >> (w * WT) & ((1u << WT) - 1);
-        uint32_t from[WT];
-#pragma unroll
-        for (int k = 0; k < WT; ++k) {
-          const uint32_t x = pl.tok[j0 + w * WT + k];
-          int slot = first_st + (int)(x >> 8) - first;
-          if (slot >= m.ring) slot -= m.ring;
-          from[k] = ring + slot * m.slot_bytes + (x & 255u) * EB;
-        }
-        uint8_t* const k_to = k_base + to * k_page + (j0 & (a.page - 1)) * EB + 4 * w;
-        uint8_t* const v_to = v_base + to * v_page + (j0 & (a.page - 1)) * EB + 4 * w - (long long)k_rows * row_bytes;
-        if (!dead) {
-#pragma unroll 4
-          for (int r = my_row; r < r1; r += 8) {
-            E x[WT];
-#pragma unroll
-            for (int k = 0; k < WT; ++k) x[k] = lds_elem<E>(from[k] + r * row_bytes);
-            uint8_t* const dst = (r < k_rows ? k_to : v_to) + r * row_bytes;
-            uint32_t word = x[0];
-#pragma unroll
-            for (int k = 1; k < WT; ++k) word |= (uint32_t)x[k] << (8 * EB * k);
-            if (mine == (1u << WT) - 1) {
-              *reinterpret_cast<uint32_t*>(dst) = word;
-            } else {
-#pragma unroll
-              for (int k = 0; k < WT; ++k)
-                if (mine >> k & 1) reinterpret_cast<E*>(dst)[k] = x[k];
-            }
+        const uint32_t in_page = ((uint32_t)j0 & (PAGE - 1)) * EB + 4 * w;
+        uint8_t* const k_to = k_base + grp.z * k_page + in_page;
+        uint8_t* const v_to = v_base + grp.z * v_page + in_page;
+        if (grp.w == (1 << G) - 1 && !dead) {
+#pragma unroll 2
+          for (int r = k0; r < k1; r += 8) *reinterpret_cast<uint32_t*>(k_to + r * ROW) = gather_word<EB>(from, r * ROW);
+#pragma unroll 2
+          for (int r = v0; r < v1; r += 8) *reinterpret_cast<uint32_t*>(v_to + r * ROW) = gather_word<EB>(from, (k_rows + r) * ROW);
+        } else if (grp.w && !dead) {  // the end of a sequence, or a page that is not in the pool
+          const uint32_t mine = (uint32_t)grp.w >> (w * WT);
+          for (int r = k0; r < k1; r += 8) {
+            const uint32_t word = gather_word<EB>(from, r * ROW);
+            for (int k = 0; k < WT; ++k)
+              if (mine >> k & 1) reinterpret_cast<E*>(k_to + r * ROW)[k] = (E)(word >> (8 * EB * k));
+          }
+          for (int r = v0; r < v1; r += 8) {
+            const uint32_t word = gather_word<EB>(from, (k_rows + r) * ROW);
+            for (int k = 0; k < WT; ++k)
+              if (mine >> k & 1) reinterpret_cast<E*>(v_to + r * ROW)[k] = (E)(word >> (8 * EB * k));
           }
         }
-        // pages that the next group does not need any more
-        const int next = j0 + G < n ? (int)(pl.tok[j0 + G] >> 8) : n_pages;
-        if (first < next) __syncwarp();
-        for (; first < next; ++first) {
-          if (lane == 0) mbar_arrive(empty + 8 * first_st);
-          if (++first_st == m.ring) first_st = 0;
+        if (first < grp.y) {  // pages that the next group does not need any more
+          __syncwarp();
+          for (; first < grp.y; ++first) {
+            if (lane == 0) mbar_arrive(empty + 8 * first_st);
+            if (++first_st == m.ring) first_st = 0;
+          }
         }
       }
     }
@@ -448,14 +460,18 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   }
 }
 
-template <typename E, typename ES>
+template <typename E, typename ES, int PAGE>
 static cudaError_t launch_move(const MoveArgs& m, cudaStream_t st) {
-  auto kern = evict_move_kernel<E, ES>;
+  auto kern = evict_move_kernel<E, ES, PAGE>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)m.smem);
   if (e != cudaSuccess) return e;
   const unsigned runs = m.e.in_place ? 1u : (unsigned)((m.e.budget + m.run - 1) / m.run);
   kern<<<dim3(runs * m.split, m.e.Hkv, m.e.S), kMoveThreads, m.smem, st>>>(m);
   return cudaGetLastError();
+}
+template <typename E, typename ES>
+static cudaError_t launch_move_page(const MoveArgs& m, cudaStream_t st) {
+  return m.e.page == 16 ? launch_move<E, ES, 16>(m, st) : m.e.page == 32 ? launch_move<E, ES, 32>(m, st) : launch_move<E, ES, 64>(m, st);
 }
 
 template <int THREADS>
@@ -572,7 +588,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   if (m.ring < group + 1) m.ring = group + 1;
   if (m.ring > kMoveMaxRing) m.ring = kMoveMaxRing;
   m.smem = m.ring_at + m.ring * m.slot_bytes;
-  const cudaError_t e = eb == 4 ? launch_move<uint32_t, uint32_t>(m, st) : eb == 2 ? launch_move<uint16_t, uint32_t>(m, st)
-                        : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move<uint8_t, uint32_t>(m, st) : launch_move<uint8_t, uint8_t>(m, st);
+  const cudaError_t e = eb == 4 ? launch_move_page<uint32_t, uint32_t>(m, st) : eb == 2 ? launch_move_page<uint16_t, uint32_t>(m, st)
+                        : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move_page<uint8_t, uint32_t>(m, st) : launch_move_page<uint8_t, uint8_t>(m, st);
   return cuda_result(e, "evict_move_kernel launch");
 }
