@@ -243,6 +243,13 @@ struct MovePlan {                 // of one run of new positions
   int n_pages;
 };
 
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+
 // `slot0`: ring slot of the run's first page
 template <int EB>
 __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx, int slot0,
@@ -384,20 +391,33 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     const int n_pages = pl.n_pages;
     slot0 = (slot0 + n_pages) % m.ring;
     if (warp == kMoveWarps) {
-      if (lane == 0) {
-        for (int u = 0; u < n_pages; ++u) {
-          if (!dead && !mbar_wait(empty + 8 * st, par ^ 1, 0)) dead = true;
-          if (dead) break;
-          const int blk = pl.page_blk[u];
-          mbar_arrive_expect_tx(full + 8 * st, blk >= 0 ? (uint32_t)(k_rows + v_rows) * ROW : 0u);
-          if (blk >= 0) {
-            bulk_g2s(ring + st * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * ROW, full + 8 * st);
-            bulk_g2s(ring + st * m.slot_bytes + k_rows * ROW, v_base + blk * v_page, (uint32_t)v_rows * ROW, full + 8 * st);
+      // a lane per page, up to 16 at a time: one thread alone would spend longer on a page than the copy takes.  A lane issues as soon as
+      // its own slot is free, whatever the others wait for (the first pages of a batch may have to pass for the last
+      // ones to get their slots).
+      const int batch = min(16, m.ring);  // no two lanes on one slot
+      for (int u0 = 0; u0 < n_pages && !dead; u0 += batch) {
+        const int u = u0 + lane;
+        bool open = lane < batch && u < n_pages;
+        const int slot = (st + lane) % m.ring;
+        const uint32_t wait_for = par ^ 1 ^ ((uint32_t)((st + lane) / m.ring) & 1u);
+        const int blk = open ? pl.page_blk[u] : -1;
+        for (uint32_t polls = 0; __any_sync(0xffffffffu, open); ++polls) {
+          if (polls > (1u << 22)) {
+            dead = true;
+            break;
           }
-          step();
+          if (open && mbar_test(empty + 8 * slot, wait_for)) {
+            open = false;
+            mbar_arrive_expect_tx(full + 8 * slot, blk >= 0 ? (uint32_t)(k_rows + v_rows) * ROW : 0u);
+            if (blk >= 0) {
+              bulk_g2s(ring + slot * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * ROW, full + 8 * slot);
+              bulk_g2s(ring + slot * m.slot_bytes + k_rows * ROW, v_base + blk * v_page, (uint32_t)v_rows * ROW, full + 8 * slot);
+            }
+          }
         }
-        if (dead) *fail_ptr = 1;
+        for (int x = min(batch, n_pages - u0); x > 0; --x) step();
       }
+      if (dead && lane == 0) *fail_ptr = 1;
     } else if (warp == kMoveWarps + 1) {
       if (part == 0) {
         if (m.sc[0].rows) move_scales<ES>(a, pl, m.sc[0], h, n, p0);
