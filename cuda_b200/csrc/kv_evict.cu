@@ -428,48 +428,85 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
       const int row = lane >> 2, w = lane & 3;
       const int k0 = k_rows * warp / kMoveWarps + row, k1 = k_rows * (warp + 1) / kMoveWarps;
       const int v0 = v_rows * warp / kMoveWarps + row, v1 = v_rows * (warp + 1) / kMoveWarps;
-      int ready = 0, first = 0, first_st = st;  // pages that have arrived; the first one still held, and its slot
-      for (int j0 = 0; j0 < n; j0 += G) {
-        const int4 grp = pl.group[j0 / G];
-        uint32_t from[WT];
+      int ready = 0, first = 0, first_st = st;  // pages that have arrived; the first one still held, its slot and phase
+      uint32_t first_par = par;
+      for (int j0 = 0; j0 < n;) {
+        // two groups at a time where the ring can hold all their pages: what a group costs a warp is latency
+        const int4 ga = pl.group[j0 / G];
+        int4 gb = j0 + G < n ? pl.group[j0 / G + 1] : ga;
+        const bool two = j0 + G < n && gb.x - first < m.ring;
+        if (!two) gb = ga;
+        uint32_t fa[WT], fb[WT];
 #pragma unroll
-        for (int k = 0; k < WT; ++k) from[k] = pl.addr[j0 + w * WT + k];
-        for (; ready <= grp.x; ++ready) {
-          if (!dead && !tc_wait(full + 8 * st, par)) {
-            dead = true;
-            *fail_ptr = 1;
-          }
-          step();
+        for (int k = 0; k < WT; ++k) {
+          fa[k] = pl.addr[j0 + w * WT + k];
+          fb[k] = pl.addr[j0 + (two ? G : 0) + w * WT + k];
         }
-        const uint32_t in_page = ((uint32_t)j0 & (PAGE - 1)) * EB + 4 * w;
-        uint8_t* const k_to = k_base + grp.z * k_page + in_page;
-        uint8_t* const v_to = v_base + grp.z * v_page + in_page;
-        if (grp.w == (1 << G) - 1 && !dead) {
-#pragma unroll 2
-          for (int r = k0; r < k1; r += 8) *reinterpret_cast<uint32_t*>(k_to + r * ROW) = gather_word<EB>(from, r * ROW);
-#pragma unroll 2
-          for (int r = v0; r < v1; r += 8) *reinterpret_cast<uint32_t*>(v_to + r * ROW) = gather_word<EB>(from, (k_rows + r) * ROW);
-        } else if (grp.w && !dead) {  // the end of a sequence, or a page that is not in the pool
-          const uint32_t mine = (uint32_t)grp.w >> (w * WT);
-          for (int r = k0; r < k1; r += 8) {
-            const uint32_t word = gather_word<EB>(from, r * ROW);
-            for (int k = 0; k < WT; ++k)
-              if (mine >> k & 1) reinterpret_cast<E*>(k_to + r * ROW)[k] = (E)(word >> (8 * EB * k));
+        if (!dead && ready <= gb.x) {  // a lane per page
+          const int page = ready + lane, slot = first_st + page - first;
+          const bool wrap = slot >= m.ring;
+          bool open = page <= gb.x;
+          for (uint32_t polls = 0; __any_sync(0xffffffffu, open); ++polls) {
+            if (open && mbar_test(full + 8 * (wrap ? slot - m.ring : slot), first_par ^ (wrap ? 1u : 0u))) open = false;
+            if (polls > (1u << 22)) {
+              dead = true;
+              *fail_ptr = 1;
+              break;
+            }
           }
-          for (int r = v0; r < v1; r += 8) {
-            const uint32_t word = gather_word<EB>(from, (k_rows + r) * ROW);
-            for (int k = 0; k < WT; ++k)
-              if (mine >> k & 1) reinterpret_cast<E*>(v_to + r * ROW)[k] = (E)(word >> (8 * EB * k));
+          ready = gb.x + 1;
+        }
+        const uint32_t in_a = ((uint32_t)j0 & (PAGE - 1)) * EB + 4 * w, in_b = ((uint32_t)(j0 + G) & (PAGE - 1)) * EB + 4 * w;
+        uint8_t* const ka = k_base + ga.z * k_page + in_a;
+        uint8_t* const va = v_base + ga.z * v_page + in_a;
+        uint8_t* const kb = k_base + gb.z * k_page + in_b;
+        uint8_t* const vb = v_base + gb.z * v_page + in_b;
+        if (two && ga.w == (1 << G) - 1 && gb.w == (1 << G) - 1 && !dead) {
+          auto rows = [&](int r0, int r1, uint32_t slab, uint8_t* to_a, uint8_t* to_b) {
+#pragma unroll 2
+            for (int r = r0; r < r1; r += 8) {
+              const uint32_t x = gather_word<EB>(fa, slab + r * ROW), y = gather_word<EB>(fb, slab + r * ROW);
+              *reinterpret_cast<uint32_t*>(to_a + r * ROW) = x;
+              *reinterpret_cast<uint32_t*>(to_b + r * ROW) = y;
+            }
+          };
+          rows(k0, k1, 0, ka, kb);
+          rows(v0, v1, k_rows * ROW, va, vb);
+        } else if (!dead) {  // one group, the end of a sequence, or a page that is not in the pool
+          auto rows = [&](int r0, int r1, uint32_t slab, const uint32_t (&from)[WT], uint8_t* to, uint32_t have) {
+            for (int r = r0; r < r1; r += 8) {
+              const uint32_t word = gather_word<EB>(from, slab + r * ROW);
+              if (have == (1u << G) - 1) {
+                *reinterpret_cast<uint32_t*>(to + r * ROW) = word;
+                continue;
+              }
+              for (int k = 0; k < WT; ++k)
+                if (have >> (w * WT + k) & 1) reinterpret_cast<E*>(to + r * ROW)[k] = (E)(word >> (8 * EB * k));
+            }
+          };
+          rows(k0, k1, 0, fa, ka, (uint32_t)ga.w);
+          rows(v0, v1, k_rows * ROW, fa, va, (uint32_t)ga.w);
+          if (two) {
+            rows(k0, k1, 0, fb, kb, (uint32_t)gb.w);
+            rows(v0, v1, k_rows * ROW, fb, vb, (uint32_t)gb.w);
           }
         }
-        if (first < grp.y) {  // pages that the next group does not need any more
+        j0 += two ? 2 * G : G;
+        const int done = gb.y - first;  // pages that the next group does not need any more
+        if (done > 0) {
           __syncwarp();
-          for (; first < grp.y; ++first) {
-            if (lane == 0) mbar_arrive(empty + 8 * first_st);
-            if (++first_st == m.ring) first_st = 0;
+          const int slot = first_st + lane;
+          if (lane < done) mbar_arrive(empty + 8 * (slot >= m.ring ? slot - m.ring : slot));
+          first = gb.y;
+          first_st += done;
+          if (first_st >= m.ring) {
+            first_st -= m.ring;
+            first_par ^= 1;
           }
         }
       }
+      st = first_st;
+      par = first_par;
     }
     __syncthreads();
     if (*fail_ptr) break;  // uniform: written before the barrier
