@@ -228,6 +228,7 @@ struct MoveArgs {
   int split;         // CTAs that share the rows of a KV head
   int run;           // new positions that a CTA plans at a time
   int ring;          // slabs in flight
+  int teams;         // of warps, which take the groups in turn
   uint32_t slot_bytes, ring_at, smem;
 };
 
@@ -257,13 +258,25 @@ __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, c
   constexpr int G = 16 / EB;
   const EvictArgs& a = m.e;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, shift = 31 - __clz(a.page);
+  int* const tokens = reinterpret_cast<int*>(pl.addr);  // (a place in addr is overwritten by the thread that has read it last)
+  for (int j = tid; j < n; j += kMoveThreads) tokens[j] = kept[p0 + j];
+  __syncthreads();
   uint32_t base = 0;
-  int t = tid < n ? kept[p0 + tid] : -1, prev = tid > 0 && tid < n ? kept[p0 + tid - 1] : -1;
+  int t = -1, prev = -1, blk_ahead = -1, to_ahead = -1, t_ahead = -1, prev_ahead = -1;
+  auto look_ahead = [&](int j) {
+    t_ahead = j < n ? tokens[j] : -1;
+    prev_ahead = j > 0 && j < n ? tokens[j - 1] : -1;
+    blk_ahead = (t_ahead >= 0 && t_ahead < ctx) ? bt[t_ahead >> shift] : -1;
+    to_ahead = j < n ? nbt[(p0 + j) >> shift] : -1;
+  };
+  look_ahead(tid);
   for (int j0 = 0; j0 < n; j0 += kMoveThreads) {
-    const int j = j0 + tid, jn = j + kMoveThreads;
-    const int t_next = jn < n ? kept[p0 + jn] : -1, prev_next = jn < n ? kept[p0 + jn - 1] : -1;
+    const int j = j0 + tid;
+    t = t_ahead;
+    prev = prev_ahead;
+    int blk = blk_ahead, to = to_ahead;
+    look_ahead(j + kMoveThreads);  // before any address of this step is stored: the first of them is the `prev` of the next step
     const bool first = j < n && (j == 0 || (t >> shift) != (prev >> shift));
-    int blk = (t >= 0 && t < ctx) ? bt[t >> shift] : -1, to = j < n ? nbt[(p0 + j) >> shift] : -1;
     if (blk >= a.num_blocks) blk = -1;
     if (to >= a.num_blocks) to = -1;
     if (j < n && (blk < 0 || to < 0) && a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
@@ -287,8 +300,6 @@ __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, c
       if (first) pl.page_blk[u] = blk;
       if ((j & (a.page - 1)) == 0) pl.to[j >> shift] = to;
     }
-    t = t_next;
-    prev = prev_next;
     __syncthreads();
   }
   if (tid < 16) pl.addr[n + tid] = ring;  // the last group is read whole
@@ -424,38 +435,66 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
         if (m.sc[1].rows) move_scales<ES>(a, pl, m.sc[1], h, n, p0);
       }
     } else {
-      // rows of this warp, the same share of K and of V; a lane owns one word of every eighth row
-      const int row = lane >> 2, w = lane & 3;
-      const int k0 = k_rows * warp / kMoveWarps + row, k1 = k_rows * (warp + 1) / kMoveWarps;
-      const int v0 = v_rows * warp / kMoveWarps + row, v1 = v_rows * (warp + 1) / kMoveWarps;
+      // a team's warps share the rows, K and V alike; a lane owns one word of every eighth row
+      const int row = lane >> 2, w = lane & 3, crew = kMoveWarps / m.teams, team = warp / crew, at = warp % crew;
+      const int k0 = k_rows * at / crew + row, k1 = k_rows * (at + 1) / crew;
+      const int v0 = v_rows * at / crew + row, v1 = v_rows * (at + 1) / crew;
       int ready = 0, first = 0, first_st = st;  // pages that have arrived; the first one still held, its slot and phase
       uint32_t first_par = par;
+      auto wait_upto = [&](int page_last) {  // a lane per page: page_last - first < ring
+        if (dead || ready > page_last) return;
+        const int page = ready + lane, slot = first_st + page - first;
+        const bool wrap = slot >= m.ring;
+        bool open = page <= page_last;
+        for (uint32_t polls = 0; __any_sync(0xffffffffu, open); ++polls) {
+          if (open && mbar_test(full + 8 * (wrap ? slot - m.ring : slot), first_par ^ (wrap ? 1u : 0u))) open = false;
+          if (polls > (1u << 22)) {
+            dead = true;
+            *fail_ptr = 1;
+            break;
+          }
+        }
+        ready = page_last + 1;
+      };
+      // All pages before `next` have been read as far as this warp reads them.  A page is waited for before it is released, also
+      // one that only other teams read: its slot's earlier use is then over for everybody.
+      auto release = [&](int next) {
+        while (first < next) {
+          const int done = min(next - first, m.ring);
+          wait_upto(first + done - 1);
+          __syncwarp();
+          const int slot = first_st + lane;
+          if (lane < done) mbar_arrive(empty + 8 * (slot >= m.ring ? slot - m.ring : slot));
+          first += done;
+          first_st += done;
+          if (first_st >= m.ring) {
+            first_st -= m.ring;
+            first_par ^= 1;
+          }
+        }
+      };
+      int turn = 0;  // pairs of groups go round the teams
       for (int j0 = 0; j0 < n;) {
         // two groups at a time where the ring can hold all their pages: what a group costs a warp is latency
         const int4 ga = pl.group[j0 / G];
         int4 gb = j0 + G < n ? pl.group[j0 / G + 1] : ga;
-        const bool two = j0 + G < n && gb.x - first < m.ring;
+        const int page0 = pl.page[j0];
+        const bool two = j0 + G < n && gb.x - page0 < m.ring;
         if (!two) gb = ga;
+        const bool ours = turn == team;
+        if (++turn == m.teams) turn = 0;
+        if (!ours) {
+          j0 += two ? 2 * G : G;
+          continue;
+        }
         uint32_t fa[WT], fb[WT];
 #pragma unroll
         for (int k = 0; k < WT; ++k) {
           fa[k] = pl.addr[j0 + w * WT + k];
           fb[k] = pl.addr[j0 + (two ? G : 0) + w * WT + k];
         }
-        if (!dead && ready <= gb.x) {  // a lane per page
-          const int page = ready + lane, slot = first_st + page - first;
-          const bool wrap = slot >= m.ring;
-          bool open = page <= gb.x;
-          for (uint32_t polls = 0; __any_sync(0xffffffffu, open); ++polls) {
-            if (open && mbar_test(full + 8 * (wrap ? slot - m.ring : slot), first_par ^ (wrap ? 1u : 0u))) open = false;
-            if (polls > (1u << 22)) {
-              dead = true;
-              *fail_ptr = 1;
-              break;
-            }
-          }
-          ready = gb.x + 1;
-        }
+        release(page0);
+        wait_upto(gb.x);  // and with it for all before: nothing is written that is still to be read
         const uint32_t in_a = ((uint32_t)j0 & (PAGE - 1)) * EB + 4 * w, in_b = ((uint32_t)(j0 + G) & (PAGE - 1)) * EB + 4 * w;
         uint8_t* const ka = k_base + ga.z * k_page + in_a;
         uint8_t* const va = v_base + ga.z * v_page + in_a;
@@ -492,19 +531,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
           }
         }
         j0 += two ? 2 * G : G;
-        const int done = gb.y - first;  // pages that the next group does not need any more
-        if (done > 0) {
-          __syncwarp();
-          const int slot = first_st + lane;
-          if (lane < done) mbar_arrive(empty + 8 * (slot >= m.ring ? slot - m.ring : slot));
-          first = gb.y;
-          first_st += done;
-          if (first_st >= m.ring) {
-            first_st -= m.ring;
-            first_par ^= 1;
-          }
-        }
+        release(gb.y);
       }
+      release(n_pages);
       st = first_st;
       par = first_par;
     }
@@ -630,10 +659,11 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   const int sms = current_sm_count(), group = 16 / eb;
   auto slot = [&](int split) { return (uint32_t)(((D + v_rows) / split * row_bytes + 127) / 128 * 128); };
   m.ring_at = (1024 + sizeof(MovePlan) + 127) / 128 * 128;
-  // The ring holds one slab more than a group has tokens, and about 64 KB.  Rows are split until two such rings fit an SM and,
-  // in place, until every SM has work; elsewhere there are runs of positions for that, as long as pays for their plan.
+  // The ring holds one slab more than a group has tokens, and about 64 KB: two rings fit an SM.  Rows are split so that this is
+  // up to 32 slabs (the window in which the teams work) and, in place, until every SM has work; elsewhere there are runs of
+  // positions for that, as long as pays for their plan.
   m.split = 1;
-  while (m.split < 8 && m.ring_at + (group + 1) * slot(m.split) > 112 * 1024) m.split *= 2;
+  while (m.split < 8 && slot(m.split) > 2048) m.split *= 2;
   m.run = kMoveRun;
   if (in_place) {
     while (m.split < 8 && pairs * m.split * 2 <= 2 * sms) m.split *= 2;
@@ -645,6 +675,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   if (m.ring < group + 1) m.ring = group + 1;
   if (m.ring > kMoveMaxRing) m.ring = kMoveMaxRing;
   m.smem = m.ring_at + m.ring * m.slot_bytes;
+  m.teams = 4;
   const cudaError_t e = eb == 4 ? launch_move_page<uint32_t, uint32_t>(m, st) : eb == 2 ? launch_move_page<uint16_t, uint32_t>(m, st)
                         : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move_page<uint8_t, uint32_t>(m, st) : launch_move_page<uint8_t, uint8_t>(m, st);
   return cuda_result(e, "evict_move_kernel launch");
