@@ -1,5 +1,7 @@
 // Eviction from a paged KV cache: which tokens stay (a selection by rank per sequence and KV head), and their move to the
 // front of the same or of other pages.
+#include <type_traits>
+
 #include "host_common.cuh"
 #include "tcgen05_primitives.cuh"
 
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
 // above the group that is written, or is in the ring already; rows belong to warps, so no other order matters.  The tokens of a head are then one
 // CTA's work, and with few (sequence, head) pairs the rows are split over more CTAs; into other pages every run of new
 // positions is a CTA of its own.
-constexpr int kMoveWarps = 8, kMoveThreads = 32 * (kMoveWarps + 2), kMoveRun = 2048, kMoveMaxRing = 32;
+constexpr int kMoveWarps = 8, kMoveLoaders = 4, kMoveThreads = 32 * (kMoveWarps + kMoveLoaders + 1), kMoveRun = 2048, kMoveMaxRing = 32;
 
 struct MoveTensor {
   uint8_t* p;
@@ -312,15 +314,15 @@ __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, c
   __syncthreads();
 }
 
-// scales: a lane takes a token, 8 of them at a time (all loads before the stores: in place)
+// scales: a lane takes a token, 4 of them at a time (all loads before the stores: in place)
 template <typename E>
 __device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int h, int n, int p0) {
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.page);
   E* const p = reinterpret_cast<E*>(mt.p);
-  for (int j0 = 0; j0 < n; j0 += 256) {
-    long long from[8], to[8];
+  for (int j0 = 0; j0 < n; j0 += 128) {
+    long long from[4], to[4];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < 4; ++x) {
       const int j = j0 + x * 32 + lane;
       from[x] = -1;
       to[x] = 0;
@@ -330,36 +332,64 @@ __device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan& 
       }
     }
     for (int r = 0; r < mt.rows; ++r) {
-      E v[8];
+      E v[4];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = from[x] >= 0 ? p[from[x] + r * a.page] : (E)0;
+      for (int x = 0; x < 4; ++x) v[x] = from[x] >= 0 ? p[from[x] + r * a.page] : (E)0;
       __syncwarp();
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
+      for (int x = 0; x < 4; ++x)
         if (from[x] >= 0) p[to[x] + r * a.page] = v[x];
       __syncwarp();
     }
   }
 }
 
-// 4 bytes of a new row: 4, 2 or 1 elements from their places in the ring
-template <int EB>
-__device__ __forceinline__ uint32_t gather_word(const uint32_t (&from)[4 / EB], uint32_t offset) {
-  if constexpr (EB == 4) {
-    return lds32(from[0] + offset);
-  } else if constexpr (EB == 2) {
-    return prmt(lds16(from[0] + offset), lds16(from[1] + offset), 0x5410);
-  } else {
-    uint32_t x[4];
+// 4 bytes of a new row, `AT` bytes behind the first: 4, 2 or 1 elements from their places in the ring
+template <int EB, int AT>
+__device__ __forceinline__ uint32_t gather_word(const uint32_t (&from)[4 / EB]) {
+  uint32_t x[4 / EB];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x[k]) : "r"(from[k] + offset));
-    return prmt(prmt(x[0], x[1], 0x0040), prmt(x[2], x[3], 0x0040), 0x5410);
+  for (int k = 0; k < 4 / EB; ++k) {
+    if constexpr (EB == 4) asm volatile("ld.shared.b32 %0, [%1 + %2];" : "=r"(x[k]) : "r"(from[k]), "n"(AT));
+    else if constexpr (EB == 1) asm volatile("ld.shared.u8 %0, [%1 + %2];" : "=r"(x[k]) : "r"(from[k]), "n"(AT));
+    else asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1 + %2];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(x[k]) : "r"(from[k]), "n"(AT));
   }
+  if constexpr (EB == 4) return x[0];
+  else if constexpr (EB == 2) return prmt(x[0], x[1], 0x5410);
+  else return prmt(prmt(x[0], x[1], 0x0040), prmt(x[2], x[3], 0x0040), 0x5410);
+}
+// ITER rows, eight apart, of one tensor into one new group
+template <typename E, int ROW, int ITER>
+__device__ __forceinline__ void move_words(const uint32_t (&from)[4 / sizeof(E)], uint8_t* to, uint32_t mine) {
+  constexpr int EB = sizeof(E), WT = 4 / EB;
+  auto put = [&](uint8_t* at, uint32_t word) {
+    if (mine == (1u << WT) - 1) {
+      *reinterpret_cast<uint32_t*>(at) = word;
+    } else {
+#pragma unroll
+      for (int k = 0; k < WT; ++k)
+        if (mine >> k & 1) reinterpret_cast<E*>(at)[k] = (E)(word >> (8 * EB * k));
+    }
+  };
+  put(to, gather_word<EB, 0>(from));
+  if constexpr (ITER > 1) put(to + 8 * ROW, gather_word<EB, 8 * ROW>(from));
+}
+template <typename E, int ROW, int ITER>
+__device__ __forceinline__ void move_words_2(const uint32_t (&fa)[4 / sizeof(E)], const uint32_t (&fb)[4 / sizeof(E)], uint8_t* a, uint8_t* b) {
+  constexpr int EB = sizeof(E);
+  const uint32_t x = gather_word<EB, 0>(fa), y = gather_word<EB, 0>(fb);
+  if constexpr (ITER > 1) {
+    const uint32_t u = gather_word<EB, 8 * ROW>(fa), v = gather_word<EB, 8 * ROW>(fb);
+    *reinterpret_cast<uint32_t*>(a + 8 * ROW) = u;
+    *reinterpret_cast<uint32_t*>(b + 8 * ROW) = v;
+  }
+  *reinterpret_cast<uint32_t*>(a) = x;
+  *reinterpret_cast<uint32_t*>(b) = y;
 }
 
-// E: an element of K and V, ES: of their scales
-template <typename E, typename ES, int PAGE>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ MoveArgs m) {
+// E: an element of K and V, ES: of their scales.  KI, VI: rows of a lane, K and V (a warp has 8 KI rows of K, or fewer).
+template <typename E, typename ES, int PAGE, int KI, int VI>
+__global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __grid_constant__ MoveArgs m) {
   constexpr int EB = sizeof(E), G = 16 / EB, WT = 4 / EB;  // tokens of a group, of a word
   constexpr int ROW = PAGE * EB;                           // bytes of a row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -401,44 +431,39 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     plan_run<EB>(m, pl, kept, bt, nbt, p0, n, ctx, slot0, ring);
     const int n_pages = pl.n_pages;
     slot0 = (slot0 + n_pages) % m.ring;
-    if (warp == kMoveWarps) {
-      // a lane per page, up to 16 at a time: one thread alone would spend longer on a page than the copy takes.  A lane issues as soon as
-      // its own slot is free, whatever the others wait for (the first pages of a batch may have to pass for the last
-      // ones to get their slots).
-      const int batch = min(16, m.ring);  // no two lanes on one slot
-      for (int u0 = 0; u0 < n_pages && !dead; u0 += batch) {
-        const int u = u0 + lane;
-        bool open = lane < batch && u < n_pages;
-        const int slot = (st + lane) % m.ring;
-        const uint32_t wait_for = par ^ 1 ^ ((uint32_t)((st + lane) / m.ring) & 1u);
-        const int blk = open ? pl.page_blk[u] : -1;
-        for (uint32_t polls = 0; __any_sync(0xffffffffu, open); ++polls) {
-          if (polls > (1u << 22)) {
-            dead = true;
-            break;
-          }
-          if (open && mbar_test(empty + 8 * slot, wait_for)) {
-            open = false;
-            mbar_arrive_expect_tx(full + 8 * slot, blk >= 0 ? (uint32_t)(k_rows + v_rows) * ROW : 0u);
-            if (blk >= 0) {
-              bulk_g2s(ring + slot * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * ROW, full + 8 * slot);
-              bulk_g2s(ring + slot * m.slot_bytes + k_rows * ROW, v_base + blk * v_page, (uint32_t)v_rows * ROW, full + 8 * slot);
-            }
+    if (warp >= kMoveWarps && warp < kMoveWarps + kMoveLoaders) {
+      // pages in turn with the other loading warps: alone, one would spend longer on a page than its copies take
+      const int mine = warp - kMoveWarps;
+      for (int u = 0; u < n_pages; ++u, step()) {
+        if (u % kMoveLoaders != mine) continue;
+        if (!mbar_wait(empty + 8 * st, par ^ 1, 0)) {
+          dead = true;
+          *fail_ptr = 1;
+          break;
+        }
+        const int blk = pl.page_blk[u];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full + 8 * st, blk >= 0 ? (uint32_t)(k_rows + v_rows) * ROW : 0u);
+          if (blk >= 0) {
+            bulk_g2s(ring + st * m.slot_bytes, k_base + blk * k_page, (uint32_t)k_rows * ROW, full + 8 * st);
+            bulk_g2s(ring + st * m.slot_bytes + k_rows * ROW, v_base + blk * v_page, (uint32_t)v_rows * ROW, full + 8 * st);
           }
         }
-        for (int x = min(batch, n_pages - u0); x > 0; --x) step();
+        __syncwarp();
       }
-      if (dead && lane == 0) *fail_ptr = 1;
-    } else if (warp == kMoveWarps + 1) {
+    } else if (warp == kMoveWarps + kMoveLoaders) {
       if (part == 0) {
         if (m.sc[0].rows) move_scales<ES>(a, pl, m.sc[0], h, n, p0);
         if (m.sc[1].rows) move_scales<ES>(a, pl, m.sc[1], h, n, p0);
       }
     } else {
-      // a team's warps share the rows, K and V alike; a lane owns one word of every eighth row
+      // a team's warps share the rows, K and V alike; a lane owns one word of one or two rows of each
       const int row = lane >> 2, w = lane & 3, crew = kMoveWarps / m.teams, team = warp / crew, at = warp % crew;
-      const int k0 = k_rows * at / crew + row, k1 = k_rows * (at + 1) / crew;
-      const int v0 = v_rows * at / crew + row, v1 = v_rows * (at + 1) / crew;
+      const int kr = k_rows / crew * at + row, vr = v_rows / crew * at + row;
+      const bool k_live = KI > 1 || row < k_rows / crew, v_live = VI > 1 || row < v_rows / crew;
+      uint8_t* const k_row = k_base + kr * ROW + 4 * w;
+      uint8_t* const v_row = v_base + vr * ROW + 4 * w;
+      const uint32_t k_slab = kr * ROW, v_slab = (k_rows + vr) * ROW;
       int ready = 0, first = 0, first_st = st;  // pages that have arrived; the first one still held, its slot and phase
       uint32_t first_par = par;
       auto wait_upto = [&](int page_last) {  // a lane per page: page_last - first < ring
@@ -495,40 +520,28 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
         }
         release(page0);
         wait_upto(gb.x);  // and with it for all before: nothing is written that is still to be read
-        const uint32_t in_a = ((uint32_t)j0 & (PAGE - 1)) * EB + 4 * w, in_b = ((uint32_t)(j0 + G) & (PAGE - 1)) * EB + 4 * w;
-        uint8_t* const ka = k_base + ga.z * k_page + in_a;
-        uint8_t* const va = v_base + ga.z * v_page + in_a;
-        uint8_t* const kb = k_base + gb.z * k_page + in_b;
-        uint8_t* const vb = v_base + gb.z * v_page + in_b;
-        if (two && ga.w == (1 << G) - 1 && gb.w == (1 << G) - 1 && !dead) {
-          auto rows = [&](int r0, int r1, uint32_t slab, uint8_t* to_a, uint8_t* to_b) {
-#pragma unroll 2
-            for (int r = r0; r < r1; r += 8) {
-              const uint32_t x = gather_word<EB>(fa, slab + r * ROW), y = gather_word<EB>(fb, slab + r * ROW);
-              *reinterpret_cast<uint32_t*>(to_a + r * ROW) = x;
-              *reinterpret_cast<uint32_t*>(to_b + r * ROW) = y;
+        if (!dead) {
+          const uint32_t in_a = ((uint32_t)j0 & (PAGE - 1)) * EB, in_b = ((uint32_t)(j0 + G) & (PAGE - 1)) * EB;
+          const bool whole = two && ga.w == (1 << G) - 1 && gb.w == (1 << G) - 1;
+          auto tensor = [&](auto iter, uint32_t slab, uint8_t* base_row, long long page_bytes) {
+            constexpr int ITER = decltype(iter)::value;
+            uint32_t xa[WT], xb[WT];
+#pragma unroll
+            for (int k = 0; k < WT; ++k) {
+              xa[k] = fa[k] + slab;
+              xb[k] = fb[k] + slab;
+            }
+            uint8_t* const to_a = base_row + ga.z * page_bytes + in_a;
+            uint8_t* const to_b = base_row + gb.z * page_bytes + in_b;
+            if (whole) {
+              move_words_2<E, ROW, ITER>(xa, xb, to_a, to_b);
+            } else {  // one group, the end of a sequence, or a page that is not in the pool
+              move_words<E, ROW, ITER>(xa, to_a, (uint32_t)ga.w >> (w * WT) & ((1u << WT) - 1));
+              if (two) move_words<E, ROW, ITER>(xb, to_b, (uint32_t)gb.w >> (w * WT) & ((1u << WT) - 1));
             }
           };
-          rows(k0, k1, 0, ka, kb);
-          rows(v0, v1, k_rows * ROW, va, vb);
-        } else if (!dead) {  // one group, the end of a sequence, or a page that is not in the pool
-          auto rows = [&](int r0, int r1, uint32_t slab, const uint32_t (&from)[WT], uint8_t* to, uint32_t have) {
-            for (int r = r0; r < r1; r += 8) {
-              const uint32_t word = gather_word<EB>(from, slab + r * ROW);
-              if (have == (1u << G) - 1) {
-                *reinterpret_cast<uint32_t*>(to + r * ROW) = word;
-                continue;
-              }
-              for (int k = 0; k < WT; ++k)
-                if (have >> (w * WT + k) & 1) reinterpret_cast<E*>(to + r * ROW)[k] = (E)(word >> (8 * EB * k));
-            }
-          };
-          rows(k0, k1, 0, fa, ka, (uint32_t)ga.w);
-          rows(v0, v1, k_rows * ROW, fa, va, (uint32_t)ga.w);
-          if (two) {
-            rows(k0, k1, 0, fb, kb, (uint32_t)gb.w);
-            rows(v0, v1, k_rows * ROW, fb, vb, (uint32_t)gb.w);
-          }
+          if (k_live) tensor(std::integral_constant<int, KI>{}, k_slab, k_row, k_page);
+          if (v_live) tensor(std::integral_constant<int, VI>{}, v_slab, v_row, v_page);
         }
         j0 += two ? 2 * G : G;
         release(gb.y);
@@ -546,18 +559,26 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   }
 }
 
-template <typename E, typename ES, int PAGE>
+template <typename E, typename ES, int PAGE, int KI, int VI>
 static cudaError_t launch_move(const MoveArgs& m, cudaStream_t st) {
-  auto kern = evict_move_kernel<E, ES, PAGE>;
+  auto kern = evict_move_kernel<E, ES, PAGE, KI, VI>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)m.smem);
   if (e != cudaSuccess) return e;
   const unsigned runs = m.e.in_place ? 1u : (unsigned)((m.e.budget + m.run - 1) / m.run);
   kern<<<dim3(runs * m.split, m.e.Hkv, m.e.S), kMoveThreads, m.smem, st>>>(m);
   return cudaGetLastError();
 }
+template <typename E, typename ES, int PAGE>
+static cudaError_t launch_move_rows(const MoveArgs& m, cudaStream_t st) {
+  const int crew = kMoveWarps / m.teams, k = m.t[0].rows / m.split / crew, v = m.t[1].rows / m.split / crew;  // rows of a warp
+  if (k == 16 && v == 16) return launch_move<E, ES, PAGE, 2, 2>(m, st);
+  if constexpr (sizeof(E) == 1)
+    if (k == 16) return launch_move<E, ES, PAGE, 2, 1>(m, st);
+  return launch_move<E, ES, PAGE, 1, 1>(m, st);
+}
 template <typename E, typename ES>
 static cudaError_t launch_move_page(const MoveArgs& m, cudaStream_t st) {
-  return m.e.page == 16 ? launch_move<E, ES, 16>(m, st) : m.e.page == 32 ? launch_move<E, ES, 32>(m, st) : launch_move<E, ES, 64>(m, st);
+  return m.e.page == 16 ? launch_move_rows<E, ES, 16>(m, st) : m.e.page == 32 ? launch_move_rows<E, ES, 32>(m, st) : launch_move_rows<E, ES, 64>(m, st);
 }
 
 template <int THREADS>
@@ -663,7 +684,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   // up to 32 slabs (the window in which the teams work) and, in place, until every SM has work; elsewhere there are runs of
   // positions for that, as long as pays for their plan.
   m.split = 1;
-  while (m.split < 8 && slot(m.split) > 2048) m.split *= 2;
+  while (m.split < 8 && slot(m.split) > 8192) m.split *= 2;
   m.run = kMoveRun;
   if (in_place) {
     while (m.split < 8 && pairs * m.split * 2 <= 2 * sms) m.split *= 2;
@@ -675,7 +696,8 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   if (m.ring < group + 1) m.ring = group + 1;
   if (m.ring > kMoveMaxRing) m.ring = kMoveMaxRing;
   m.smem = m.ring_at + m.ring * m.slot_bytes;
-  m.teams = 4;
+  m.teams = 1;  // a warp has 16 rows of K, or the 8 of an eighth of head_dim 64
+  while (m.teams < kMoveWarps && D / m.split / (kMoveWarps / m.teams) < 16) m.teams *= 2;
   const cudaError_t e = eb == 4 ? launch_move_page<uint32_t, uint32_t>(m, st) : eb == 2 ? launch_move_page<uint16_t, uint32_t>(m, st)
                         : p->scale_mode == CUDA_LLM_SCALE_PER_TOKEN ? launch_move_page<uint8_t, uint32_t>(m, st) : launch_move_page<uint8_t, uint8_t>(m, st);
   return cuda_result(e, "evict_move_kernel launch");
