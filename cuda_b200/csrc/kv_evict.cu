@@ -234,12 +234,12 @@ struct MoveArgs {
   uint32_t slot_bytes, ring_at, smem;
 };
 
+template <int EB>
 struct MovePlan {                 // of one run of new positions
-  uint32_t addr[kMoveRun + 16];   // where in the ring a token's elements lie (those of the first row)
-  uint16_t page[kMoveRun];        // a token's page in the list below
-  uint8_t off[kMoveRun];          // its place in that page
+  uint16_t tok[kMoveRun + 16];    // a token's ring slot << 8 | its place in its page
+  uint16_t page[kMoveRun];        // its page in the list below
   int page_blk[kMoveRun];         // pages that hold kept tokens, in order; -1: not in the pool
-  int4 group[kMoveRun / 4];       // 16 bytes of a row: last page needed, pages done with it, new page, tokens that there are
+  int4 group[kMoveRun * EB / 16]; // 16 bytes of a row: last page needed, pages done with it, new page, tokens that there are
   int to[kMoveRun / 16];          // new pages, -1: not in the pool
   uint32_t there[kMoveRun / 32];  // which new positions have a token to move
   uint32_t scan[kMoveThreads / 32];
@@ -255,12 +255,11 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
 
 // `slot0`: ring slot of the run's first page
 template <int EB>
-__device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx, int slot0,
-                         uint32_t ring) {
+__device__ void plan_run(const MoveArgs& m, MovePlan<EB>& pl, const int32_t* kept, const int32_t* bt, const int32_t* nbt, int p0, int n, int ctx, int slot0) {
   constexpr int G = 16 / EB;
   const EvictArgs& a = m.e;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, shift = 31 - __clz(a.page);
-  int* const tokens = reinterpret_cast<int*>(pl.addr);  // (a place in addr is overwritten by the thread that has read it last)
+  int* const tokens = pl.page_blk;  // until the step that writes a page's entry, which no step ahead reads as a token
   for (int j = tid; j < n; j += kMoveThreads) tokens[j] = kept[p0 + j];
   __syncthreads();
   uint32_t base = 0;
@@ -277,7 +276,7 @@ __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, c
     t = t_ahead;
     prev = prev_ahead;
     int blk = blk_ahead, to = to_ahead;
-    look_ahead(j + kMoveThreads);  // before any address of this step is stored: the first of them is the `prev` of the next step
+    look_ahead(j + kMoveThreads);
     const bool first = j < n && (j == 0 || (t >> shift) != (prev >> shift));
     if (blk >= a.num_blocks) blk = -1;
     if (to >= a.num_blocks) to = -1;
@@ -296,15 +295,14 @@ __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, c
       base += pl.scan[w];
     }
     if (j < n) {
-      pl.addr[j] = ring + (slot0 + u) % (uint32_t)m.ring * m.slot_bytes + (uint32_t)(t & (a.page - 1)) * EB;
+      pl.tok[j] = (uint16_t)((slot0 + u) % (uint32_t)m.ring << 8 | (uint32_t)(t & (a.page - 1)));
       pl.page[j] = (uint16_t)u;
-      pl.off[j] = (uint8_t)(t & (a.page - 1));
       if (first) pl.page_blk[u] = blk;
       if ((j & (a.page - 1)) == 0) pl.to[j >> shift] = to;
     }
     __syncthreads();
   }
-  if (tid < 16) pl.addr[n + tid] = ring;  // the last group is read whole
+  if (tid < 16) pl.tok[n + tid] = 0;  // the last group is read whole
   if (tid == 0) pl.n_pages = (int)base;
   for (int g = tid; g * G < n; g += kMoveThreads) {
     const int j = g * G;
@@ -315,8 +313,8 @@ __device__ void plan_run(const MoveArgs& m, MovePlan& pl, const int32_t* kept, c
 }
 
 // scales: a lane takes a token, 4 of them at a time (all loads before the stores: in place)
-template <typename E>
-__device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan& pl, const MoveTensor& mt, int h, int n, int p0) {
+template <typename E, int EB>
+__device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan<EB>& pl, const MoveTensor& mt, int h, int n, int p0) {
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.page);
   E* const p = reinterpret_cast<E*>(mt.p);
   for (int j0 = 0; j0 < n; j0 += 128) {
@@ -327,7 +325,7 @@ __device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan& 
       from[x] = -1;
       to[x] = 0;
       if (j < n && (pl.there[j >> 5] >> (j & 31) & 1)) {
-        from[x] = ((long long)pl.page_blk[pl.page[j]] * a.Hkv + h) * mt.rows * a.page + pl.off[j];
+        from[x] = ((long long)pl.page_blk[pl.page[j]] * a.Hkv + h) * mt.rows * a.page + (pl.tok[j] & 255);
         to[x] = ((long long)pl.to[j >> shift] * a.Hkv + h) * mt.rows * a.page + ((p0 + j) & (a.page - 1));
       }
     }
@@ -393,7 +391,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __gri
   constexpr int EB = sizeof(E), G = 16 / EB, WT = 4 / EB;  // tokens of a group, of a word
   constexpr int ROW = PAGE * EB;                           // bytes of a row
   extern __shared__ __align__(128) uint8_t smem[];
-  MovePlan& pl = *reinterpret_cast<MovePlan*>(smem + 1024);
+  MovePlan<EB>& pl = *reinterpret_cast<MovePlan<EB>*>(smem + 1024);
   const EvictArgs& a = m.e;
   const uint32_t base = smem_u32(smem), full = base, empty = base + 8 * kMoveMaxRing, ring = base + m.ring_at;
   volatile int* fail_ptr = reinterpret_cast<volatile int*>(smem + 16 * kMoveMaxRing);
@@ -428,7 +426,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __gri
   // in place: all runs of the head, one after another; else one
   for (int p0 = run0 * m.run; p0 < total; p0 += a.in_place ? m.run : total) {
     const int n = min(m.run, total - p0);
-    plan_run<EB>(m, pl, kept, bt, nbt, p0, n, ctx, slot0, ring);
+    plan_run<EB>(m, pl, kept, bt, nbt, p0, n, ctx, slot0);
     const int n_pages = pl.n_pages;
     slot0 = (slot0 + n_pages) % m.ring;
     if (warp >= kMoveWarps && warp < kMoveWarps + kMoveLoaders) {
@@ -515,8 +513,9 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __gri
         uint32_t fa[WT], fb[WT];
 #pragma unroll
         for (int k = 0; k < WT; ++k) {
-          fa[k] = pl.addr[j0 + w * WT + k];
-          fb[k] = pl.addr[j0 + (two ? G : 0) + w * WT + k];
+          const uint32_t ta = pl.tok[j0 + w * WT + k], tb = pl.tok[j0 + (two ? G : 0) + w * WT + k];
+          fa[k] = ring + (ta >> 8) * m.slot_bytes + (ta & 255u) * EB;
+          fb[k] = ring + (tb >> 8) * m.slot_bytes + (tb & 255u) * EB;
         }
         release(page0);
         wait_upto(gb.x);  // and with it for all before: nothing is written that is still to be read
@@ -679,8 +678,8 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   const long long pairs = (long long)a.S * a.Hkv;
   const int sms = current_sm_count(), group = 16 / eb;
   auto slot = [&](int split) { return (uint32_t)(((D + v_rows) / split * row_bytes + 127) / 128 * 128); };
-  m.ring_at = (1024 + sizeof(MovePlan) + 127) / 128 * 128;
-  // The ring holds one slab more than a group has tokens, and about 64 KB: two rings fit an SM.  Rows are split so that this is
+  m.ring_at = (1024 + (eb == 1 ? sizeof(MovePlan<1>) : eb == 2 ? sizeof(MovePlan<2>) : sizeof(MovePlan<4>)) + 127) / 128 * 128;
+  // The ring holds one slab more than a group has tokens, and as many as leave room for two CTAs on an SM.  Rows are split so that this is
   // up to 32 slabs (the window in which the teams work) and, in place, until every SM has work; elsewhere there are runs of
   // positions for that, as long as pays for their plan.
   m.split = 1;
@@ -692,7 +691,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
     while (m.run > 256 && pairs * m.split * ((a.budget + m.run - 1) / m.run) < 2 * sms) m.run /= 2;
   }
   m.slot_bytes = slot(m.split);
-  m.ring = (int)(64 * 1024 / m.slot_bytes);
+  m.ring = (int)((113 * 1024 - m.ring_at) / m.slot_bytes);
   if (m.ring < group + 1) m.ring = group + 1;
   if (m.ring > kMoveMaxRing) m.ring = kMoveMaxRing;
   m.smem = m.ring_at + m.ring * m.slot_bytes;
