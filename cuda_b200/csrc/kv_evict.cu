@@ -28,18 +28,18 @@ __device__ __forceinline__ int evict_ctx(const EvictArgs& a, int s, bool report)
   return max(ctx, 0);
 }
 
-// Scores as unsigned integers of the same order: NaN lowest, then -inf .. +inf (-0 and +0 alike), protected tokens on top.
-__device__ __forceinline__ uint32_t rank_key(float x, bool is_protected) {
-  if (is_protected) return 0xffffffffu;
-  if (x != x) return 0u;
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+// Scores as unsigned integers of the same order: NaN lowest, then -inf .. +inf, -0 as +0; and back.
+__device__ __forceinline__ uint32_t rank_key(float x) {
+  const uint32_t u = x != x ? 0xffffffffu : __float_as_uint(x + 0.f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float key_score(uint32_t k) { return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u)); }
 
 // ---- selection ------------------------------------------------------------------------------------------------------
 // A thread-block cluster per (KV head, sequence); each CTA holds its part of the score row in shared memory.  The budget-th
-// largest key comes from four passes over its bytes: a histogram per CTA (lanes with the same byte add once), summed over the
-// cluster through distributed shared memory.  Then each warp counts, and afterwards writes, the kept tokens of its own run
+// largest key comes from three passes over 11, 11 and 10 of its bits (the first, sign, exponent and two bits of the fraction,
+// spreads scores of similar size over enough bins for plain atomics): a histogram per CTA, summed over the cluster
+// through distributed shared memory.  Then each warp counts, and afterwards writes, the kept tokens of its own run
 // of positions, so that the order needs one prefix sum.  The row is read once, before anything is written: new_scores may be
 // scores.
 constexpr int kSelMaxPart = 49152;  // scores per CTA: 192 KB
@@ -64,11 +64,25 @@ __device__ __forceinline__ uint32_t sel_remote(const uint32_t* p, uint32_t rank)
   return v;
 }
 
+constexpr int kSelBins = 2048;
+
+// PER consecutive words of CTA `rank`
+template <int PER>
+__device__ __forceinline__ void sel_remote_vec(const uint32_t* p, uint32_t rank, uint32_t (&v)[PER]) {
+  static_assert(PER == 2 || PER == 4, "");
+  if constexpr (PER == 4)
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [ra];\n\t}"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(smem_u32(p)), "r"(rank) : "memory");
+  else
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %2, %3;\n\tld.shared::cluster.v2.u32 {%0, %1}, [ra];\n\t}"
+                 : "=r"(v[0]), "=r"(v[1]) : "r"(smem_u32(p)), "r"(rank) : "memory");
+}
+
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a) {
-  constexpr int WARPS = THREADS / 32;
-  extern __shared__ float row[];
-  __shared__ uint32_t hist[4][256], digit_sum[256];
+  constexpr int WARPS = THREADS / 32, PER = kSelBins / THREADS;
+  extern __shared__ uint32_t row[];          // keys of this CTA's part
+  __shared__ __align__(16) uint32_t hist[3][kSelBins];
   __shared__ uint32_t counts[2];             // kept for sure, on the edge: of this CTA
   __shared__ uint32_t warp_gt[WARPS], warp_eq[WARPS], found[2];
   const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -88,74 +102,68 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
     return;
   }
   const int t0 = (int)((long long)ctx * rank / parts), n = (int)((long long)ctx * (rank + 1) / parts) - t0;
-  for (int i = tid; i < 4 * 256; i += THREADS) (&hist[0][0])[i] = 0;
 #pragma unroll 4
-  for (int i = tid; i < n; i += THREADS) row[i] = sc[t0 + i];
+  for (int i = tid; i < 3 * kSelBins; i += THREADS) (&hist[0][0])[i] = 0;
+#pragma unroll 8
+  for (int i = tid; i < n; i += THREADS) row[i] = rank_key(sc[t0 + i]);
   __syncthreads();
-  auto key_at = [&](int i) { return rank_key(row[i], t0 + i < a.sink || t0 + i >= ctx - a.recent); };
-  uint32_t prefix = 0, left = (uint32_t)n_keep;
+  const int m0 = max(0, a.sink - t0), m1 = min(n, ctx - a.recent - t0);  // tokens that are ranked
+  uint32_t prefix = 0, left = (uint32_t)(n_keep - a.sink - a.recent);    // of them stay
 #pragma unroll 1
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
-    for (int i0 = 0; i0 < n; i0 += THREADS) {
-      const int i = i0 + tid;
-      const uint32_t k = i < n ? key_at(i) : 0u;
-      const bool in = i < n && (k & mask) == prefix;
-      const uint32_t digit = (k >> shift) & 255;
-      if (pass == 0) {  // sign and exponent: few different bytes, lanes with the same one add once
-        const uint32_t same = __match_any_sync(0xffffffffu, in ? digit : 256u);
-        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[0][digit], (uint32_t)__popc(same));
-      } else if (in) {
-        atomicAdd(&hist[pass][digit], 1u);
-      }
+  for (int pass = 0; pass < 3 && left > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
+#pragma unroll 4
+    for (int i = m0 + tid; i < m1; i += THREADS) {
+      const uint32_t k = row[i];
+      if ((k & mask) == prefix) atomicAdd(&hist[pass][(k >> shift) & (kSelBins - 1) & (pass == 2 ? 1023u : 2047u)], 1u);
     }
     if (parts > 1) sel_cluster_sync();
     else __syncthreads();
-    if (tid < 256) {
-      uint32_t sum = hist[pass][tid];
-      if (parts > 1) {
-        sum = 0;
-        for (uint32_t q = 0; q < parts; ++q) sum += sel_remote(&hist[pass][tid], q);
-      }
-      digit_sum[tid] = sum;
+    // a thread's bins from the top down, and how many keys lie above them
+    uint32_t c[PER], mine = 0;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) c[x] = 0;
+    for (uint32_t q = 0; q < parts; ++q) {
+      uint32_t y[PER];
+      sel_remote_vec<PER>(&hist[pass][kSelBins - PER * (tid + 1)], q, y);
+#pragma unroll
+      for (int x = 0; x < PER; ++x) c[x] += y[PER - 1 - x];
     }
+#pragma unroll
+    for (int x = 0; x < PER; ++x) mine += c[x];
+    uint32_t above = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, above, o);
+      if (lane >= o) above += y;
+    }
+    if (lane == 31) warp_gt[warp] = above;
     __syncthreads();
-    if (warp == 0) {  // the largest digit d with (keys above d) < left <= (keys from d up)
-      uint32_t c[8], mine = 0;
+    above += __reduce_add_sync(0xffffffffu, lane < warp && lane < WARPS ? warp_gt[lane] : 0u) - mine;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        c[x] = digit_sum[255 - (lane * 8 + x)];
-        mine += c[x];
+    for (int x = 0; x < PER; ++x) {
+      if (above < left && left <= above + c[x]) {  // one bin of one thread
+        found[0] = (uint32_t)(kSelBins - 1 - (tid * PER + x));
+        found[1] = left - above;
       }
-      uint32_t before = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += y;
-      }
-      before -= mine;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        if (before < left && left <= before + c[x]) {
-          found[0] = 255 - (lane * 8 + x);
-          found[1] = left - before;
-        }
-        before += c[x];
-      }
+      above += c[x];
     }
     __syncthreads();
     prefix |= found[0] << shift;
     left = found[1];
   }
-  // keep all keys above `prefix` and the first `left` that equal it
-  const uint32_t edge = prefix;
+  // keep all ranked keys above `edge` and the first `left` that equal it (none at all if no ranked token stays)
+  const uint32_t edge = left > 0 ? prefix : 0xffffffffu;
   const int per = ((n + WARPS - 1) / WARPS + 31) & ~31, b0 = min(n, warp * per), b1 = min(n, b0 + per);
+  auto above_at = [&](int i) { return i < m0 || i >= m1 || row[i] > edge; };
+  auto edge_at = [&](int i) { return i >= m0 && i < m1 && row[i] == edge; };
   uint32_t gt = 0, eq = 0;
+#pragma unroll 4
   for (int i0 = b0; i0 < b1; i0 += 32) {
-    const uint32_t k = i0 + lane < b1 ? key_at(i0 + lane) : 0u;
-    gt += __popc(__ballot_sync(0xffffffffu, i0 + lane < b1 && k > edge));
-    eq += __popc(__ballot_sync(0xffffffffu, i0 + lane < b1 && k == edge));
+    const int i = i0 + lane;
+    gt += __popc(__ballot_sync(0xffffffffu, i < b1 && above_at(i)));
+    eq += __popc(__ballot_sync(0xffffffffu, i < b1 && edge_at(i)));
   }
   if (lane == 0) {
     warp_gt[warp] = gt;
@@ -191,14 +199,13 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
   }
   for (int i0 = b0; i0 < b1; i0 += 32) {
     const int i = i0 + lane;
-    const uint32_t k = i < b1 ? key_at(i) : 0u;
-    const bool is_gt = i < b1 && k > edge, is_eq = i < b1 && k == edge;
+    const bool is_gt = i < b1 && above_at(i), is_eq = i < b1 && edge_at(i);
     const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq), below = (1u << lane) - 1;
     const uint32_t e = at_eq + __popc(be & below);
     if (is_gt || (is_eq && e < left)) {
       const uint32_t to = at_gt + __popc(bg & below) + min(e, left);
       kept[to] = t0 + i;
-      if (ns) ns[to] = row[i];
+      if (ns) ns[to] = key_score(row[i]);
     }
     at_gt += __popc(bg);
     at_eq += __popc(be);
@@ -584,7 +591,7 @@ template <int THREADS>
 static cudaError_t launch_select(const EvictArgs& a, int parts, int most, cudaStream_t st) {
   auto kern = evict_select_kernel<THREADS>;
   const int smem = ((most + parts - 1) / parts + 1) * 4;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelMaxPart * 4 + 64);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelMaxPart * 4 + 4);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(parts, a.Hkv, a.S);
@@ -665,7 +672,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   if (row_most > a.max_tokens) row_most = a.max_tokens;
   int parts = 1;
   while (parts < 8 && row_most > 8192ll * parts) parts *= 2;
-  rc = cuda_result(row_most > 4096 ? launch_select<1024>(a, parts, (int)row_most, st) : launch_select<256>(a, parts, (int)row_most, st),
+  rc = cuda_result(row_most > 8192 ? launch_select<1024>(a, parts, (int)row_most, st) : launch_select<512>(a, parts, (int)row_most, st),
                    "evict_select_kernel launch");
   if (rc != CUDA_LLM_OK) return rc;
   const int D = p->head_dim, v_rows = p->v_format == CUDA_LLM_KV_FP4_E2M1 ? D / 2 : D;
