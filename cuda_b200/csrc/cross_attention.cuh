@@ -22,9 +22,67 @@ __device__ __forceinline__ int cross_kv_len(const CrossArgs& a, int b) {
   return n < 0 ? 0 : (n < a.Skv ? n : a.Skv);
 }
 
+// Batch rows in the order of falling length: blocks of the longest start first and the short ones fill the last wave.
+// (Block-uniform; every thread counts for one row how many go before it.)
+template <int THREADS>
+__device__ __forceinline__ int longest_first(const CrossArgs& c, int z) {
+  if (!c.kv_lens || c.B == 1 || c.B > THREADS) return z;
+  __shared__ int pick;
+  const int b = threadIdx.x;
+  if (b < c.B) {
+    const int n = cross_kv_len(c, b);
+    int before = 0;
+    for (int x = 0; x < c.B; ++x) {
+      const int y = cross_kv_len(c, x);
+      before += (y > n || (y == n && x < b)) ? 1 : 0;
+    }
+    if (before == z) pick = b;
+  }
+  __syncthreads();
+  return pick;
+}
+
+// ---- clusters: the CTAs that share the states of one (sequence, KV head) and join their parts
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 dsmem_ld128(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 dsmem_ld64(uint32_t addr, uint32_t rank) {
+  float2 v;
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [ra];\n\t}"
+      : "=f"(v.x), "=f"(v.y) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+
+// CTAs per (sequence, KV head, row block): enough for two CTAs on every SM, at most 8 and at most one per `tiles`.
+inline int cross_parts(long long blocks, int tiles) {
+  const int sms = current_sm_count();
+  int parts = 1;
+  while (parts < 8 && parts * 2 <= tiles && blocks * parts < 2ll * sms) parts *= 2;
+  return parts;
+}
+
 constexpr float kLn2 = 0.6931471805599453f;
 
-cudaError_t launch_cross_simt(const CrossArgs& a, int D, cudaStream_t st);   // fp32 arithmetic
+cudaError_t launch_cross_simt(const CrossArgs& a, int D, cudaStream_t st);   // fp32 tensors
+cudaError_t launch_cross_stream(const CrossArgs& a, int D, cudaStream_t st); // fp32 tensors, up to 16 query rows per KV head
 cudaError_t launch_cross_token(const CrossArgs& a, int D, cudaStream_t st);  // 16-bit types, up to 64 query rows per KV head
 cudaError_t launch_cross_prompt(const CrossArgs& a, int D, cudaStream_t st); // 16-bit types, many query rows
 cudaError_t cross_wait_timeouts(unsigned int* count);    // bounded waits that ran out, per kernel

@@ -43,25 +43,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
       : "memory");
 }
 
-// Batch rows in the order of falling length: blocks of the longest start first and the short ones fill the last wave.
-// (Block-uniform; every thread counts for one row how many go before it.)
-__device__ __forceinline__ int longest_first(const CrossArgs& c, int z) {
-  if (!c.kv_lens || c.B == 1 || c.B > kPromptThreads) return z;
-  __shared__ int pick;
-  const int b = threadIdx.x;
-  if (b < c.B) {
-    const int n = cross_kv_len(c, b);
-    int before = 0;
-    for (int x = 0; x < c.B; ++x) {
-      const int y = cross_kv_len(c, x);
-      before += (y > n || (y == n && x < b)) ? 1 : 0;
-    }
-    if (before == z) pick = b;
-  }
-  __syncthreads();
-  return pick;
-}
-
 template <int D>
 constexpr int prompt_slots() { return D == 128 ? 5 : 8; }
 template <int D>
@@ -79,7 +60,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
   const uint32_t sQ = base + 1024, ring = sQ + NCH * QCH;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = longest_first(a.c, blockIdx.z);
+  const int b = longest_first<kPromptThreads>(a.c, blockIdx.z);
   const int chunks = a.c.group / a.gsz;
   const int kvh = blockIdx.y / chunks, head0 = kvh * a.c.group + (blockIdx.y - kvh * chunks) * a.gsz;
   const int BQ = kPromptRows / a.gsz;  // positions per CTA

@@ -34,34 +34,6 @@ __device__ __forceinline__ void tma_tile_4d(uint32_t dst, const void* map, int c
       ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 dsmem_ld128(uint32_t addr, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 dsmem_ld64(uint32_t addr, uint32_t rank) {
-  float2 v;
-  asm volatile(
-      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [ra];\n\t}"
-      : "=f"(v.x), "=f"(v.y) : "r"(addr), "r"(rank) : "memory");
-  return v;
-}
-
 template <int D>
 constexpr int tok_stages() { return D == 128 ? 3 : 6; }
 template <int D>
@@ -77,7 +49,7 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
   const uint32_t full = base, empty = base + 8 * NST, fail_at = base + 16 * NST, ring = base + 1024;
   volatile uint32_t* fail_ptr = reinterpret_cast<volatile uint32_t*>(smem + 16 * NST);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int kvh = blockIdx.y, b = longest_first<kTokThreads>(a.c, blockIdx.z);
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
   (void)fail_at;
 
@@ -358,9 +330,7 @@ cudaError_t launch_cross_token(const CrossArgs& c, int D, cudaStream_t st) {
       return cudaErrorInvalidValue;
   }
   const int tiles = (c.Skv + kTokTile - 1) / kTokTile;
-  const long long pairs = (long long)c.B * c.Hkv;
-  int parts = 1;
-  while (parts < 8 && parts * 2 <= tiles && pairs * parts < 4096) parts *= 2;
+  const int parts = cross_parts((long long)c.B * c.Hkv, tiles);
   const bool bf16 = c.dtype == CUDA_LLM_BF16;
   if (D == 64) return bf16 ? go_rows<64, true>(a, parts, st) : go_rows<64, false>(a, parts, st);
   return bf16 ? go_rows<128, true>(a, parts, st) : go_rows<128, false>(a, parts, st);
