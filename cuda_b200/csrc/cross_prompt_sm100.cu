@@ -8,9 +8,11 @@
 //                     exponentials, P (16-bit) back over the columns of S
 //   warp 8            TMA: Q once, then K and V tiles of 128 states into a ring of 32 KB slots
 //   warp 9            (10, 11 idle) allocates TMEM, issues the MMAs of both tiles in turn: PV_0(j), S_0(j+1), PV_1(j), S_1(j+1)
-// Tensor memory: S0/P0 | S1/P1 | O0 | O1, 128 columns each.  P overwrites S: every MMA that reads P of step j is issued
-// before the S of step j + 1, and the tensor pipe works in order.  The same order makes "S(j) is complete" mean "P V (j - 1) is
-// complete", so a softmax thread may rescale O without another barrier.  O is rescaled only when a row maximum grew
+// Tensor memory, head_dim 128: S0/P0 | S1/P1 | O0 | O1, 128 columns each, all there is.  P overwrites S: every MMA that reads P
+// of step j is issued before the S of step j + 1, and the tensor pipe works in order.  The same order makes "S(j) is complete"
+// mean "P V (j - 1) is complete", so a softmax thread may rescale O without another barrier.
+// head_dim 64 leaves columns for P of its own (S0 | S1 | O0 | O1 | P0 | P1): S(j + 1) then follows as soon as the softmax has
+// read S(j), and is ready when it comes back; P and O wait for the P V before instead.  O is rescaled only when a row maximum grew
 // by more than 2^8 (P stays below 256), which after the first tiles is rare.
 // What lies behind a sequence's length inside the last tile may be NaN: S is replaced by -inf there and the V rows are
 // zeroed in shared memory before the last P V.
@@ -51,12 +53,14 @@ constexpr size_t prompt_smem() { return 1024 + (size_t)kPromptRows * D * 2 + (si
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const __grid_constant__ CrossPromptArgs a) {
   constexpr int NCH = D / 64, NS = prompt_slots<D>();
+  constexpr bool OWN_P = D == 64;                        // P has tensor memory of its own
+  constexpr uint32_t T_O = 256, T_P = OWN_P ? 256 + 2 * D : 0, P_STEP = OWN_P ? 64 : 128, O_STEP = OWN_P ? D : 128;
   constexpr uint32_t QCH = kPromptRows * 128, KCH = kPromptKeys * 128, SLOT = NCH * KCH;
   constexpr float NEG_INF = -__builtin_huge_valf();
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t q_full = base, full = base + 8, empty = full + 8 * NS, s_full = empty + 8 * NS, p_full = s_full + 16, o_full = p_full + 16,
-                 v_fixed = o_full + 16, tmem_slot = v_fixed + 8;
+                 v_fixed = o_full + 16, s_read = v_fixed + 8, pv_done = s_read + 16, tmem_slot = pv_done + 16;
   const uint32_t sQ = base + 1024, ring = sQ + NCH * QCH;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -81,6 +85,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, 4);  // one arrival per softmax warp of the tile
       mbar_init(o_full + 8 * i, 1);
+      mbar_init(s_read + 8 * i, 4);
+      mbar_init(pv_done + 8 * i, 1);
     }
     mbar_init(v_fixed, 1);
     mbar_fence_init();
@@ -179,19 +185,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
         if (ok && j + 1 < n_tiles) ok = next_slot(ks);
         if (ok && fix_v && j + 1 == n_tiles) ok = tc_wait(v_fixed, 0);
         for (int i = 0; ok && i < n_q; ++i) {
+          if (OWN_P && j + 1 < n_tiles) {
+            ok = tc_wait(s_read + 8 * i, j & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(i, ks);
+            if (i == n_q - 1) umma_commit(empty + 8 * ks);
+          }
           ok = tc_wait(p_full + 8 * i, j & 1);
           if (!ok) break;
           tc_fence_after();
           const uint32_t vl = v_lo + ((vs * SLOT) >> 4);
 #pragma unroll
           for (int kk = 0; kk < kPromptKeys / 16; ++kk)
-            umma_f16_ts_parts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, vl + ((kk * 2048) >> 4), hi, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+            umma_f16_ts_parts(tmem + T_O + i * O_STEP, tmem + T_P + i * P_STEP + kk * 8, vl + ((kk * 2048) >> 4), hi, idesc_o,
+                              (j > 0 || kk > 0) ? 1u : 0u);
+          if (OWN_P) umma_commit(pv_done + 8 * i);
           if (i == n_q - 1) umma_commit(empty + 8 * vs);
-          if (j + 1 < n_tiles) {
+          if (j + 1 == n_tiles) {
+            umma_commit(o_full + 8 * i);
+          } else if (!OWN_P) {
             issue_s(i, ks);
             if (i == n_q - 1) umma_commit(empty + 8 * ks);
-          } else {
-            umma_commit(o_full + 8 * i);
           }
         }
       }
@@ -203,7 +218,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
   if ((warp >> 2) < n_q) {
     const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + 256 + i * 128;
+    const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + T_O + i * O_STEP, tP = tmem + lanes + T_P + i * P_STEP;
     const int r = i * 128 + row, head = head0 + r / BQ, pos = q0 + r % BQ;
     float m_run = -1.0e30f, l_run = 0.f;
     bool ok = true;
@@ -214,6 +229,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
       tc_wait_ld();
+      if (OWN_P) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read + 8 * i);
+      }
       const int left = len - j * kPromptKeys;
       if (left < kPromptKeys) {
 #pragma unroll
@@ -232,6 +252,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
           mx8[(e >> 1) & 7] = fmax3(mx8[(e >> 1) & 7], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
       const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
       const float m_tile = mx * a.c.scale_log2;
+      if (OWN_P && j > 0) {  // O and P are free
+        if (!tc_wait(pv_done + 8 * i, (j - 1) & 1)) { ok = false; break; }
+        tc_fence_after();
+      }
       if (__any_sync(0xffffffffu, m_tile > m_run + 8.f)) {  // some row of the warp needs a new reference
         const float m_new = (m_tile > m_run + 8.f) ? m_tile : m_run;
         const float alpha = fast_exp2(m_run - m_new);
@@ -264,7 +288,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
           fadd2(ps[2 * k], ps[2 * k + 1], ps[2 * k], ps[2 * k + 1], p0, p1);
           pk[e >> 1] = BF16 ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
         }
-        tmem_st16(tS + c * 16, pk);
+        tmem_st16(tP + c * 16, pk);
       }
       tc_wait_st();
       l_run += (((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7])));
