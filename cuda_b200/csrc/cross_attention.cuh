@@ -23,11 +23,10 @@ __device__ __forceinline__ int cross_kv_len(const CrossArgs& a, int b) {
 }
 
 // Batch rows in the order of falling length: blocks of the longest start first and the short ones fill the last wave.
-// (Block-uniform; every thread counts for one row how many go before it.)
+// (Block-uniform; every thread counts for one row how many go before it.  `pick`: a word of shared memory.)
 template <int THREADS>
-__device__ __forceinline__ int longest_first(const CrossArgs& c, int z) {
+__device__ __forceinline__ int longest_first(const CrossArgs& c, int z, volatile int* pick) {
   if (!c.kv_lens || c.B == 1 || c.B > THREADS) return z;
-  __shared__ int pick;
   const int b = threadIdx.x;
   if (b < c.B) {
     const int n = cross_kv_len(c, b);
@@ -36,10 +35,10 @@ __device__ __forceinline__ int longest_first(const CrossArgs& c, int z) {
       const int y = cross_kv_len(c, x);
       before += (y > n || (y == n && x < b)) ? 1 : 0;
     }
-    if (before == z) pick = b;
+    if (before == z) *pick = b;
   }
   __syncthreads();
-  return pick;
+  return *pick;
 }
 
 // ---- clusters: the CTAs that share the states of one (sequence, KV head) and join their parts
@@ -71,11 +70,49 @@ __device__ __forceinline__ float2 dsmem_ld64(uint32_t addr, uint32_t rank) {
   return v;
 }
 
+constexpr int kMaxParts = 8;
+struct JoinedWord {
+  float4 x;    // sum of the parts' O, weighted
+  float M, L;  // their common maximum and sum
+};
+// Four elements of one row from the parts of all CTAs: {m, l} of the row at `ml_at`, the elements at `o_at` (the same places in
+// every CTA).  All loads first: one after another they would cost a remote latency each.
+__device__ __forceinline__ JoinedWord join_parts(uint32_t ml_at, uint32_t o_at, int parts) {
+  float2 ml[kMaxParts];
+  float4 y[kMaxParts];
+#pragma unroll
+  for (int q = 0; q < kMaxParts; ++q) {
+    ml[q] = make_float2(-__builtin_huge_valf(), 0.f);
+    y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (q < parts) {
+      ml[q] = dsmem_ld64(ml_at, q);
+      y[q] = dsmem_ld128(o_at, q);
+    }
+  }
+  JoinedWord j;
+  j.M = ml[0].x;
+#pragma unroll
+  for (int q = 1; q < kMaxParts; ++q) j.M = fmaxf(j.M, ml[q].x);
+  const float ref = j.M == -__builtin_huge_valf() ? 0.f : j.M;
+  j.L = 0.f;
+  j.x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int q = 0; q < kMaxParts; ++q) {
+    const float w = exp2f(ml[q].x - ref);
+    j.L = fmaf(ml[q].y, w, j.L);
+    j.x.x = fmaf(y[q].x, w, j.x.x);
+    j.x.y = fmaf(y[q].y, w, j.x.y);
+    j.x.z = fmaf(y[q].z, w, j.x.z);
+    j.x.w = fmaf(y[q].w, w, j.x.w);
+  }
+  return j;
+}
+
 // CTAs per (sequence, KV head, row block): enough for two CTAs on every SM, at most 8 and at most one per `tiles`.
 inline int cross_parts(long long blocks, int tiles) {
   const int sms = current_sm_count();
   int parts = 1;
-  while (parts < 8 && parts * 2 <= tiles && blocks * parts < 2ll * sms) parts *= 2;
+  while (parts < kMaxParts && parts * 2 <= tiles && blocks * parts < 2ll * sms) parts *= 2;
   return parts;
 }
 

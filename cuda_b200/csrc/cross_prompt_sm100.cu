@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
   const uint32_t sQ = base + 1024, ring = sQ + NCH * QCH;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = longest_first<kPromptThreads>(a.c, blockIdx.z);
+  const int b = longest_first<kPromptThreads>(a.c, blockIdx.z, reinterpret_cast<volatile int*>(smem + 1020));
   const int chunks = a.c.group / a.gsz;
   const int kvh = blockIdx.y / chunks, head0 = kvh * a.c.group + (blockIdx.y - kvh * chunks) * a.gsz;
   const int BQ = kPromptRows / a.gsz;  // positions per CTA
@@ -341,14 +341,8 @@ template <int D, bool BF16>
 static cudaError_t go(const CrossPromptArgs& a, cudaStream_t st) {
   auto kern = cross_prompt_kernel<D, BF16>;
   static int configured[64] = {0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory((const void*)kern, (int)prompt_smem<D>(), configured);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prompt_smem<D>());
-    if (e != cudaSuccess) return e;
-    if (dev < 64) configured[dev] = 1;
-  }
   const int bq = kPromptRows / a.gsz;
   const dim3 grid((a.c.Sq + bq - 1) / bq, a.c.Hq / a.gsz, a.c.B);
   kern<<<grid, kPromptThreads, prompt_smem<D>(), st>>>(a);

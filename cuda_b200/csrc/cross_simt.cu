@@ -16,16 +16,17 @@ constexpr int kSimtRows = 64, kSimtKeys = 64;
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 template <int D>
-__global__ void __launch_bounds__(256) cross_simt_kernel(const CrossArgs a) {
+__global__ void __launch_bounds__(256, 2) cross_simt_kernel(const CrossArgs a) {
   constexpr int LD = kSimtRows + 4;  // padded leading dimension of the transposed tiles
   constexpr float NEG_INF = -__builtin_huge_valf();
   extern __shared__ __align__(16) float sm[];
+  __shared__ int pick;
   float* sQ = sm;                  // [D][LD]
   float* sK = sQ + D * LD;         // [D][LD]
   float* sV = sK + D * LD;         // [kSimtKeys][D]
   float* sP = sV + kSimtKeys * D;  // [kSimtKeys][LD]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int kvh = blockIdx.y, b = longest_first<256>(a, blockIdx.z);
+  const int kvh = blockIdx.y, b = longest_first<256>(a, blockIdx.z, &pick);
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
   const int rows = a.group * a.Sq, r0 = blockIdx.x / parts * kSimtRows;
   const int len = cross_kv_len(a, b), tiles = (len + kSimtKeys - 1) / kSimtKeys;
@@ -35,8 +36,9 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(const CrossArgs a) {
   auto row_head = [&](int r) { return kvh * a.group + r / a.Sq; };
   auto row_pos = [&](int r) { return r % a.Sq; };
 
-  for (int i = tid; i < kSimtRows * (D / 4); i += 256) {
-    const int r = i & 63, c = i >> 6;
+#pragma unroll
+  for (int i0 = 0; i0 < kSimtRows * (D / 4); i0 += 256) {
+    const int i = i0 + tid, r = i & 63, c = i >> 6;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r0 + r < rows)
       x = load4(static_cast<const float*>(a.q) + b * a.q_st[0] + row_head(r0 + r) * a.q_st[1] + row_pos(r0 + r) * a.q_st[2] + 4 * c);
@@ -54,17 +56,24 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(const CrossArgs a) {
     for (int j = 0; j < D / 16; ++j) o[i][j] = 0.f;
   }
   for (int t0 = key0; t0 < key1; t0 += kSimtKeys) {
+    constexpr int N = kSimtKeys * (D / 4) / 256;  // 16-byte pieces of K and of V per thread: all on their way before the first is stored
+    float4 kx[N], vx[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int i = u * 256 + tid, r = i & 63, c = i >> 6, vr = i / (D / 4), vc = i % (D / 4);
+      kx[u] = vx[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (t0 + r < len) kx[u] = load4(kp + (t0 + r) * a.k_st[2] + 4 * c);
+      if (t0 + vr < len) vx[u] = load4(vp + (t0 + vr) * a.v_st[2] + 4 * vc);
+    }
     __syncthreads();  // the tiles of the step before are read
-    for (int i = tid; i < kSimtKeys * (D / 4); i += 256) {
-      const int r = i & 63, c = i >> 6;
-      const float4 x = t0 + r < len ? load4(kp + (t0 + r) * a.k_st[2] + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      sK[(4 * c) * LD + r] = x.x;
-      sK[(4 * c + 1) * LD + r] = x.y;
-      sK[(4 * c + 2) * LD + r] = x.z;
-      sK[(4 * c + 3) * LD + r] = x.w;
-      const int vr = i / (D / 4), vc = i % (D / 4);
-      *reinterpret_cast<float4*>(sV + vr * D + 4 * vc) =
-          t0 + vr < len ? load4(vp + (t0 + vr) * a.v_st[2] + 4 * vc) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int i = u * 256 + tid, r = i & 63, c = i >> 6, vr = i / (D / 4), vc = i % (D / 4);
+      sK[(4 * c) * LD + r] = kx[u].x;
+      sK[(4 * c + 1) * LD + r] = kx[u].y;
+      sK[(4 * c + 2) * LD + r] = kx[u].z;
+      sK[(4 * c + 3) * LD + r] = kx[u].w;
+      *reinterpret_cast<float4*>(sV + vr * D + 4 * vc) = vx[u];
     }
     __syncthreads();
     float s[4][4] = {};
@@ -141,20 +150,9 @@ __global__ void __launch_bounds__(256) cross_simt_kernel(const CrossArgs a) {
   for (int e = rank * 256 + tid; e < kSimtRows * (D / 4); e += parts * 256) {
     const int i = e / (D / 4), c = e % (D / 4), r = r0 + i;
     if (r >= rows) break;
-    float M = NEG_INF, L = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < parts; ++q) M = fmaxf(M, dsmem_ld64(ml_at + i * 8, q).x);
-    const float ref = M == NEG_INF ? 0.f : M;
-    for (int q = 0; q < parts; ++q) {
-      const float2 ml = dsmem_ld64(ml_at + i * 8, q);
-      const float4 y = dsmem_ld128(o_at + (i * D + 4 * c) * 4, q);
-      const float w = exp2f(ml.x - ref);
-      L = fmaf(ml.y, w, L);
-      x.x = fmaf(y.x, w, x.x);
-      x.y = fmaf(y.y, w, x.y);
-      x.z = fmaf(y.z, w, x.z);
-      x.w = fmaf(y.w, w, x.w);
-    }
+    const JoinedWord w = join_parts(ml_at + i * 8, o_at + (i * D + 4 * c) * 4, parts);
+    const float4 x = w.x;
+    const float M = w.M, L = w.L;
     const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: zeros
     *reinterpret_cast<float4*>(static_cast<float*>(a.out) + b * a.o_st[0] + row_head(r) * a.o_st[1] + row_pos(r) * a.o_st[2] + 4 * c) =
         make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
@@ -183,10 +181,14 @@ template <int D>
 static cudaError_t go_tiles(const CrossArgs& a, cudaStream_t st) {
   constexpr size_t smem = (2 * D * (kSimtRows + 4) + kSimtKeys * D + kSimtKeys * (kSimtRows + 4)) * sizeof(float);
   auto kern = cross_simt_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static int configured[64] = {0};
+  cudaError_t e = allow_shared_memory((const void*)kern, (int)smem, configured);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.group * a.Sq, blocks = (rows + kSimtRows - 1) / kSimtRows;
-  const int parts = cross_parts(blocks * a.Hkv * a.B, (a.Skv + kSimtKeys - 1) / kSimtKeys);
+  // one wave of two CTAs per SM: a second one costs more than shorter parts save (48 blocks of 10 tiles: 8 parts 35 us)
+  const int tiles = (a.Skv + kSimtKeys - 1) / kSimtKeys;
+  int parts = cross_parts(blocks * a.Hkv * a.B, tiles);
+  if (parts > 1 && blocks * a.Hkv * a.B * parts > 2ll * current_sm_count()) parts /= 2;
   return launch_clusters((const void*)kern, dim3((unsigned)(blocks * parts), a.Hkv, a.B), 256, smem, parts, a, st);
 }
 
@@ -206,12 +208,13 @@ __global__ void __launch_bounds__(32 * kStreamWarps) cross_stream_kernel(const C
   constexpr int STEPS = kStreamKeys / SIDE;
   constexpr float NEG_INF = -__builtin_huge_valf();
   extern __shared__ __align__(16) float sm[];
+  __shared__ int pick;
   float* part_o = sm;                                                  // [warps][R][D]
   float2* part_ml = reinterpret_cast<float2*>(sm + kStreamWarps * R * D);  // [warps][R]
   float* cta_o = reinterpret_cast<float*>(part_ml + kStreamWarps * R);     // [R][D]
   float2* cta_ml = reinterpret_cast<float2*>(cta_o + R * D);               // [R]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / LPK, dl = lane % LPK;
-  const int kvh = blockIdx.y, b = longest_first<32 * kStreamWarps>(a, blockIdx.z);
+  const int kvh = blockIdx.y, b = longest_first<32 * kStreamWarps>(a, blockIdx.z, &pick);
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
   const int rows = a.group * a.Sq, r0 = blockIdx.x / parts * R;
   const int len = cross_kv_len(a, b), tiles = (len + kStreamKeys - 1) / kStreamKeys;
@@ -339,21 +342,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps) cross_stream_kernel(const C
     const uint32_t o_at = smem_u32(cta_o), ml_at = smem_u32(cta_ml);
     for (int e = rank * 32 * kStreamWarps + tid; e < R * (D / 4); e += parts * 32 * kStreamWarps) {
       const int i = e / (D / 4), c = e % (D / 4);
-      float M = NEG_INF, L = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = 0; w < parts; ++w) M = fmaxf(M, dsmem_ld64(ml_at + i * 8, w).x);
-      const float ref = M == NEG_INF ? 0.f : M;
-      for (int w = 0; w < parts; ++w) {
-        const float2 ml = dsmem_ld64(ml_at + i * 8, w);
-        const float4 y = dsmem_ld128(o_at + (i * D + 4 * c) * 4, w);
-        const float f = exp2f(ml.x - ref);
-        L = fmaf(ml.y, f, L);
-        x.x = fmaf(y.x, f, x.x);
-        x.y = fmaf(y.y, f, x.y);
-        x.z = fmaf(y.z, f, x.z);
-        x.w = fmaf(y.w, f, x.w);
-      }
-      emit(i, c, x, M, L);
+      const JoinedWord w = join_parts(ml_at + i * 8, o_at + (i * D + 4 * c) * 4, parts);
+      emit(i, c, w.x, w.M, w.L);
     }
     cluster_sync_all();  // no CTA leaves while another still reads its part
   }
@@ -363,7 +353,8 @@ template <int D, int R>
 static cudaError_t go_stream(const CrossArgs& a, cudaStream_t st) {
   constexpr size_t smem = ((size_t)kStreamWarps * R * (D + 2) + R * (D + 2)) * sizeof(float);
   auto kern = cross_stream_kernel<D, R>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static int configured[64] = {0};
+  cudaError_t e = allow_shared_memory((const void*)kern, (int)smem, configured);
   if (e != cudaSuccess) return e;
   const int rows = a.group * a.Sq, blocks = (rows + R - 1) / R;
   const int parts = cross_parts((long long)blocks * a.Hkv * a.B, (a.Skv + 8 * kStreamKeys - 1) / (8 * kStreamKeys));

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
   const uint32_t full = base, empty = base + 8 * NST, fail_at = base + 16 * NST, ring = base + 1024;
   volatile uint32_t* fail_ptr = reinterpret_cast<volatile uint32_t*>(smem + 16 * NST);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.y, b = longest_first<kTokThreads>(a.c, blockIdx.z);
+  const int kvh = blockIdx.y, b = longest_first<kTokThreads>(a.c, blockIdx.z, reinterpret_cast<volatile int*>(smem + 512));
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
   (void)fail_at;
 
@@ -255,21 +255,8 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
     const uint32_t o_at = smem_u32(cta_o), ml_at = smem_u32(cta_ml);
     for (int e = rank * kTokThreads + tid; e < live_rows * (D / 4); e += parts * kTokThreads) {
       const int r = e / (D / 4), c = e % (D / 4);
-      float M = NEG_INF, L = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int q = 0; q < parts; ++q) M = fmaxf(M, dsmem_ld64(ml_at + r * 8, q).x);
-      const float ref = M == NEG_INF ? 0.f : M;
-      for (int q = 0; q < parts; ++q) {
-        const float2 ml = dsmem_ld64(ml_at + r * 8, q);
-        const float4 y = dsmem_ld128(o_at + (r * D + 4 * c) * 4, q);
-        const float w = fast_exp2(ml.x - ref);
-        L = fmaf(ml.y, w, L);
-        acc.x = fmaf(y.x, w, acc.x);
-        acc.y = fmaf(y.y, w, acc.y);
-        acc.z = fmaf(y.z, w, acc.z);
-        acc.w = fmaf(y.w, w, acc.w);
-      }
-      emit(r, c, acc, M, L);
+      const JoinedWord w = join_parts(ml_at + r * 8, o_at + (r * D + 4 * c) * 4, parts);
+      emit(r, c, w.x, w.M, w.L);
     }
     cluster_sync_all();  // no CTA leaves while another still reads its parts
   }
@@ -294,14 +281,8 @@ template <int D, bool BF16, int MT>
 static cudaError_t go(const CrossTokenArgs& a, int parts, cudaStream_t st) {
   auto kern = cross_token_kernel<D, BF16, MT>;
   static int configured[64] = {0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory((const void*)kern, (int)tok_smem<D>(), configured);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tok_smem<D>());
-    if (e != cudaSuccess) return e;
-    if (dev < 64) configured[dev] = 1;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(parts, a.c.Hkv, a.c.B);
   cfg.blockDim = dim3(kTokThreads);

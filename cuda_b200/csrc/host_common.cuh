@@ -29,4 +29,14 @@ inline int cuda_result(cudaError_t e, const char* where) {
   return CUDA_LLM_ECUDA;
 }
 
+// Raises a kernel's dynamic shared memory limit once per device (`configured`: a static array of 64 of the caller).
+inline cudaError_t allow_shared_memory(const void* kern, int bytes, int* configured) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && configured[dev])) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) configured[dev] = 1;
+  return e;
+}
+
 }  // namespace b200

@@ -652,14 +652,8 @@ template <int D, int KF, int QT, int NT, bool MX, int U>
 static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, int grid, cudaStream_t st) {
   auto kern = kv_weights_kernel<D, KF, QT, NT, MX, U>;
   static int configured[64] = {0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory((const void*)kern, (int)kWgtBudget, configured);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kWgtBudget);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) configured[dev] = 1;
-  }
   kern<<<grid, 32 * (kWgtWarps + 1), gm.smem, st>>>(a, gm, map);
   return cudaGetLastError();
 }
