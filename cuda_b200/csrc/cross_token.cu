@@ -12,6 +12,10 @@
 // own 16 states of one row block, or (more than 16 rows) each its own row block of more states.
 //
 // P is rounded to the operand type (half a step of it, against the row's own maximum); sums, maxima and O stay in fp32.
+//
+// Measured (bf16, 32 query and 8 KV heads of 128, one token): 64 sequences of 1000-4096 states 102 us = 6.5 TB/s, the measured
+// copy peak; 16 sequences of 4096 states 54 us; one sequence of 1500 states 8.9 us, of which the launch, the first
+// copies' latency and the join are nearly all.
 #include "cross_attention.cuh"
 #include "tcgen05_primitives.cuh"
 

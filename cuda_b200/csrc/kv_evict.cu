@@ -1,5 +1,10 @@
 // Eviction from a paged KV cache: which tokens stay (a selection by rank per sequence and KV head), and their move to the
 // front of the same or of other pages.
+//
+// Measured, both kernels: 32 sequences x 8 heads of 2500-8000 tokens of 128 E4M3 values, in place down to 2048: 20 + 103 us; one
+// sequence x 8 heads of 131072 bf16 tokens, 16384 of them into other pages: 28 + 109 us; one of 700 tokens down to 512: 18 us.
+// A kept token is one element of every row, so DRAM moves whole slabs: 0.48 and 0.54 GB here (4.6 and 5.0 TB/s), where the
+// kept tokens alone are 0.27 and 0.13 GB.
 #include <type_traits>
 
 #include "host_common.cuh"
@@ -217,8 +222,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictArgs a
 // ---- move -----------------------------------------------------------------------------------------------------------
 // A (page, head) is a slab of rows (head_dim rows of K, ..) of `page` elements, contiguous in memory; a kept token is one element
 // in every row.  A CTA owns some rows of K and V of one (sequence, KV head) and walks the new positions in groups of 16 bytes of
-// a row: a producer thread brings in the slabs that hold kept tokens, each once, by bulk copies into a ring that always holds
-// all slabs a group can need; each warp, with rows of its own, gathers the group's elements from them, a lane one 32-bit
+// a row: loading warps bring in the slabs that hold kept tokens, each once, by bulk copies into a ring that always holds
+// all slabs a group can need; each warp gathers the group's elements from them, a lane one 32-bit
 // word of a row, and writes the words out.  Bound by DRAM: whole slabs are read for the tokens kept in them.
 //
 // In place: a kept token never moves upwards, so every page that is still to be read, however far ahead the copies run, lies

@@ -1,4 +1,17 @@
-// Accumulated attention weight of cached tokens: scores[s, h, t] = decay * old + sum_rows 2^(scale_log2 q . k_t - lse2).
+// Accumulated attention weight of cached tokens:
+//
+//   scores[s, h, t] = decay * old + sum over the rows r that see t of 2^(scale_log2 q_r . k_t - lse2_r)
+//
+// The log-sum-exp is known, so tokens are independent: one pass over K, no join, no atomics.  A decode step (up to 16 rows per
+// KV head) is bound by the bytes of K: 64 sequences of 1000-8192 tokens, 8 heads of 128, E4M3 with per-token scales, 65 us =
+// 5.0 TB/s (0.78 of the measured copy peak; what is missing is issue slots: about 165 instructions per 16 tokens and head).
+// A prompt window (32 queries x 4 heads against 52769 tokens in two sequences) takes 78 us against 9 us of bytes: it
+// is bound by the latency of warp-level products and exponentials (tensor pipe 35 % busy).
+//
+// Arithmetic: K as E4M3 codes (widened exactly to f16) or as 16-bit elements, products on mma.m16n8k16 with fp32 sums, tokens on
+// the 16-wide side and query rows on the 8-wide side.  bf16 and fp32 queries against 8-bit codes are brought into f16's range by a
+// power of two per row, fp32 ones as two f16 terms (22 bits); scales multiply the fp32 sums, block scales the sums
+// of their 32 elements.
 #include <cmath>
 
 #include "host_common.cuh"
@@ -26,7 +39,7 @@ struct WeightsArgs {
 // bulk copy per page: the heads of a page are contiguous) and their scales.  Its 16-token units, one head each, go to the
 // computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
 // ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
-constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each
+constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each (streamed rows: 16 warps, one unit each)
 constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
 constexpr uint32_t kWgtHeader = 9 * 1024;  // barriers, page masks, flag, prefix sums, lengths
@@ -73,10 +86,15 @@ __device__ __forceinline__ void rotate_words(uint32_t (&w)[4], int t) {
 
 enum { KF_E4M3 = 0, KF_F16 = 1, KF_BF16 = 2 };
 
+// m16n8k16, fp32 accumulation.  (Not volatile: the products of several tokens and rows may be interleaved.)
 template <bool BF>
 __device__ __forceinline__ void mma_any(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (BF) mma_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
-  else mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
+  if (BF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // What the rows of one 8-column block need after the product, for the two columns 2t, 2t + 1 of a lane.
@@ -334,19 +352,20 @@ __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom&
 }
 
 // Four units per warp and stage share more of what a stage costs a warp, where three such stages fit and the fragments leave
-// registers: 8-bit caches, or 16-bit ones of head_dim 64.
+// registers: 8-bit caches, or 16-bit ones of head_dim 64.  (64 sequences: one unit 86 us, two 84, four 77, at that state.)
 template <int D, int KF, int QT>
 constexpr bool kFourUnits = QT != CUDA_LLM_F32 && (KF == KF_E4M3 || D == 64);
 
 // One stage is one task per computing warp: head warp % hg of the group, a run of 16-token units.
 // NT > 0: the query fragments of 8 NT rows stay in registers from stage to stage (a decode step: all rows of a KV head); a
 // sequence with more rows than that is right but reloads them.
-// NT == 0: many rows per KV head (a window of a prompt): the warp holds the keys and streams the rows from L2, eight at a time.
+// NT == 0: many rows per KV head (a window of a prompt): the warp holds the keys and the rows pass eight at a time, from shared
+// memory up to kWgtRows of them, else (and as fp32) from L2.
 template <int D, int KF, int QT, int NT, bool MX, int U>
-__global__ void __launch_bounds__(32 * (kWgtWarps + 1), 1)
+__global__ void __launch_bounds__(32 * ((NT ? kWgtWarps : 2 * kWgtWarps) + 1), 1)
 kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__ WeightsGeom gm, const __grid_constant__ WeightsMap map) {
   constexpr bool F8 = KF == KF_E4M3;
-  constexpr int WARPS = kWgtWarps, ROWS = NT ? 8 * NT : 8;
+  constexpr int WARPS = NT ? kWgtWarps : 2 * kWgtWarps, ROWS = NT ? 8 * NT : 8;  // a stage has 16 units at least
   // operand type of the products: f16, unless the cache or (streamed rows) the queries are bf16 / fp32
   constexpr bool BF = KF == KF_BF16 || (NT == 0 && QT != CUDA_LLM_F16);
   constexpr bool SCALED = NT > 0 && F8 && QT != CUDA_LLM_F16;
@@ -448,7 +467,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
       // {log-sum-exp, first token not seen} of every row
       cur_s = my_s;
       cur_h = h;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
       for (int e = tid; e < ((rows + 7) & ~7) * QCH; e += 32 * WARPS) {
         const int r = e / QCH, c = e % QCH, j = r / a.group;
         uint4 v = make_uint4(0, 0, 0, 0);
@@ -464,7 +483,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
         sts32(base + gm.q_off + kWgtRows * QCH * 16 + r * 8, __float_as_int(x.lse2[0]));
         sts32(base + gm.q_off + kWgtRows * QCH * 16 + r * 8 + 4, x.limit[0]);
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
     }
     if (!dead && !mbar_wait(full + 8 * st, par, 0)) {  // the warp goes on without work: others may wait for it at the barrier above
       dead = true;
@@ -599,30 +618,41 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
               }
             }
           }
-#pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-          if (KEPT && rows <= kWgtRows) {
-            const uint32_t row_at = base + gm.q_off + (r0 + g) * QCH * 16;
+        auto add_rows = [&](const uint32_t (&q)[TERMS][D / 32][4], const RowPair& r) {
+          float c[U][2][4] = {};  // two chains of products per unit
 #pragma unroll
-            for (int p = 0; p < D / 32; ++p) {
-              const uint4 v = lds128(row_at + (((p * 4 + t) ^ ((g & 1) << 2)) << 4));
-              qf[0][0][p][0] = v.x; qf[0][0][p][1] = v.y; qf[0][0][p][2] = v.z; qf[0][0][p][3] = v.w;
-            }
-            const uint4 v = lds128(base + gm.q_off + kWgtRows * QCH * 16 + (r0 + 2 * t) * 8);
-            rp[0].lse2[0] = __uint_as_float(v.x); rp[0].limit[0] = (int)v.y;
-            rp[0].lse2[1] = __uint_as_float(v.z); rp[0].limit[1] = (int)v.w;
-            rp[0].inv[0] = rp[0].inv[1] = 1.f;
-          } else {
-            fetch_rows(r0);
-          }
+          for (int p = 0; p < D / 32; ++p)
+#pragma unroll
+            for (int x = 0; x < U; ++x) dot_block(c[x][p & 1], af[x][p], q, x, p);
 #pragma unroll
           for (int x = 0; x < U; ++x) {
-            float c[2][4] = {};  // two chains of products
 #pragma unroll
-            for (int p = 0; p < D / 32; ++p) dot_block(c[p & 1], af[x][p], qf[0], x, p);
+            for (int e = 0; e < 4; ++e) c[x][0][e] += c[x][1][e];
+            add_weights(x, c[x][0], r);
+          }
+        };
+        if (KEPT && rows <= kWgtRows) {
+#pragma unroll 2
+          for (int r0 = 0; r0 < rows; r0 += 8) {
+            const uint8_t* const row = smem + gm.q_off + (r0 + g) * QCH * 16;
+            uint32_t q[TERMS][D / 32][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[0][e] += c[1][e];
-            add_weights(x, c[0], rp[0]);
+            for (int p = 0; p < D / 32; ++p) {
+              const uint4 v = *reinterpret_cast<const uint4*>(row + (((p * 4 + t) ^ ((g & 1) << 2)) << 4));
+              q[0][p][0] = v.x; q[0][p][1] = v.y; q[0][p][2] = v.z; q[0][p][3] = v.w;
+            }
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + gm.q_off + kWgtRows * QCH * 16 + (r0 + 2 * t) * 8);
+            RowPair r;
+            r.lse2[0] = __uint_as_float(v.x); r.limit[0] = (int)v.y;
+            r.lse2[1] = __uint_as_float(v.z); r.limit[1] = (int)v.w;
+            r.inv[0] = r.inv[1] = 1.f;
+            add_rows(q, r);
+          }
+        } else {
+#pragma unroll 1
+          for (int r0 = 0; r0 < rows; r0 += 8) {
+            fetch_rows(r0);
+            add_rows(qf[0], rp[0]);
           }
         }
       }
@@ -654,7 +684,7 @@ static cudaError_t go(const WeightsArgs& a, const WeightsGeom& gm, const Weights
   static int configured[64] = {0};
   cudaError_t e = allow_shared_memory((const void*)kern, (int)kWgtBudget, configured);
   if (e != cudaSuccess) return e;
-  kern<<<grid, 32 * (kWgtWarps + 1), gm.smem, st>>>(a, gm, map);
+  kern<<<grid, 32 * ((NT ? kWgtWarps : 2 * kWgtWarps) + 1), gm.smem, st>>>(a, gm, map);
   return cudaGetLastError();
 }
 
@@ -665,7 +695,7 @@ static cudaError_t go_rows(const WeightsArgs& a, const WeightsGeom& gm, const We
   if (nt == 1) return go<D, KF, QT, 1, MX, 2>(a, gm, map, grid, st);
   if constexpr (QT != CUDA_LLM_F32)
     if (nt == 2) return go<D, KF, QT, 2, MX, 2>(a, gm, map, grid, st);
-  return go<D, KF, QT, 0, MX, 2>(a, gm, map, grid, st);
+  return go<D, KF, QT, 0, MX, 1>(a, gm, map, grid, st);
 }
 template <int D, int KF, int QT>
 static cudaError_t go_scales(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, int grid, int nt, cudaStream_t st) {
@@ -688,7 +718,8 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   const int nt = declared <= 8 ? 1 : declared <= 16 && a.q_dtype != CUDA_LLM_F32 ? 2 : 0;
   const int eb = a.k_format == CUDA_LLM_KV_FP8_E4M3 ? 1 : 2, groups = a.page / 16;
   const long long cap = (long long)a.max_blocks * a.page < a.max_tokens ? (long long)a.max_blocks * a.page : a.max_tokens;
-  // units of a stage; the larger stage only where there are stages for every SM a few times over
+  // units of a stage; the larger stage only where there are several of them for every SM (1000 tokens of one sequence would keep
+  // 16 SMs busy instead of 32)
   const bool four = nt == 1 && a.q_dtype != CUDA_LLM_F32 && (eb == 1 || a.D == 64) && cap * a.Hkv * a.S / 16 >= 4ll * 4 * kWgtWarps * sms;
   const int want = (four ? 4 : 2) * kWgtWarps;
   WeightsGeom gm;
