@@ -19,10 +19,11 @@
 //
 // Measured: bf16, 4 x 32 / 8 heads of 128, 2048 positions, 4096-8192 states: 717 us = 1150 TFLOP/s cold, 790 us back to back under
 // the power cap (0.74 of the sustained cuBLAS rate).  fp16, 8 x 16 heads of 64, 447 positions, 201-1500 states: 37 us.
-// A pair of tiles takes about 3440 cycles per 128 states, 2048 of them MMA at the nominal rate; the tensor pipe counts 1.46 times
+// A pair of tiles took about 3440 cycles per 128 states (by the clock register, before the last steps), 2048 of them MMA at the nominal rate; the tensor pipe counts 1.46 times
 // its nominal cycles, since an MMA of 128 x 128 with both operands in shared memory reads them at exactly the rate of
-// the memory, beside the TMA's writes.  Tried and slower: a cubic exponential on the FMA pipe for 25-50 % of the weights (765 ->
-// 835-844 us), P handed over in two or four parts (804-880), two threads per row (751).  Two CTAs per MMA
+// the memory, beside the TMA's writes.  Tried and slower, each against this form in the
+// same run: a polynomial exponential on the FMA pipe for 25 / 33 / 50 % of the weights (765 -> 797 / 835 / 844 us), P handed over
+// in four parts (725 -> 879-887) or two (754 -> 787-804); two threads per row (717 -> 750, separate runs).  Two CTAs per MMA
 // (half of B from each) would relieve the operand reads.
 // All waits are bounded; one that runs out raises a counter and the CTA falls through to the exit that frees TMEM.
 #include "cross_attention.cuh"

@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps) cross_stream_kernel(const C
       float s[STEPS];
 #pragma unroll
       for (int x = 0; x < STEPS; ++x) s[x] = fmaf(q[r].x, k[x].x, fmaf(q[r].y, k[x].y, fmaf(q[r].z, k[x].z, q[r].w * k[x].w)));
-      int have = STEPS, bit = LPK / 2;
+      int bit = LPK / 2;
 #pragma unroll
       for (int half = STEPS / 2; half >= 1; half /= 2) {
         const bool up = dl & bit;
@@ -265,7 +265,6 @@ __global__ void __launch_bounds__(32 * kStreamWarps) cross_stream_kernel(const C
           }
         bit /= 2;
       }
-      (void)have;
       float sum = s[0];
 #pragma unroll
       for (int o2 = LPK / STEPS / 2; o2 >= 1; o2 /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o2);

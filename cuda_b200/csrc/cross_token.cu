@@ -14,7 +14,7 @@
 // P is rounded to the operand type (half a step of it, against the row's own maximum); sums, maxima and O stay in fp32.
 //
 // Measured (bf16, 32 query and 8 KV heads of 128, one token): 64 sequences of 1000-4096 states 102 us = 6.5 TB/s, the measured
-// copy peak; 16 sequences of 4096 states 54 us; one sequence of 1500 states 8.9 us, of which the launch, the first
+// copy peak; 16 sequences of 4096 states 54 us; one sequence of 1500 states 8.2 us, of which the launch, the first
 // copies' latency and the join are nearly all.
 #include "cross_attention.cuh"
 #include "tcgen05_primitives.cuh"
@@ -50,12 +50,11 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
   constexpr float NEG_INF = -__builtin_huge_valf();
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t full = base, empty = base + 8 * NST, fail_at = base + 16 * NST, ring = base + 1024;
+  const uint32_t full = base, empty = base + 8 * NST, ring = base + 1024;
   volatile uint32_t* fail_ptr = reinterpret_cast<volatile uint32_t*>(smem + 16 * NST);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.y, b = longest_first<kTokThreads>(a.c, blockIdx.z, reinterpret_cast<volatile int*>(smem + 512));
   const int rank = (int)cluster_rank(), parts = (int)cluster_size();
-  (void)fail_at;
 
   if (tid == 0) {
     for (int i = 0; i < NST; ++i) {

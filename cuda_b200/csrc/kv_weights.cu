@@ -4,9 +4,10 @@
 //
 // The log-sum-exp is known, so tokens are independent: one pass over K, no join, no atomics.  A decode step (up to 16 rows per
 // KV head) is bound by the bytes of K: 64 sequences of 1000-8192 tokens, 8 heads of 128, E4M3 with per-token scales, 65 us =
-// 5.0 TB/s (0.78 of the measured copy peak; what is missing is issue slots: about 165 instructions per 16 tokens and head).
-// A prompt window (32 queries x 4 heads against 52769 tokens in two sequences) takes 78 us against 9 us of bytes: it
-// is bound by the latency of warp-level products and exponentials (tensor pipe 35 % busy).
+// 5.0 TB/s (0.78 of the measured copy peak; what is missing is issue slots: 165 warp instructions per 16 tokens and head, counted
+// when it took 77 us).
+// A prompt window (32 queries x 4 heads against 52769 tokens in two sequences) takes 76-78 us against 9 us of bytes (8 warps with
+// two units: 82): it is bound by the latency of warp-level products and exponentials (tensor pipe 35 % busy, counted with 8 warps).
 //
 // Arithmetic: K as E4M3 codes (widened exactly to f16) or as 16-bit elements, products on mma.m16n8k16 with fp32 sums, tokens on
 // the 16-wide side and query rows on the 8-wide side.  bf16 and fp32 queries against 8-bit codes are brought into f16's range by a
@@ -39,7 +40,7 @@ struct WeightsArgs {
 // bulk copy per page: the heads of a page are contiguous) and their scales.  Its 16-token units, one head each, go to the
 // computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
 // ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
-constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each (streamed rows: 16 warps, one unit each)
+constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each (streamed rows: 16 warps, one each)
 constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
 constexpr uint32_t kWgtHeader = 9 * 1024;  // barriers, page masks, flag, prefix sums, lengths
