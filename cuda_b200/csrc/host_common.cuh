@@ -29,6 +29,14 @@ inline int cuda_result(cudaError_t e, const char* where) {
   return CUDA_LLM_ECUDA;
 }
 
+// Whether no two of the rows [n0][n1] of `width` elements, addressed by two strides, share an element.
+inline bool rows_apart(long long st0, long long n0, long long st1, long long n1, long long width) {
+  if (n0 <= 1) return n1 <= 1 || st1 >= width;
+  if (n1 <= 1) return st0 >= width;
+  const bool first = st0 <= st1;  // which index steps over the shorter distance
+  return first ? st0 >= width && st1 >= st0 * (n0 - 1) + width : st1 >= width && st0 >= st1 * (n1 - 1) + width;
+}
+
 // Raises a kernel's dynamic shared memory limit once per device (`configured`: a static array of 64 of the caller).
 inline cudaError_t allow_shared_memory(const void* kern, int bytes, int* configured) {
   int dev = 0;

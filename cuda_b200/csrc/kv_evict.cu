@@ -651,6 +651,7 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   }
   if (p->budget < 1 || p->sink < 0 || p->recent < 0 || (long long)p->sink + p->recent > p->budget)
     return refuse(CUDA_LLM_EINVAL, "budget must be at least 1 and at least sink + recent");
+  if (p->budget > (1 << 30)) return refuse(CUDA_LLM_EINVAL, "a budget of more than 2^30 tokens");
   if (p->max_tokens > CUDA_LLM_EVICT_MAX_TOKENS) return refuse(CUDA_LLM_EINVAL, "score rows of more than CUDA_LLM_EVICT_MAX_TOKENS entries");
   if (p->num_seqs == 0) return CUDA_LLM_OK;
   if (p->max_blocks_per_seq < 0 || p->new_max_blocks_per_seq < 0 || p->num_blocks <= 0)
@@ -667,6 +668,11 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
   long long most = (long long)p->max_blocks_per_seq * p->page_size;
   if (most > p->max_tokens) most = p->max_tokens;
   if (most > p->budget) most = p->budget;
+  if (p->new_scores && !rows_apart(p->new_score_strides[0], p->num_seqs, p->new_score_strides[1], p->num_kv_heads, most))
+    return refuse(CUDA_LLM_EINVAL, "new score rows overlap");
+  if (p->new_scores == p->scores &&
+      ((p->num_seqs > 1 && p->new_score_strides[0] != p->score_strides[0]) || (p->num_kv_heads > 1 && p->new_score_strides[1] != p->score_strides[1])))
+    return refuse(CUDA_LLM_EINVAL, "new_scores is scores with other strides");
   if ((long long)p->new_max_blocks_per_seq * p->page_size < most) return refuse(CUDA_LLM_EINVAL, "new_block_tables is too narrow for the kept tokens");
   if (((uintptr_t)p->key_cache | (uintptr_t)p->value_cache | (scaled ? (uintptr_t)p->k_scale | (uintptr_t)p->v_scale : 0)) & 15)
     return refuse(CUDA_LLM_EALIGN, "caches and scales must be 16-byte aligned");

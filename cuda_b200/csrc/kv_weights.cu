@@ -800,6 +800,9 @@ extern "C" int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* p, v
   if (!p->key_cache || !p->block_tables || !p->context_lens || !p->scores || (!kv16 && !p->k_scale) ||
       (p->total_q > 0 && (!p->query || !p->lse)))
     return refuse(CUDA_LLM_EINVAL, "null tensor");
+  if (p->max_tokens > (1 << 30)) return refuse(CUDA_LLM_EINVAL, "score rows of more than 2^30 entries");
+  if (!rows_apart(p->score_strides[0], p->num_seqs, p->score_strides[1], p->num_kv_heads, p->max_tokens))
+    return refuse(CUDA_LLM_EINVAL, "score rows overlap");
   if (!p->cu_q_lens && p->total_q != p->num_seqs) return refuse(CUDA_LLM_EINVAL, "query has more or fewer rows than sequences: pass cu_q_lens");
   if (((uintptr_t)p->query | (uintptr_t)p->key_cache | (uintptr_t)(kv16 ? nullptr : p->k_scale)) & 15)
     return refuse(CUDA_LLM_EALIGN, "query, cache and scales must be 16-byte aligned");

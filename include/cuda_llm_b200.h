@@ -332,9 +332,10 @@ int cuda_llm_mx_attention_tcgen05_launches(uint64_t* launches);
  *   out[b, h, i] = sum_t softmax_t(softmax_scale * q[b, h, i] . k[b, h / group, t]) v[b, h / group, t]
  * over the states t < kv_lens[b], group = num_q_heads / num_kv_heads.  A length of 0 (or less) gives zeros and a
  * log-sum-exp of -inf; a length above kv_len counts as kv_len.  What lies behind a sequence's length is not read into any
- * result (it may hold infinities and NaN).  Tensors are addressed by three strides each (batch, head, position, in
- * elements; head_dim is contiguous): [B, H, S, D] and [B, S, H, D] need no copy, a stride of 0 shares states
- * between batch rows (beams) or heads.  A dimension of one element may carry any stride.  No workspace; any
+ * result (it may hold infinities and NaN).  A row all of whose scores are -inf gives zeros, too; one with a score of
+ * NaN or +inf gives NaN.  Tensors are addressed by three strides each (batch, head, position, in elements; head_dim is
+ * contiguous): [B, H, S, D] and [B, S, H, D] need no copy, a stride of 0 shares states between batch rows
+ * (beams) or heads.  A dimension of one element may carry any stride.  `out` overlaps no input.  No workspace; any
  * number of calls may be in flight, on any streams.
  *   16-bit types: few query rows per KV head stream the states once, split over a thread-block cluster and joined
  *   through its shared memory; more rows run on tcgen05.mma.  fp32: a plain fp32 kernel. */
@@ -386,7 +387,7 @@ typedef struct CudaLlmKvWeightsParams {
   const int32_t* context_lens; /* [num_seqs]                                                    */
   const int32_t* cu_q_lens;    /* [num_seqs + 1], or NULL: one query token per sequence         */
   const float* lse;            /* [total_q, num_q_heads] natural log                            */
-  float* scores;               /* [num_seqs, num_kv_heads, max_tokens], read and written        */
+  float* scores;               /* [num_seqs, num_kv_heads, max_tokens], read and written; rows apart */
   uint32_t* status;            /* optional: CUDA_LLM_ST_* bits are OR-ed into it                */
   int64_t score_strides[2];    /* sequence, KV head, in elements                                */
   int32_t num_seqs;
@@ -418,14 +419,15 @@ int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* params, void* s
  *   length hold what they held.  The pages of a sequence must then be its own.
  *   another table: every sequence is copied, also one within its budget; its pages must not be pages that block_tables
  *   names, and the old ones are not written.
- * `new_scores`, if not NULL, receives the kept tokens' scores (it may be `scores` itself).  Entries behind the new
+ * `new_scores`, if not NULL, receives the kept tokens' scores (it may be `scores` itself, with the same strides, and must not
+ * overlap it otherwise; where tokens went, -0 comes back as +0 and NaN as one NaN).  Entries behind the new
  * length are not written, in the caches, the scales and new_scores alike.  Per-block scales are refused: tokens
  * of pages with different scales cannot share a page without being quantised again.  Lengths that pass the table or
  * the score row are cut (CUDA_LLM_ST_BAD_CTX); tokens whose old or new page index is outside the pool are not
  * moved (CUDA_LLM_ST_BAD_BLOCK). */
 typedef struct CudaLlmKvEvictParams {
   const float* scores;             /* [num_seqs, num_kv_heads, max_tokens]                      */
-  float* new_scores;               /* optional [num_seqs, num_kv_heads, >= budget]              */
+  float* new_scores;               /* optional [num_seqs, num_kv_heads, >= budget], rows apart  */
   void* key_cache;                 /* see CudaLlmKvFormat                                       */
   void* value_cache;
   void* k_scale;                   /* NULL for 16- and 32-bit caches                            */

@@ -145,3 +145,18 @@ def test_extension_signatures(ext):
                                             "recent", "new_block_tables", "new_scores", "kv_format", "status"))):
         for name in names:
             assert name + ":" in fn.__doc__, name
+
+
+@pytest.mark.parametrize("strides", [(0, 256), (512, 0), (256, 256), (512, 255), (511, 256), (-512, 256)])
+def test_score_rows_that_overlap(lib, strides):
+    pair = (C.c_int64 * 2)(*strides)
+    assert lib.cuda_llm_kv_accumulate_weights(C.byref(weights(score_strides=pair)), None) == L.EINVAL
+    assert lib.cuda_llm_kv_evict(C.byref(evict(new_scores=0xb000, new_score_strides=(C.c_int64 * 2)(*[x // 4 for x in strides]))), None) == L.EINVAL
+
+
+def test_limits_of_the_row_lengths(lib):
+    wide = (C.c_int64 * 2)(2 ** 33, 2 ** 31)
+    assert lib.cuda_llm_kv_accumulate_weights(C.byref(weights(max_tokens=2 ** 30 + 1, score_strides=wide)), None) == L.EINVAL
+    assert lib.cuda_llm_kv_evict(C.byref(evict(budget=2 ** 30 + 1)), None) == L.EINVAL
+    same = (C.c_int64 * 2)(1024, 512)
+    assert lib.cuda_llm_kv_evict(C.byref(evict(new_scores=0x1000, new_score_strides=same)), None) == L.EINVAL
