@@ -19,12 +19,12 @@
 //
 // Measured: bf16, 4 x 32 / 8 heads of 128, 2048 positions, 4096-8192 states: 717 us = 1150 TFLOP/s cold, 790 us back to back under
 // the power cap (0.74 of the sustained cuBLAS rate).  fp16, 8 x 16 heads of 64, 447 positions, 201-1500 states: 37 us.
-// A pair of tiles took about 3440 cycles per 128 states (by the clock register, before the last steps), 2048 of them MMA at the nominal rate; the tensor pipe counts 1.46 times
-// its nominal cycles, since an MMA of 128 x 128 with both operands in shared memory reads them at exactly the rate of
-// the memory, beside the TMA's writes.  Tried and slower, each against this form in the
-// same run: a polynomial exponential on the FMA pipe for 25 / 33 / 50 % of the weights (765 -> 797 / 835 / 844 us), P handed over
-// in four parts (725 -> 879-887) or two (754 -> 787-804); two threads per row (717 -> 750, separate runs).  Two CTAs per MMA
-// (half of B from each) would relieve the operand reads.
+// A pair of tiles took about 3440 cycles per 128 states (by the clock register, before the last steps), 2048 of them MMA at the
+// nominal rate; the tensor pipe counts 1.46 times its nominal cycles, since an MMA of 128 x 128 with both operands in shared memory
+// reads them at exactly the rate of the memory, beside the TMA's writes.  Tried and slower, each against this form in the same
+// run: a polynomial exponential on the FMA pipe for 25 / 33 / 50 % of the weights (765 -> 797 / 835 / 844 us), P handed over in
+// four parts (725 -> 879-887) or two (754 -> 787-804); two threads per row (717 -> 750, separate runs).  Two CTAs per MMA (half
+// of B from each) would relieve the operand reads.
 // All waits are bounded; one that runs out raises a counter and the CTA falls through to the exit that frees TMEM.
 #include "cross_attention.cuh"
 #include "softmax_math.cuh"
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + T_O + i * O_STEP, tP = tmem + lanes + T_P + i * P_STEP;
     const int r = i * 128 + row, head = head0 + r / BQ, pos = q0 + r % BQ;
-    float m_run = -1.0e30f, l_run = 0.f;
+    float m_run = -3.0e38f, l_run = 0.f;  // below every score but -inf, whose weight is then zero
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
       if (!tc_wait(s_full + 8 * i, j & 1)) { ok = false; break; }
@@ -310,7 +310,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
       if (lane == 0) give_up();
     } else {
       tc_fence_after();
-      const float inv = n_tiles > 0 ? 1.f / l_run : 0.f;
+      const bool seen = l_run != 0.f;  // the largest score weighs 1 at least, unless all are -inf
+      const float inv = seen ? 1.f / l_run : 0.f;
       const bool store = pos < a.c.Sq;
       uint16_t* op = static_cast<uint16_t*>(a.c.out) + b * a.c.o_st[0] + head * a.c.o_st[1] + (store ? pos : 0) * a.c.o_st[2];
 #pragma unroll 1
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
         }
       }
       if (store && a.c.lse)
-        a.c.lse[((size_t)b * a.c.Hq + head) * a.c.Sq + pos] = n_tiles > 0 ? kLn2 * (m_run + log2f(l_run)) : NEG_INF;
+        a.c.lse[((size_t)b * a.c.Hq + head) * a.c.Sq + pos] = seen ? kLn2 * (m_run + log2f(l_run)) : NEG_INF;
     }
   }
   }
