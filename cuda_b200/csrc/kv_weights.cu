@@ -6,8 +6,8 @@
 // KV head) is bound by the bytes of K: 64 sequences of 1000-8192 tokens, 8 heads of 128, E4M3 with per-token scales, 65 us =
 // 5.0 TB/s (0.78 of the measured copy peak; what is missing is issue slots: 165 warp instructions per 16 tokens and head, counted
 // when it took 77 us).
-// A prompt window (32 queries x 4 heads against 52769 tokens in two sequences) takes 76-78 us against 9 us of bytes (8 warps with
-// two units: 82): it is bound by the latency of warp-level products and exponentials (tensor pipe 35 % busy, counted with 8 warps).
+// Windows of a prompt with more rows go to kv_weights_window_kernel; those of up to 64 (or 128) rows stay here, bound by the latency
+// of warp-level products and exponentials (tensor pipe 35 % busy at 128 rows).
 //
 // Arithmetic: K as E4M3 codes (widened exactly to f16) or as 16-bit elements, products on mma.m16n8k16 with fp32 sums, tokens on
 // the 16-wide side and query rows on the 8-wide side.  bf16 and fp32 queries against 8-bit codes are brought into f16's range by a
@@ -15,25 +15,10 @@
 // of their 32 elements.
 #include <cmath>
 
-#include "host_common.cuh"
+#include "kv_weights.cuh"
 #include "tcgen05_primitives.cuh"
 
 namespace b200 {
-
-struct WeightsArgs {
-  const void* q;
-  const uint8_t* kc;
-  const uint8_t* ks;
-  const int32_t *bt, *ctx, *cuq;
-  const float* lse;
-  float* scores;
-  uint32_t* status;
-  long long st_seq, st_head;
-  int S, total_q, Hq, Hkv, group, D, page, max_blocks, num_blocks, max_tokens, q_dtype, k_format, scale_mode, causal;
-  int group_shift;  // log2(group), or -1
-  int q_first;  // query row of the first sequence when there are no offsets
-  float scale_log2, decay;
-};
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Geometry.  A stage of the ring holds K of `hg` KV heads of one sequence for tok_stage consecutive tokens (whole pages, one
@@ -41,7 +26,6 @@ struct WeightsArgs {
 // computing warps.  All stages of the call, in (sequence, head group, token) order, are cut into equal contiguous
 // ranges, one per CTA; every CTA finds its range from a prefix sum over the context lengths.
 constexpr int kWgtWarps = 8;          // computing warps; a stage is 2 or 4 16-token units for each (streamed rows: 16 warps, one each)
-constexpr int kWgtSeqs = 1024;        // sequences per launch (their prefix sums live in shared memory)
 constexpr int kWgtMaxStages = 8;
 constexpr uint32_t kWgtHeader = 9 * 1024;  // barriers, page masks, flag, prefix sums, lengths
 static_assert(192 + 4 * (2 * kWgtSeqs + 4) <= kWgtHeader, "header");
@@ -231,56 +215,6 @@ __device__ __forceinline__ void load_rows_scaled(const void* q, size_t at, bool 
   }
 }
 
-// The plan of a CTA: its range of stages and the prefix sums to find sequences by.
-struct WeightsPlan {
-  const int *pre, *lens;
-  int w0, w1, s0;
-};
-template <int THREADS>
-__device__ __forceinline__ WeightsPlan make_plan(const WeightsArgs& a, const WeightsGeom& gm, int* pre, int* lens) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int cap = (int)min((long long)a.max_blocks * a.page, (long long)a.max_tokens);
-  for (int s = tid; s < a.S; s += THREADS) {
-    int n = a.ctx[s];
-    if (n > cap) {
-      if (a.status && blockIdx.x == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_CTX);
-      n = cap;
-    }
-    lens[s] = max(n, 0);
-  }
-  __syncthreads();
-  if (tid < 32) {
-    int sum = 0;
-    if (lane == 0) pre[0] = 0;
-    for (int s0 = 0; s0 < a.S; s0 += 32) {
-      const int s = s0 + lane;
-      int x = s < a.S ? (lens[s] + gm.tok_stage - 1) / gm.tok_stage * gm.n_hg : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (s < a.S) pre[s + 1] = sum + x;
-      sum += __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
-  __syncthreads();
-  WeightsPlan p;
-  p.pre = pre;
-  p.lens = lens;
-  const long long total = pre[a.S];
-  p.w0 = (int)(total * blockIdx.x / gridDim.x);
-  p.w1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-  int lo = 0, hi = a.S - 1;  // the last sequence with pre[s] <= w0
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= p.w0) lo = mid;
-    else hi = mid - 1;
-  }
-  p.s0 = lo;
-  return p;
-}
-
 // Producer warp: lane 0 issues the copies; the block-table entries of the next 32 / pages stages are fetched by all lanes.
 // Beside a stage lies a mask of the pages that were copied (bad block-table entries are not).
 __device__ __forceinline__ void produce(const WeightsArgs& a, const WeightsGeom& gm, const WeightsMap& map, const WeightsPlan& pl, uint32_t full, uint32_t empty, uint32_t live_at,
@@ -392,7 +326,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
     *fail_ptr = 0;
     mbar_fence_init();
   }
-  const WeightsPlan pl = make_plan<32 * (WARPS + 1)>(a, gm, pre, lens);
+  const WeightsPlan pl = make_plan<32 * (WARPS + 1)>(a, gm.tok_stage, gm.n_hg, pre, lens);
   if (pl.w0 >= pl.w1) return;
   if (warp == WARPS) {
     produce(a, gm, map, pl, full, empty, live_at, ring, fail_ptr);
@@ -470,10 +404,8 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
       cur_h = h;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
       for (int e = tid; e < ((rows + 7) & ~7) * QCH; e += 32 * WARPS) {
-        const int r = e / QCH, c = e % QCH, j = r / a.group;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows)
-          v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + ((size_t)(my_q0 + j) * a.Hq + h * a.group + (r - j * a.group)) * D + c * 8);
+        const int r = e / QCH, c = e % QCH, from = min(r, rows - 1), j = from / a.group;
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + ((size_t)(my_q0 + j) * a.Hq + h * a.group + (from - j * a.group)) * D + c * 8);
         uint32_t x[4] = {v.x, v.y, v.z, v.w};
         rotate_words(x, c & 3);
         sts128(base + gm.q_off + (r * QCH + (c ^ ((r & 1) << 2))) * 16, x[0], x[1], x[2], x[3]);
@@ -498,11 +430,12 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
         cur_r = r0;
 #pragma unroll
         for (int nt = 0; nt < QN; ++nt) {
-          const int r = r0 + nt * 8 + g, j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
+          // rows that pad a block repeat the last one, with a weight of zero: an infinity in K then meets no zero
+          const int r = min(r0 + nt * 8 + g, rows - 1), j = a.group_shift >= 0 ? r >> a.group_shift : r / a.group;
           const size_t at = ((size_t)(my_q0 + j) * a.Hq + h * a.group + (r - j * a.group)) * D;
           row_pair(a, r0 + nt * 8, rows, my_q0, my_nq, my_ctx, h, t, rp[nt]);
-          if constexpr (SCALED) load_rows_scaled<D, QT, TERMS>(a.q, at, r < rows, t, qf[nt], rp[nt].inv);
-          else load_rows<D, QT>(a.q, at, r < rows, t, qf[nt]);
+          if constexpr (SCALED) load_rows_scaled<D, QT, TERMS>(a.q, at, rows > 0, t, qf[nt], rp[nt].inv);
+          else load_rows<D, QT>(a.q, at, rows > 0, t, qf[nt]);
         }
       };
       if (NT > 0 && (my_s != cur_s || h != cur_h || cur_r != 0)) fetch_rows(0);
@@ -722,6 +655,12 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   // units of a stage; the larger stage only where there are several of them for every SM (1000 tokens of one sequence would keep
   // 16 SMs busy instead of 32)
   const bool four = nt == 1 && a.q_dtype != CUDA_LLM_F32 && (eb == 1 || a.D == 64) && cap * a.Hkv * a.S / 16 >= 4ll * 4 * kWgtWarps * sms;
+  // Many rows (16-bit queries): on tcgen05.  us here / there, E4M3 keys: 20 rows 162 / 219, 64 rows 68 / 68, 128 rows 76 / 54, 256
+  // rows 360 / 66, 1024 rows 434 / 82; 16-bit keys: 64 rows 31 / 37, 128 rows 39 / 49.  8 heads of 1000 tokens, fewer tiles than
+  // SMs, 128 rows: 14.5 / 16.4.
+  const bool fills = cap * a.Hkv * a.S >= 256ll * sms;
+  const bool window = (declared > kWgtRows || (declared > 64 && eb == 1 && fills)) && a.q_dtype != CUDA_LLM_F32 &&
+                      !(a.q_dtype == CUDA_LLM_F16 && eb == 1 && a.scale_mode == CUDA_LLM_SCALE_MX_E8M0);
   const int want = (four ? 4 : 2) * kWgtWarps;
   WeightsGeom gm;
   gm.hg = nt ? 8 : 1;
@@ -767,7 +706,7 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
     x.scores += s0 * a.st_seq;
     const long long most = (cap + gm.tok_stage - 1) / gm.tok_stage * gm.n_hg * x.S;
     const int grid = (int)(most < sms ? most : sms);
-    const cudaError_t e = a.D == 64 ? go_types<64>(x, gm, map, grid, nt, st) : go_types<128>(x, gm, map, grid, nt, st);
+    const cudaError_t e = window ? launch_kv_weights_window(x, cap, sms, st) : a.D == 64 ? go_types<64>(x, gm, map, grid, nt, st) : go_types<128>(x, gm, map, grid, nt, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

@@ -117,6 +117,33 @@ def test_rows_in_and_out_of_shared_memory(q_dtype):
     E.check_weights(E.cache("w", lens=[200] * 6, q_lens=[32, 33, 31, 200, 1, 32], hq=8, hkv=2, d=64, page=64, q_dtype=q_dtype, seed=2))
 
 
+@pytest.mark.parametrize("fmt", ["fp8_token", "fp8_head", "fp8_block", "mx8", "bf16", "f16"])
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 64), (128, 16), (128, 32), (128, 64)])
+@pytest.mark.parametrize("q_len", [40, 90, 150])
+def test_windows_of_a_prompt(fmt, d, page, q_len):
+    """One, two and three blocks of 128 rows per KV head (40 to 150 queries of 4 heads), several tiles and heads for every CTA,
+    sequences without queries, of one token, of fewer tokens than queries."""
+    dt = torch.float16 if fmt == "f16" else torch.bfloat16
+    E.check_weights(E.cache("w", lens=[2900, 260, 0, 1, 4100, 700, 257, q_len], q_lens=[q_len, q_len, 0, 1, q_len, 0, 33, q_len], hq=32, hkv=8, d=d, page=page,
+                            fmt=fmt, q_dtype=dt, seed=d + page), causal=q_len != 90, decay=0.5)
+
+
+@pytest.mark.parametrize("fmt", ["fp8_token", "fp8_block"])
+def test_windows_of_a_prompt_in_other_layouts(fmt):
+    """fp16 queries on 8-bit keys, a group that is no power of two, one KV head; a page that is not in the pool."""
+    E.check_weights(E.cache("w", lens=[1500, 300], q_lens=[70, 64], hq=5, hkv=1, d=128, page=16, fmt=fmt, q_dtype=torch.float16, seed=3))
+    wl = E.cache("w", lens=[1500, 900], q_lens=[70, 64], hq=12, hkv=4, d=64, page=32, fmt=fmt, seed=4)
+    lse = E.true_lse(wl, True)
+    base = torch.rand(2, 4, wl.block_tables.shape[1] * 32, device="cuda")
+    fine = E.accumulate(wl, lse, base.clone())
+    wl.block_tables[0, 7], wl.block_tables[1, 3] = -5, wl.key_cache.shape[0]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = E.accumulate(wl, lse, base.clone(), status=status)
+    assert int(status) == L.ST_BAD_BLOCK
+    fine[0, :, 7 * 32:8 * 32], fine[1, :, 3 * 32:4 * 32] = base[0, :, 7 * 32:8 * 32], base[1, :, 3 * 32:4 * 32]
+    assert torch.equal(got, fine)
+
+
 @pytest.mark.parametrize("ragged", [False, True])
 def test_more_sequences_than_a_launch_holds(ragged):
     n = 2100
@@ -176,6 +203,33 @@ def test_score_rows_that_overlap_are_refused():
     # read only, they may: every head keeps the same tokens
     kept, _ = E.evict(wl, torch.rand(1, 1, 48, device="cuda").expand(2, 2, 48), 20)
     assert torch.equal(kept[0, 0], kept[0, 1]) and torch.equal(kept[0], kept[1])
+
+
+@pytest.mark.parametrize("q_lens", [None, [3, 40, 100]])
+@pytest.mark.parametrize("hq", [2, 6, 16])
+@pytest.mark.parametrize("fmt", ["bf16", "fp8_token", "mx8"])
+def test_keys_that_are_not_finite(fmt, hq, q_lens):
+    """A token that scores -inf in every row weighs nothing, one that is NaN becomes NaN, and no other token feels them."""
+    wl = E.cache("w", lens=[70, 150, 333], q_lens=q_lens, hq=hq, hkv=2, d=64, page=16, fmt=fmt, seed=hq)
+    wl.query[..., 0] = 1.0
+    lse = E.true_lse(wl, True)
+    base = torch.rand(3, 2, wl.block_tables.shape[1] * 16, device="cuda")
+    fine = E.accumulate(wl, lse, base.clone())
+    tokens = {0: 5, 1: 20, 2: 200}
+    for s, t in tokens.items():
+        page = int(wl.block_tables[s, t // 16])
+        if fmt == "bf16":
+            wl.key_cache[page, :, 0, t % 16] = -math.inf
+        wl.key_cache[page, :, 3, t % 16 + 1] = math.nan if fmt == "bf16" else 0x7f
+    got = E.accumulate(wl, lse, base.clone())
+    same = torch.ones_like(base, dtype=torch.bool)
+    for s, t in tokens.items():
+        assert got[s, :, t + 1].isnan().all()
+        same[s, :, t + 1] = False
+        if fmt == "bf16":
+            assert torch.equal(got[s, :, t], base[s, :, t])
+            same[s, :, t] = False
+    assert torch.equal(got[same], fine[same])
 
 
 # ---- eviction
