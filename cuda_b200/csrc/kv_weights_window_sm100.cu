@@ -12,7 +12,7 @@
 // E4M3 codes are exact in f16 and bf16.  Block scales go into the keys (bf16 queries): bf16 holds code x 2^(block exponent - the
 // token's largest) exactly down to 2^-117 of the largest block; the largest exponent and other scales multiply S.
 // Measured (E4M3 keys with block scales, 32 queries x 4 heads against 52769 tokens of 8 heads of 128): 54 us, where the warp-level
-// kernel takes 76; 256 rows of 4 sequences of 8000-16384 tokens 66 us (387 TFLOP/s) against 360, 1024 rows against 2 of 5000-8192
+// kernel takes 76 (49 us back to back without a cold L2); 256 rows of 4 sequences of 8000-16384 tokens 66 us (387 TFLOP/s) against 360, 1024 rows against 2 of 5000-8192
 // 82 us against 434.  Bound by the loading warps' way through a tile (load latency, widening, and the issue of the MMAs, which
 // holds one of them up): about 7700 cycles a tile of 128 rows, of which the exponentials need 2048.  128 tokens a tile took 68 us, and
 // an issuing warp of its own as much: it leaves too few registers.
