@@ -7,8 +7,8 @@
 // One CTA of 256 threads takes 64 query rows (head-major: the rows of the heads that share a KV head) and walks the
 // states of its sequence; thread (ty, tx) of a 16 x 16 grid holds 4 rows x 4 states of S and 4 rows x D/16 columns of O.
 // Q, K and P sit transposed in shared memory, so that each step of a product reads two 16-byte fragments for 16 FMAs; a cluster
-// shares the states of a block of rows where blocks are few.  Bound by those shared-memory reads: 26 TFLOP/s of the 70 of the FMA
-// pipes (4 x 16 heads of 128, 512 positions, 1024 states: 655 us); 2 x 8 heads of 64, 129 positions, 300-577 states: 31 us.
+// shares the states of a block of rows where blocks are few.  Bound by those shared-memory reads: 28 TFLOP/s of the 70 of the FMA
+// pipes (4 x 16 heads of 128, 512 positions, 1024 states: 603 us); 2 x 8 heads of 64, 129 positions, 300-577 states: 23 us.
 #include "cross_attention.cuh"
 
 namespace b200 {
@@ -179,6 +179,32 @@ static cudaError_t launch_clusters(const void* kern, dim3 grid, int threads, siz
   return cudaLaunchKernelExC(&cfg, kern, args);
 }
 
+// Clusters of `parts` CTAs of the tile kernel that the current device runs at once.
+template <int D>
+static cudaError_t clusters_at_once(const void* kern, size_t smem, int parts, int* count) {
+  static int known[64][kMaxParts + 1] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && known[dev][parts]) {
+    *count = known[dev][parts];
+    return cudaSuccess;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(parts);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(count, kern, &cfg);
+  if (e == cudaSuccess && dev < 64) known[dev][parts] = *count;
+  return e;
+}
+
 template <int D>
 static cudaError_t go_tiles(const CrossArgs& a, cudaStream_t st) {
   constexpr size_t smem = (2 * D * (kSimtRows + 4) + kSimtKeys * D + kSimtKeys * (kSimtRows + 4)) * sizeof(float);
@@ -187,10 +213,24 @@ static cudaError_t go_tiles(const CrossArgs& a, cudaStream_t st) {
   cudaError_t e = allow_shared_memory((const void*)kern, (int)smem, configured);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.group * a.Sq, blocks = (rows + kSimtRows - 1) / kSimtRows;
-  // one wave of two CTAs per SM: a second one costs more than shorter parts save (48 blocks of 10 tiles: 8 parts 35 us)
-  const int tiles = (a.Skv + kSimtKeys - 1) / kSimtKeys;
-  int parts = cross_parts(blocks * a.Hkv * a.B, tiles);
-  if (parts > 1 && blocks * a.Hkv * a.B * parts > 2ll * current_sm_count()) parts /= 2;
+  // The split with the shortest run: waves of clusters times tiles of a part, and one more for its start and join.  How many
+  // clusters run at once depends on their size, as a cluster lies within one group of SMs (38 blocks of 63 tiles: 6 parts take 117 us,
+  // 7, which need a second wave, 150).  us here / with powers of two up to a wave of single CTAs: 48 blocks of 10 tiles 27 / 35
+  // (64 elements, 5 parts / 4), 62 / 68 (128 elements), 38 of 63 tiles 117 / 162, 512 blocks of 16 tiles 603 / 652 (128 elements, 2 / 1).
+  const long long tiles = (a.Skv + kSimtKeys - 1) / kSimtKeys, all = blocks * a.Hkv * a.B;
+  int parts = 1;
+  long long best = 0;
+  for (int p = 1; p <= kMaxParts && (p == 1 || p <= tiles); ++p) {
+    int at_once = 0;
+    e = clusters_at_once<D>((const void*)kern, smem, p, &at_once);
+    if (e != cudaSuccess) return e;
+    if (at_once < 1) continue;
+    const long long cost = (all + at_once - 1) / at_once * ((tiles + p - 1) / p + 1);
+    if (best == 0 || cost < best) {
+      best = cost;
+      parts = p;
+    }
+  }
   return launch_clusters((const void*)kern, dim3((unsigned)(blocks * parts), a.Hkv, a.B), 256, smem, parts, a, st);
 }
 

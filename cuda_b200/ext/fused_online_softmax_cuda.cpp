@@ -1,4 +1,5 @@
-// PyTorch extension `fused_online_softmax_cuda`: the decode path and the GQA prefill in front of it.
+// PyTorch extension `fused_online_softmax_cuda`: the decode path and the GQA prefill in front of it; attention to an encoder's
+// states and eviction from the paged cache by accumulated attention weight, which the reference does not have.
 //
 // Same module name, function names, argument names and defaults as the reference binding
 // (fused_softmax_binding.cpp in the reference project: paged_attention_forward :109-173 / m.def

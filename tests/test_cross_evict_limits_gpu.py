@@ -232,6 +232,30 @@ def test_keys_that_are_not_finite(fmt, hq, q_lens):
     assert torch.equal(got[same], fine[same])
 
 
+def test_all_kernels_at_once():
+    """Windows, decode weights, prompt attention and eviction on four streams, three times over: the results of one at a time."""
+    win = E.cache("w", lens=[3000, 1700], q_lens=[40, 33], hq=32, hkv=8, d=128, page=16, seed=1)
+    dec = E.cache("w", lens=[900] * 8, hq=8, hkv=2, d=64, page=16, fmt="bf16", seed=2)
+    evi = [E.cache("w", lens=[900, 1200], hq=8, hkv=2, d=64, page=16, seed=3) for _ in range(4)]
+    lse = [E.true_lse(x, True) for x in (win, dec)]
+    base = [torch.rand(x.num_seqs, x.num_kv_heads, x.block_tables.shape[1] * 16, device="cuda") for x in (win, dec, evi[0])]
+    cross = X.make(2, 8, 2, 300, 900, 64, torch.bfloat16, seed=4)
+    jobs = [lambda i: E.accumulate(win, lse[0], base[0].clone()), lambda i: E.accumulate(dec, lse[1], base[1].clone()),
+            lambda i: ops.cross_attention_forward(*cross), lambda i: E.evict(evi[i], base[2], 500, sink=1, recent=9)[0]]
+    want = [job(0) for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for i in range(1, 4):
+        got = []
+        for s, job in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(job(i))
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            assert torch.equal(w, g)
+        assert E.same(evi[i].key_cache, evi[0].key_cache) and E.same(evi[i].v_scale, evi[0].v_scale)
+
+
 # ---- eviction
 @pytest.mark.parametrize("fmt,d", [("mx4v", 64), ("mx4v", 128), ("fp8_token", 64), ("f32", 64), ("bf16", 128)])
 @pytest.mark.parametrize("page", [16, 64])
