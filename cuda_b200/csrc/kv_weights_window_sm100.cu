@@ -11,11 +11,12 @@
 //   warp 8            also allocates TMEM and issues the MMAs
 // E4M3 codes are exact in f16 and bf16.  Block scales go into the keys (bf16 queries): bf16 holds code x 2^(block exponent - the
 // token's largest) exactly down to 2^-117 of the largest block; the largest exponent and other scales multiply S.
-// Measured (E4M3 keys with block scales, 32 queries x 4 heads against 52769 tokens of 8 heads of 128): 54 us, where the warp-level
-// kernel takes 76 (49 us back to back without a cold L2); 256 rows of 4 sequences of 8000-16384 tokens 66 us (387 TFLOP/s) against 360, 1024 rows against 2 of 5000-8192
-// 82 us against 434.  Bound by the loading warps' way through a tile (load latency, widening, and the issue of the MMAs, which
-// holds one of them up): about 7700 cycles a tile of 128 rows, of which the exponentials need 2048.  128 tokens a tile took 68 us, and
-// an issuing warp of its own as much: it leaves too few registers.
+// Measured (events around single calls; E4M3 keys with block scales, 32 queries x 4 heads against 52769 tokens of 8 heads of 128):
+// 54 us, where the warp-level kernel takes 76; 256 rows of 4 sequences of 8000-16384 tokens 66 us (387 TFLOP/s) against 360, 1024
+// rows against 2 of 5000-8192 82 us against 434.  About 7700 cycles a tile of 128 rows, of which the exponentials need 2048; no
+// pipe is full (exponentials 29 %, tensor 16 %, issue 41 %), so it is latency that bounds it.
+// Slower: 128 tokens a tile (68 us), an issuing warp of its own (68, it leaves too few registers), MMAs issued by the weighing
+// warps (61).
 // The rows of a head stay in shared memory while its tokens pass, up to kWinBlocks blocks of 128; with more each tile loads
 // them again.  Rows that pad a block repeat the last row with a weight of zero, so that an infinity in K meets no zero.
 #include "kv_weights.cuh"
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) kv_weights_window_kernel(const
       if (a.status) atomicOr(a.status, CUDA_LLM_ST_BAD_BLOCK);
       return -1;
     };
-    auto fetch = [&]() {  // of tile `ahead`, whose page is known; then on to the page of the team's next
+    auto fetch = [&]() {  // of tile `ahead`, whose page is known; then on to the page of the next
       ahead_blk = blk_then;
       ahead_old = 0.f;
       if (ahead_blk >= 0) {
