@@ -4,7 +4,8 @@
 // Measured, both kernels: 32 sequences x 8 heads of 2500-8000 tokens of 128 E4M3 values, in place down to 2048: 20 + 103 us; one
 // sequence x 8 heads of 131072 bf16 tokens, 16384 of them into other pages: 28 + 109 us; one of 700 tokens down to 512: 18 us.
 // A kept token is one element of every row, so DRAM moves whole slabs: 0.48 and 0.54 GB here (4.6 and 5.0 TB/s), where the
-// kept tokens alone are 0.27 and 0.13 GB.
+// kept tokens alone are 0.27 and 0.13 GB.  In place, few long rows are slow: two sequences of 4 heads, the longer cut from 51333 to
+// 33301 tokens, take 566 us, since the 17 runs of a head follow one another.
 #include <type_traits>
 
 #include "host_common.cuh"
@@ -325,33 +326,36 @@ __device__ void plan_run(const MoveArgs& m, MovePlan<EB>& pl, const int32_t* kep
   __syncthreads();
 }
 
-// scales: a lane takes a token, 4 of them at a time (all loads before the stores: in place)
+// One row of the scales of K or of V: a lane takes 8 tokens at a time, and the next 8 are on their way while these are stored
+// (4 at a time, both tensors by one warp: 4 x 8 heads of 64, 9000 -> 4096 tokens in place, 114 us for 91).
+// In place that is safe: a token's old position is no lower than its new one, so what later tokens are loaded from lies
+// above what these are stored to; and these have all been loaded.
 template <typename E, int EB>
-__device__ __forceinline__ void move_scales(const EvictArgs& a, const MovePlan<EB>& pl, const MoveTensor& mt, int h, int n, int p0) {
+__device__ __forceinline__ void move_scale_row(const EvictArgs& a, const MovePlan<EB>& pl, const MoveTensor& mt, int r, int h, int n, int p0) {
+  constexpr int U = 8, STEP = 32 * U;
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.page);
-  E* const p = reinterpret_cast<E*>(mt.p);
-  for (int j0 = 0; j0 < n; j0 += 128) {
-    long long from[4], to[4];
+  E* const p = reinterpret_cast<E*>(mt.p) + r * a.page;
+  auto there = [&](int j) { return j < n && (pl.there[j >> 5] >> (j & 31) & 1); };
+  auto load = [&](int j0, E (&v)[U]) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < U; ++x) {
       const int j = j0 + x * 32 + lane;
-      from[x] = -1;
-      to[x] = 0;
-      if (j < n && (pl.there[j >> 5] >> (j & 31) & 1)) {
-        from[x] = ((long long)pl.page_blk[pl.page[j]] * a.Hkv + h) * mt.rows * a.page + (pl.tok[j] & 255);
-        to[x] = ((long long)pl.to[j >> shift] * a.Hkv + h) * mt.rows * a.page + ((p0 + j) & (a.page - 1));
-      }
+      v[x] = 0;
+      if (there(j)) v[x] = p[((long long)pl.page_blk[pl.page[j]] * a.Hkv + h) * mt.rows * a.page + (pl.tok[j] & 255)];
     }
-    for (int r = 0; r < mt.rows; ++r) {
-      E v[4];
+  };
+  E v[U], next[U];
+  load(0, v);
+  for (int j0 = 0; j0 < n; j0 += STEP) {
+    load(j0 + STEP, next);
+    __syncwarp();
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] = from[x] >= 0 ? p[from[x] + r * a.page] : (E)0;
-      __syncwarp();
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (from[x] >= 0) p[to[x] + r * a.page] = v[x];
-      __syncwarp();
+    for (int x = 0; x < U; ++x) {
+      const int j = j0 + x * 32 + lane;
+      if (there(j)) p[((long long)pl.to[j >> shift] * a.Hkv + h) * mt.rows * a.page + ((p0 + j) & (a.page - 1))] = v[x];
+      v[x] = next[x];
     }
+    __syncwarp();
   }
 }
 
@@ -464,9 +468,10 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __gri
         __syncwarp();
       }
     } else if (warp == kMoveWarps + kMoveLoaders) {
-      if (part == 0) {
-        if (m.sc[0].rows) move_scales<ES>(a, pl, m.sc[0], h, n, p0);
-        if (m.sc[1].rows) move_scales<ES>(a, pl, m.sc[1], h, n, p0);
+      // the rows of the scales go round the CTAs of the head
+      for (int r = part; r < m.sc[0].rows + m.sc[1].rows; r += m.split) {
+        const bool of_v = r >= m.sc[0].rows;
+        move_scale_row<ES>(a, pl, m.sc[of_v ? 1 : 0], of_v ? r - m.sc[0].rows : r, h, n, p0);
       }
     } else {
       // a team's warps share the rows, K and V alike; a lane owns one word of one or two rows of each
