@@ -6,8 +6,11 @@
 
 using namespace b200;
 
+// The 16-bit kernels read their inputs through tensor maps, whose boxes step over positions: a map can hold one batch row or head for
+// all (a dimension of one element), but not one position for all.
 static bool take_strides(const int64_t* st, int B, int H, int S, int D, int eb, bool output, long long* out) {
   const int extent[3] = {B, H, S};
+  if (eb == 2 && !output && S > 1 && st[2] == 0) return false;
   for (int i = 0; i < 3; ++i) {
     out[i] = extent[i] == 1 ? D : st[i];  // never multiplied by anything but 0
     if (out[i] < 0 || (out[i] * eb) % 16 || out[i] > (1ll << 36)) return false;
@@ -43,7 +46,7 @@ extern "C" int cuda_llm_cross_attention(const CudaLlmCrossAttentionParams* p, vo
   const int D = p->head_dim;
   if (!take_strides(p->q_strides, a.B, a.Hq, a.Sq, D, eb, false, a.q_st) || !take_strides(p->k_strides, a.B, a.Hkv, a.Skv, D, eb, false, a.k_st) ||
       !take_strides(p->v_strides, a.B, a.Hkv, a.Skv, D, eb, false, a.v_st) || !take_strides(p->out_strides, a.B, a.Hq, a.Sq, D, eb, true, a.o_st))
-    return refuse(CUDA_LLM_EALIGN, "strides must be multiples of 16 bytes, not negative, and no less than head_dim for out");
+    return refuse(CUDA_LLM_EALIGN, "strides must be multiples of 16 bytes, not negative, no less than head_dim for out, and not 0 for the positions of a 16-bit input");
   int rc = check_current_device();
   if (rc != CUDA_LLM_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

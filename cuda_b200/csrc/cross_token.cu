@@ -266,15 +266,14 @@ __global__ void __launch_bounds__(kTokThreads) cross_token_kernel(const __grid_c
 }
 
 // Tensor map of states [B, H, S, D] by their strides: boxes of 64 head_dim elements x `box_rows` positions, 128-byte
-// swizzle.  A stride of 0 is a dimension of one element (`hmul`, `bmul` 0).
+// swizzle.  A stride of 0 is a dimension of one element (`hmul`, `bmul` 0); positions have none (refused by the entry).
 bool encode_cross_map(CUtensorMap* map, const void* p, const long long* st, int B, int H, int S, int D, int box_rows, int* hmul, int* bmul) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (!enc) return false;
   *hmul = H > 1 && st[1] == 0 ? 0 : 1;
   *bmul = B > 1 && st[0] == 0 ? 0 : 1;
-  const long long row = S > 1 && st[2] ? st[2] : D;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)(*hmul ? H : 1), (cuuint64_t)(*bmul ? B : 1)};
-  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(st[1] ? st[1] : D) * 2, (cuuint64_t)(st[0] ? st[0] : D) * 2};
+  const cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)(st[1] ? st[1] : D) * 2, (cuuint64_t)(st[0] ? st[0] : D) * 2};
   const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

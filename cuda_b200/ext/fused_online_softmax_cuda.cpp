@@ -276,11 +276,12 @@ pybind11::object fp8_paged_attention_forward(torch::Tensor query, torch::Tensor 
 // ---- attention to an encoder's states, eviction by accumulated attention weight (no counterpart in the reference) ----
 namespace {
 
-// `t` if the kernels can address it as it lies (contiguous head_dim, 16-byte steps), else a copy
+// `t` if the kernels can address it as it lies (contiguous head_dim, 16-byte steps, in 16 bits no stride of 0 over positions), else a copy
 torch::Tensor addressable(const torch::Tensor& t) {
   const int64_t step = 16 / (int64_t)t.element_size();
   bool fine = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
   for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) % step == 0));
+  fine = fine && (t.scalar_type() == at::kFloat || t.size(2) <= 1 || t.stride(2) > 0);
   return fine ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 

@@ -458,10 +458,12 @@ def kv_cache_append(k_new, v_new, slot_block, slot_offset, key_cache, value_cach
 
 
 def _addressable(t: torch.Tensor) -> torch.Tensor:
-    """``t`` if the kernels can address it as it lies (contiguous head_dim, 16-byte steps), else a copy."""
+    """``t`` if the kernels can address it as it lies (contiguous head_dim, 16-byte steps, in 16 bits no stride of 0 over positions),
+    else a copy."""
     step = 16 // t.element_size()
     fine = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
         n == 1 or (st >= 0 and st % step == 0) for n, st in zip(t.shape[:-1], t.stride()[:-1]))
+    fine = fine and (t.dtype == torch.float32 or t.shape[2] <= 1 or t.stride(2) > 0)
     return t if fine else t.clone(memory_format=torch.contiguous_format)
 
 

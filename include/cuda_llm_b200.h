@@ -335,8 +335,8 @@ int cuda_llm_mx_attention_tcgen05_launches(uint64_t* launches);
  * result (it may hold infinities and NaN).  A row all of whose scores are -inf gives zeros, too; one with a score of
  * NaN or +inf gives NaN.  Tensors are addressed by three strides each (batch, head, position, in elements; head_dim is
  * contiguous): [B, H, S, D] and [B, S, H, D] need no copy, a stride of 0 shares states between batch rows
- * (beams) or heads.  A dimension of one element may carry any stride.  `out` overlaps no input.  No workspace; any
- * number of calls may be in flight, on any streams.
+ * (beams) or heads; over the positions of 16-bit inputs it is refused.  A dimension of one element may carry any
+ * stride.  `out` overlaps no input.  No workspace; any number of calls may be in flight, on any streams.
  *   16-bit types: few query rows per KV head stream the states once, split over a thread-block cluster and joined
  *   through its shared memory; more rows run on tcgen05.mma.  fp32: a plain fp32 kernel. */
 typedef struct CudaLlmCrossAttentionParams {

@@ -1,0 +1,45 @@
+"""Cross attention and eviction on layouts beside the usual ones.  Formulas and tolerances are those of ``test_cross_attention_gpu``
+and ``test_cache_eviction_gpu``."""
+import importlib
+import sys
+
+import pytest
+import torch
+
+import test_cross_attention_gpu as X
+from cuda_b200 import compat, ops
+
+pytestmark = pytest.mark.gpu
+DTYPES = ["bf16", "f16", "f32"]
+
+
+@pytest.fixture(scope="module")
+def ext():
+    sys.path.insert(0, compat.PATH)
+    try:
+        return importlib.import_module("fused_online_softmax_cuda")
+    finally:
+        sys.path.remove(compat.PATH)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sq", [1, 20, 90])
+@pytest.mark.parametrize("which", ["q", "k", "v", "qkv", "kv, all heads and rows too"])
+def test_one_position_for_all(ext, which, sq, dtype):
+    """Tensors expanded over their positions (a stride of 0) count as their contiguous copies."""
+    dt, d, n = X.DTYPES[dtype], 64, 150
+    q, k, v = X.make(2, 6, 3, sq, n, d, dt, seed=sq)
+    if "q" in which:
+        q = q[:, :, :1].expand(2, 6, sq, d)
+    if "k" in which:
+        k = k[:, :, -1:].expand(2, 3, n, d)
+    if "v" in which:
+        v = v[:, :, -1:].expand(2, 3, n, d)
+    if "heads" in which:
+        k, v = (x[1:, 2:, -1:].expand(2, 3, n, d) for x in (k, v))
+    lens = torch.tensor([n, 77], dtype=torch.int32, device="cuda")
+    want = ops.cross_attention_forward(q.contiguous(), k.contiguous(), v.contiguous(), lens, return_lse=True)
+    X.check(*want, *X.formula(q, k, v, lens.tolist(), 0.125), dt, d, n)
+    for m in (ops, ext):
+        got = m.cross_attention_forward(q, k, v, lens, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
