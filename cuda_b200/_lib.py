@@ -64,6 +64,7 @@ class KvWeightsParams(C.Structure):
         ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_blocks_per_seq", C.c_int32), ("num_blocks", C.c_int32),
         ("max_tokens", C.c_int32), ("max_q_len", C.c_int32), ("q_dtype", C.c_int32), ("k_format", C.c_int32),
         ("scale_mode", C.c_int32), ("is_causal", C.c_int32), ("softmax_scale", C.c_float), ("decay", C.c_float),
+        ("keep_old", C.c_int32),
     ]
 
 

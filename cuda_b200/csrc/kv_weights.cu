@@ -371,7 +371,7 @@ kv_weights_kernel(const __grid_constant__ WeightsArgs a, const __grid_constant__
           if (a.status && lane == 0) atomicOr(a.status, CUDA_LLM_ST_BAD_QLEN);
           q0 = n_q = 0;
         }
-        no_old = (t < 2 && a.decay != 0.f) ? ctx - n_q : 0;  // scores from here on start at zero
+        no_old = (t < 2 && a.decay != 0.f) ? ctx - (a.keep_old ? 0 : n_q) : 0;  // scores from here on start at zero
       }
       hgi = (w - pl.pre[s]) / per;
       u = w - pl.pre[s] - hgi * per;
@@ -756,7 +756,7 @@ extern "C" int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* p, v
   a.S = p->num_seqs; a.total_q = p->total_q; a.Hq = p->num_q_heads; a.Hkv = p->num_kv_heads; a.group = a.Hq / a.Hkv;
   a.D = p->head_dim; a.page = p->page_size; a.max_blocks = p->max_blocks_per_seq; a.num_blocks = p->num_blocks;
   a.max_tokens = p->max_tokens; a.q_dtype = p->q_dtype; a.k_format = p->k_format; a.scale_mode = p->scale_mode;
-  a.causal = p->is_causal ? 1 : 0; a.scale_log2 = p->softmax_scale * 1.4426950408889634f; a.decay = p->decay;
+  a.causal = p->is_causal ? 1 : 0; a.keep_old = p->keep_old ? 1 : 0; a.scale_log2 = p->softmax_scale * 1.4426950408889634f; a.decay = p->decay;
   a.q_first = 0;
   return cuda_result(launch_kv_weights(a, p->max_q_len, current_sm_count(), reinterpret_cast<cudaStream_t>(stream)), "kv_weights_kernel launch");
 }

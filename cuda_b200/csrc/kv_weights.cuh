@@ -14,7 +14,7 @@ struct WeightsArgs {
   float* scores;
   uint32_t* status;
   long long st_seq, st_head;
-  int S, total_q, Hq, Hkv, group, D, page, max_blocks, num_blocks, max_tokens, q_dtype, k_format, scale_mode, causal;
+  int S, total_q, Hq, Hkv, group, D, page, max_blocks, num_blocks, max_tokens, q_dtype, k_format, scale_mode, causal, keep_old;
   int group_shift;  // log2(group), or -1
   int q_first;  // query row of the first sequence when there are no offsets
   float scale_log2, decay;

@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kWinThreads, 1) kv_weights_window_kernel(const
       if (ahead_blk >= 0) {
         const int tok = ahead.u * kWinTokens + tid;
         const size_t slab = (size_t)ahead_blk * a.Hkv + ahead.h;
-        if (a.decay != 0.f && tok < ahead.ctx - ahead.n_q) ahead_old = a.scores[ahead.s * a.st_seq + ahead.h * a.st_head + tok];
+        if (a.decay != 0.f && (a.keep_old || tok < ahead.ctx - ahead.n_q)) ahead_old = a.scores[ahead.s * a.st_seq + ahead.h * a.st_head + tok];
         if (MX) {
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) ahead_e[i] = __ldg(a.ks + (slab * (D / 32) + i) * a.page + (tok & (a.page - 1)));

@@ -386,7 +386,7 @@ pybind11::object cross_attention_forward(torch::Tensor q, torch::Tensor k, torch
 torch::Tensor kv_cache_accumulate_weights(torch::Tensor query, torch::Tensor key_cache, c10::optional<torch::Tensor> k_scale,
                                           torch::Tensor block_tables, torch::Tensor context_lens, torch::Tensor lse, torch::Tensor scores,
                                           c10::optional<double> softmax_scale_opt, c10::optional<torch::Tensor> cu_q_lens, int64_t max_q_len,
-                                          bool is_causal, double decay, c10::optional<std::string> kv_format,
+                                          bool is_causal, double decay, bool keep_old, c10::optional<std::string> kv_format,
                                           c10::optional<torch::Tensor> status) {
   TORCH_CHECK(query.is_cuda() && key_cache.is_cuda(), "Inputs must be on CUDA");
   TORCH_CHECK(query.dim() == 3, "Query must be 3D [num_seqs, num_heads, head_dim]");
@@ -451,6 +451,7 @@ torch::Tensor kv_cache_accumulate_weights(torch::Tensor query, torch::Tensor key
   p.is_causal = is_causal;
   p.softmax_scale = scale_or_default(softmax_scale_opt, (int)d);
   p.decay = (float)decay;
+  p.keep_old = keep_old;
   check_rc(cuda_llm_kv_accumulate_weights(&p, at::cuda::getCurrentCUDAStream()), "cuda_llm_kv_accumulate_weights");
   return scores;
 }
@@ -561,8 +562,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("query"), pybind11::arg("key_cache"), pybind11::arg("k_scale"), pybind11::arg("block_tables"),
         pybind11::arg("context_lens"), pybind11::arg("lse"), pybind11::arg("scores"), pybind11::arg("softmax_scale") = pybind11::none(),
         pybind11::kw_only(), pybind11::arg("cu_q_lens") = pybind11::none(), pybind11::arg("max_q_len") = 1,
-        pybind11::arg("is_causal") = true, pybind11::arg("decay") = 1.0, pybind11::arg("kv_format") = pybind11::none(),
-        pybind11::arg("status") = pybind11::none());
+        pybind11::arg("is_causal") = true, pybind11::arg("decay") = 1.0, pybind11::arg("keep_old") = false,
+        pybind11::arg("kv_format") = pybind11::none(), pybind11::arg("status") = pybind11::none());
   m.def("kv_cache_evict", &kv_cache_evict, "Eviction from a paged KV cache by accumulated attention weight",
         pybind11::arg("scores"), pybind11::arg("key_cache"), pybind11::arg("value_cache"), pybind11::arg("k_scale"),
         pybind11::arg("v_scale"), pybind11::arg("block_tables"), pybind11::arg("context_lens"), pybind11::arg("budget"),

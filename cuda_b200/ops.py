@@ -533,13 +533,14 @@ def _check_scores(name, t, device, num_seqs, hkv):
 
 def kv_cache_accumulate_weights(query, key_cache, k_scale, block_tables, context_lens, lse, scores, softmax_scale=None, *,
                                 cu_q_lens: Optional[torch.Tensor] = None, max_q_len: int = 1, is_causal: bool = True,
-                                decay: float = 1.0, kv_format: Optional[str] = None, status: Optional[torch.Tensor] = None):
+                                decay: float = 1.0, keep_old: bool = False, kv_format: Optional[str] = None,
+                                status: Optional[torch.Tensor] = None):
     """Add to ``scores`` (fp32 ``[num_seqs, Hkv, tokens]``, in place, returned) the attention weight that ``query`` ``[total_q,
     Hq, D]`` spends on every cached token: ``decay * old + sum exp(scale * q . k_t - lse)`` over the queries that see the
     token and the heads that share its KV head.  ``lse`` ``[total_q, Hq]`` is what the decode of the same queries returned
-    (``return_lse=True``).  The tokens the queries brought themselves (the last q_len) start from 0; ``decay=0`` reads no old
-    score.  ``is_causal=False``: every query sees every token (encoder states in a paged cache).  ``key_cache`` and
-    ``k_scale`` as in ``fp8_paged_attention_forward``, or a 16-bit cache of the query's type with ``k_scale=None``.
+    (``return_lse=True``).  The tokens the queries brought themselves (the last q_len) start from 0; ``keep_old``: they brought
+    none, old scores count everywhere; ``decay=0`` reads no old score.  ``is_causal=False``: every query sees every token.  For an
+    encoder's states in a paged cache give ``is_causal=False, keep_old=True``.  ``key_cache`` and ``k_scale`` as in ``fp8_paged_attention_forward``, or a 16-bit cache of the query's type with ``k_scale=None``.
     ``status``: int32 tensor into which run-time findings (``ST_*`` bits) are OR-ed.  No counterpart in the reference."""
     if not (query.is_cuda and key_cache.is_cuda):
         raise RuntimeError("Inputs must be on CUDA")
@@ -594,7 +595,7 @@ def kv_cache_accumulate_weights(query, key_cache, k_scale, block_tables, context
             status=_ptr(status), score_strides=scores.stride()[:2], num_seqs=num_seqs, total_q=total_q, num_q_heads=hq,
             num_kv_heads=hkv, head_dim=d, page_size=page, max_blocks_per_seq=block_tables.shape[1], num_blocks=nb,
             max_tokens=scores.shape[2], max_q_len=max_q_len, q_dtype=_DTYPE[query.dtype], k_format=k_format, scale_mode=mode,
-            is_causal=1 if is_causal else 0, softmax_scale=scale, decay=decay)
+            is_causal=1 if is_causal else 0, softmax_scale=scale, decay=decay, keep_old=1 if keep_old else 0)
         L.check(lib.cuda_llm_kv_accumulate_weights(C.byref(p), _stream_ptr(dev)), "cuda_llm_kv_accumulate_weights")
     return scores
 

@@ -374,8 +374,9 @@ int cuda_llm_cross_attention_wait_timeouts(uint32_t* count);
  * what the decode of the same queries returned (a row of -inf saw nothing and adds nothing).  Which query sees which
  * token: is_causal, token t < context_len - q_len + 1 + j for query token j, as in the decode; otherwise every query sees
  * every token below the context length.  `old` is 0 for the tokens that the queries brought themselves, t >=
- * context_len - q_len, so that a token's score needs no clearing when it is appended; decay 0 reads no old score
- * at all.  Scores at t >= context_len are neither read nor written.  Reads K once and no V; no atomics: the same inputs
+ * context_len - q_len, so that a token's score needs no clearing when it is appended.  keep_old says that they brought
+ * none (an encoder's states in a paged cache): the old scores of all tokens count.  decay 0 reads no old score at all.
+ * Scores at t >= context_len are neither read nor written.  Reads K once and no V; no atomics: the same inputs
  * give the same bits.  A context longer than the block table or the score row is cut to it (CUDA_LLM_ST_BAD_CTX), a
  * block index outside the pool leaves its tokens' scores alone (CUDA_LLM_ST_BAD_BLOCK), query offsets that decrease
  * or leave [0, total_q] count as no queries (CUDA_LLM_ST_BAD_QLEN). */
@@ -406,6 +407,7 @@ typedef struct CudaLlmKvWeightsParams {
   int32_t is_causal;
   float softmax_scale;
   float decay;                 /* 0 to 1                                                        */
+  int32_t keep_old;            /* 0: the last q_len tokens of a context are new                 */
 } CudaLlmKvWeightsParams;
 
 int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* params, void* stream);

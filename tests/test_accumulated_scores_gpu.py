@@ -1,0 +1,81 @@
+"""Accumulated weights where the queries brought none of the tokens (``keep_old``: an encoder's states in a paged cache).  The formula and
+its tolerance are those of ``test_cache_eviction_gpu``; an old score adds one rounding of its product and of the sum, 2^-23 of it."""
+import importlib
+import math
+import sys
+
+import pytest
+import torch
+
+import test_cache_eviction_gpu as E
+from cuda_b200 import compat, ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ext():
+    sys.path.insert(0, compat.PATH)
+    try:
+        return importlib.import_module("fused_online_softmax_cuda")
+    finally:
+        sys.path.remove(compat.PATH)
+
+
+def expect(wl, lse, scores, causal, decay):
+    got, tol = E.weights_formula(wl, lse, torch.zeros_like(scores), causal, 0.0)
+    old = scores.double() * decay if decay else torch.zeros_like(scores, dtype=torch.float64)
+    live = torch.arange(scores.shape[2], device="cuda").view(1, 1, -1) < wl.context_lens.view(-1, 1, 1)
+    return torch.where(live, old + got, scores.double()), tol + 2.0 ** -23 * (old.abs() + got)
+
+
+def check(wl, causal, decay):
+    lse = E.true_lse(wl, causal)
+    scores = torch.rand(wl.num_seqs, wl.num_kv_heads, wl.block_tables.shape[1] * wl.page_size, device="cuda")
+    want, tol = expect(wl, lse, scores, causal, decay)
+    if decay == 0:
+        scores.fill_(math.nan)  # not read
+    E.accumulate(wl, lse, scores, is_causal=causal, decay=decay, keep_old=True)
+    for s in range(wl.num_seqs):
+        n = int(wl.context_lens[s])
+        assert ((scores[s, :, :n].double() - want[s, :, :n]).abs() <= tol[s, :, :n]).all(), s
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("decay", [1.0, 0.75, 0.0])
+@pytest.mark.parametrize("q_lens", [None, [1, 3, 4, 2, 1], [40, 33, 1, 90, 64]])
+@pytest.mark.parametrize("fmt", ["fp8_token", "mx8", "bf16"])
+def test_old_scores_count_everywhere(fmt, q_lens, decay, causal):
+    check(E.cache("w", lens=[333, 40, 1, 129, 2900], q_lens=q_lens, hq=8, hkv=2, d=128, page=16, fmt=fmt, seed=7), causal, decay)
+
+
+@pytest.mark.parametrize("q_len,page", [(1, 16), (8, 32), (40, 64), (90, 16)])  # one and two blocks of rows, the window kernel (90)
+def test_two_calls_add_up(q_len, page):
+    """Every state holds the weight of both steps, the last ones too; an equal second step doubles all scores."""
+    wl = E.cache("w", lens=[700, 5, 1500], q_lens=[q_len] * 3 if q_len <= 5 else [q_len, 5, q_len], hq=8, hkv=4, d=64, page=page, fmt="bf16", seed=q_len)
+    scores = torch.zeros(3, 4, wl.block_tables.shape[1] * page, device="cuda")
+    lse = E.true_lse(wl, False)
+    E.accumulate(wl, lse, scores, is_causal=False, keep_old=True)
+    first = scores.clone()
+    E.accumulate(wl, lse, scores, is_causal=False, keep_old=True)
+    assert torch.equal(scores, 2 * first)  # exact: doubling rounds nothing
+    wl.query = torch.randn_like(wl.query)
+    lse = E.true_lse(wl, False)
+    want, tol = expect(wl, lse, scores, False, 1.0)
+    E.accumulate(wl, lse, scores, is_causal=False, keep_old=True)
+    for s, n in enumerate(wl.context_lens.tolist()):
+        assert ((scores[s, :, :n].double() - want[s, :, :n]).abs() <= tol[s, :, :n]).all()
+
+
+def test_both_python_layers(ext):
+    wl = E.cache("w", lens=[70, 301], q_lens=[3, 2], hq=8, hkv=2, d=64, page=16, seed=3)
+    lse = E.true_lse(wl, False)
+    base = torch.rand(2, 2, wl.block_tables.shape[1] * 16, device="cuda")
+    for keep in (False, True):
+        got = [m.kv_cache_accumulate_weights(wl.query, wl.key_cache, wl.k_scale, wl.block_tables, wl.context_lens, lse, base.clone(), wl.softmax_scale,
+                                             cu_q_lens=wl.cu_q_lens, max_q_len=wl.max_q_len, is_causal=False, decay=0.5, keep_old=keep) for m in (ops, ext)]
+        assert torch.equal(*got)
+        if keep:
+            assert (got[0][0, :, 67:70] >= 0.5 * base[0, :, 67:70]).all()
+            assert torch.equal(got[0][0, :, :67], before[0, :, :67])
+        before = got[0]
