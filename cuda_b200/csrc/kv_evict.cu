@@ -672,12 +672,16 @@ extern "C" int cuda_llm_kv_evict(const CudaLlmKvEvictParams* p, void* stream) {
     return refuse(CUDA_LLM_EINVAL, "the same block table with another width");
   long long most = (long long)p->max_blocks_per_seq * p->page_size;
   if (most > p->max_tokens) most = p->max_tokens;
+  const long long readable = most;  // of a score row
   if (most > p->budget) most = p->budget;
   if (p->new_scores && !rows_apart(p->new_score_strides[0], p->num_seqs, p->new_score_strides[1], p->num_kv_heads, most))
     return refuse(CUDA_LLM_EINVAL, "new score rows overlap");
   if (p->new_scores == p->scores &&
       ((p->num_seqs > 1 && p->new_score_strides[0] != p->score_strides[0]) || (p->num_kv_heads > 1 && p->new_score_strides[1] != p->score_strides[1])))
     return refuse(CUDA_LLM_EINVAL, "new_scores is scores with other strides");
+  // a row is read to the end of its context while another may be written already
+  if (p->new_scores == p->scores && !rows_apart(p->score_strides[0], p->num_seqs, p->score_strides[1], p->num_kv_heads, readable))
+    return refuse(CUDA_LLM_EINVAL, "new_scores is scores and its rows overlap");
   if ((long long)p->new_max_blocks_per_seq * p->page_size < most) return refuse(CUDA_LLM_EINVAL, "new_block_tables is too narrow for the kept tokens");
   if (((uintptr_t)p->key_cache | (uintptr_t)p->value_cache | (scaled ? (uintptr_t)p->k_scale | (uintptr_t)p->v_scale : 0)) & 15)
     return refuse(CUDA_LLM_EALIGN, "caches and scales must be 16-byte aligned");

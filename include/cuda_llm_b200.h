@@ -421,9 +421,10 @@ int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* params, void* s
  *   length hold what they held.  The pages of a sequence must then be its own.
  *   another table: every sequence is copied, also one within its budget; its pages must not be pages that block_tables
  *   names, and the old ones are not written.
- * `new_scores`, if not NULL, receives the kept tokens' scores (it may be `scores` itself, with the same strides, and must not
- * overlap it otherwise; where tokens went, -0 comes back as +0 and NaN as one NaN).  Entries behind the new
- * length are not written, in the caches, the scales and new_scores alike.  Per-block scales are refused: tokens
+ * `new_scores`, if not NULL, receives the kept tokens' scores.  It may be `scores` itself, with the same strides, if whole rows
+ * (up to the table's or the row's end) are apart, and must not overlap it otherwise.  Where tokens went, -0 comes back as
+ * +0 and NaN as one NaN.  Entries behind the new length are not written, in the caches, the scales and new_scores
+ * alike.  Per-block scales are refused: tokens
  * of pages with different scales cannot share a page without being quantised again.  Lengths that pass the table or
  * the score row are cut (CUDA_LLM_ST_BAD_CTX); tokens whose old or new page index is outside the pool are not
  * moved (CUDA_LLM_ST_BAD_BLOCK). */
