@@ -74,10 +74,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cross_prompt_kernel(const _
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem + (tmem_slot - base));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = longest_first<kPromptThreads>(a.c, blockIdx.z, reinterpret_cast<volatile int*>(smem + 1020));
-  const int chunks = a.c.group / a.gsz;
-  const int kvh = blockIdx.y / chunks, head0 = kvh * a.c.group + (blockIdx.y - kvh * chunks) * a.gsz;
   const int BQ = kPromptRows / a.gsz;  // positions per CTA
-  const int q0 = blockIdx.x * BQ;
+  const int q_blocks = gridDim.x / (a.c.group / a.gsz), chunk = blockIdx.x / q_blocks;
+  const int kvh = blockIdx.y, head0 = kvh * a.c.group + chunk * a.gsz;
+  const int q0 = (blockIdx.x - chunk * q_blocks) * BQ;
   const int len = cross_kv_len(a.c, b);
   const int n_tiles = (len + kPromptKeys - 1) / kPromptKeys;
   // the second tile may hold no row at all (its heads' or positions' part starts behind the last)
@@ -354,7 +354,8 @@ static cudaError_t go(const CrossPromptArgs& a, cudaStream_t st) {
   cudaError_t e = allow_shared_memory((const void*)kern, (int)prompt_smem<D>(), configured);
   if (e != cudaSuccess) return e;
   const int bq = kPromptRows / a.gsz;
-  const dim3 grid((a.c.Sq + bq - 1) / bq, a.c.Hq / a.gsz, a.c.B);
+  // position blocks of a group's head chunks in x: the grid's y would end at 65535 query heads
+  const dim3 grid((a.c.Sq + bq - 1) / bq * (a.c.group / a.gsz), a.c.Hkv, a.c.B);
   kern<<<grid, kPromptThreads, prompt_smem<D>(), st>>>(a);
   return cudaGetLastError();
 }

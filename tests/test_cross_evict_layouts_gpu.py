@@ -43,3 +43,14 @@ def test_one_position_for_all(ext, which, sq, dtype):
     for m in (ops, ext):
         got = m.cross_attention_forward(q, k, v, lens, return_lse=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_more_heads_than_a_grid_is_high():
+    """30000 KV heads of three query heads, 33 rows each: the tensor-core kernel with one head per block."""
+    q, k, v = X.make(1, 90000, 30000, 11, 5, 64, torch.bfloat16, seed=2)
+    out, lse = ops.cross_attention_forward(q, k, v, return_lse=True)
+    for h in (0, 13000, 29000):
+        qh, kh, vh = q[:, 3 * h:3 * h + 3000], k[:, h:h + 1000], v[:, h:h + 1000]
+        part = ops.cross_attention_forward(qh, kh, vh, return_lse=True)
+        assert torch.equal(out[:, 3 * h:3 * h + 3000], part[0]) and torch.equal(lse[:, 3 * h:3 * h + 3000], part[1])
+        X.check(*part, *X.formula(qh, kh, vh, None, 0.125), torch.bfloat16, 64, 5)
