@@ -66,8 +66,10 @@ extern "C" int cuda_llm_cross_attention_wait_timeouts(uint32_t* count) {
   const int rc = check_current_device();
   if (rc != CUDA_LLM_OK) return rc;
   unsigned int token = 0, prompt = 0;
-  cudaError_t e = cross_wait_timeouts(&token);
+  // the copies below wait for the default stream alone, not for streams that run beside it
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cross_wait_timeouts(&token);
   if (e == cudaSuccess) e = cross_prompt_timeouts(&prompt);
   *count = token + prompt;
-  return cuda_result(e, "cudaMemcpyFromSymbol");
+  return cuda_result(e, "reading the counters");
 }

@@ -54,3 +54,18 @@ def test_more_heads_than_a_grid_is_high():
         part = ops.cross_attention_forward(qh, kh, vh, return_lse=True)
         assert torch.equal(out[:, 3 * h:3 * h + 3000], part[0]) and torch.equal(lse[:, 3 * h:3 * h + 3000], part[1])
         X.check(*part, *X.formula(qh, kh, vh, None, 0.125), torch.bfloat16, 64, 5)
+
+
+def test_count_of_timeouts_waits_for_side_streams():
+    """It has to count what runs on any stream, also on one that does not wait for the default stream."""
+    import ctypes
+    from cuda_b200 import _lib as L
+    side, n = torch.cuda.Stream(), ctypes.c_uint32(7)
+    buf = torch.empty(2, 2 ** 28, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(100):  # a third of a millisecond each
+            buf[0].copy_(buf[1])
+    assert not side.query()
+    assert L.load().cuda_llm_cross_attention_wait_timeouts(ctypes.byref(n)) == L.OK and n.value == 0
+    assert side.query()
