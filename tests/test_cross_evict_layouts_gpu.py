@@ -69,3 +69,16 @@ def test_count_of_timeouts_waits_for_side_streams():
     assert not side.query()
     assert L.load().cuda_llm_cross_attention_wait_timeouts(ctypes.byref(n)) == L.OK and n.value == 0
     assert side.query()
+
+
+def test_rows_of_a_batch_do_not_feel_one_another():
+    """The split over a cluster depends on the batch, so a row alone may differ in its last bits: each is within the tolerance of the formula."""
+    for sq in (1, 33, 200):
+        q, k, v = X.make(4, 8, 2, sq, 1777, 128, torch.bfloat16, seed=sq)
+        lens = torch.tensor([1777, 900, 64, 1300], dtype=torch.int32, device="cuda")
+        want = X.formula(q, k, v, lens.tolist(), 128 ** -0.5)
+        X.check(*ops.cross_attention_forward(q, k, v, lens, return_lse=True), *want, torch.bfloat16, 128, 1777)
+        for i in range(4):
+            row = slice(i, i + 1)
+            alone = ops.cross_attention_forward(q[row], k[row], v[row], lens[row], return_lse=True)
+            X.check(*alone, *(x[row] if torch.is_tensor(x) else x for x in want), torch.bfloat16, 128, 1777)
