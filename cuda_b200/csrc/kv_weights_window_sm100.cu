@@ -27,7 +27,8 @@ namespace b200 {
 
 constexpr int kWinThreads = 512, kWinTokens = 256, kWinRows = 128, kWinBlocks = 2, kWinTiles = 2;
 constexpr uint32_t kWinHeader = 9 * 1024;
-static_assert(192 + 4 * (2 * kWgtSeqs + 4) <= kWinHeader, "header");
+constexpr uint32_t kWinBlind = 192 + 4 * (2 * kWgtSeqs + 4);  // of every block and loading warp: one of its rows saw nothing
+static_assert(kWinBlind % 16 == 0 && kWinBlind + 16 * kWinBlocks <= kWinHeader, "header");
 
 __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {  // read once: past the L1 cache
   uint4 v;
@@ -207,15 +208,22 @@ __global__ void __launch_bounds__(kWinThreads, 1) kv_weights_window_kernel(const
       const int r = rb * kWinRows + ltid;
       float nl = -__builtin_huge_valf();  // no such row, or a row that saw nothing: weights of zero
       int limit = 0;
+      bool blind = false;
       if (ltid < kWinRows && r < at.rows) {
         const int j = query_of(r);
         const float v = a.lse[(size_t)(at.q0 + j) * a.Hq + at.h * a.group + (r - j * a.group)];
-        if (v != -__builtin_huge_valf()) nl = v * -1.4426950408889634f;
-        limit = a.causal ? at.ctx - at.n_q + 1 + j : at.ctx;
+        if (v != -__builtin_huge_valf()) {
+          nl = v * -1.4426950408889634f;
+          limit = a.causal ? at.ctx - at.n_q + 1 + j : at.ctx;
+        } else {
+          blind = true;  // its products may be NaN, and only the comparison with its limit keeps them out
+        }
       }
+      blind = __any_sync(0xffffffffu, blind);
       if (ltid < kWinRows) {
         reinterpret_cast<float*>(smem + row_at + qs * 1024)[ltid] = nl;
         reinterpret_cast<int*>(smem + row_at + qs * 1024 + 512)[ltid] = limit;
+        if (lane == 0) reinterpret_cast<int*>(smem + kWinBlind + qs * 16)[ltid >> 5] = blind;
       }
       fence_async_smem();
       __syncwarp();
@@ -407,12 +415,14 @@ __global__ void __launch_bounds__(kWinThreads, 1) kv_weights_window_kernel(const
         const float* nl = reinterpret_cast<const float*>(smem + row_at + qs * 1024);
         const int* limit = reinterpret_cast<const int*>(nl + kWinRows);
         const int cols = min(kWinRows, at.rows - rb * kWinRows);
+        const int4 blind = *reinterpret_cast<const int4*>(smem + kWinBlind + qs * 16);
+        const bool cut = edge || (blind.x | blind.y | blind.z | blind.w);
 #pragma unroll 1
         for (int c = 0; c < cols; c += 32) {
           uint32_t x[32];
           tmem_ld32(tmem + lanes + slot * 128 + c, x);
           tc_wait_ld();
-          if (edge || c + 32 > cols) {
+          if (cut || c + 32 > cols) {
 #pragma unroll
             for (int y = 0; y < 32; ++y) {
               const float p = fast_exp2(fmaf(__uint_as_float(x[y]), f, nl[c + y]));

@@ -371,9 +371,9 @@ int cuda_llm_cross_attention_wait_timeouts(uint32_t* count);
  * given queries spend on it:
  *   scores[s, h, t] = decay * old + sum exp(softmax_scale * q . k_t - lse[q])
  * over the query tokens of sequence s that see t and the num_q_heads / num_kv_heads heads that share KV head h.  `lse` is
- * what the decode of the same queries returned (a row of -inf saw nothing and adds nothing).  Which query sees which
- * token: is_causal, token t < context_len - q_len + 1 + j for query token j, as in the decode; otherwise every query sees
- * every token below the context length.  `old` is 0 for the tokens that the queries brought themselves, t >=
+ * what the decode of the same queries returned (a row of -inf saw nothing and adds nothing, whatever its query and the
+ * keys hold: the padding of a batch).  Which query sees which token: is_causal, token t < context_len - q_len + 1 + j
+ * for query token j, as in the decode; otherwise every query sees every token below the context length.  `old` is 0 for the tokens that the queries brought themselves, t >=
  * context_len - q_len, so that a token's score needs no clearing when it is appended.  keep_old says that they brought
  * none (an encoder's states in a paged cache): the old scores of all tokens count.  decay 0 reads no old score at all.
  * Scores at t >= context_len are neither read nor written.  Reads K once and no V; no atomics: the same inputs

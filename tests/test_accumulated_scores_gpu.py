@@ -79,3 +79,40 @@ def test_both_python_layers(ext):
             assert (got[0][0, :, 67:70] >= 0.5 * base[0, :, 67:70]).all()
             assert torch.equal(got[0][0, :, :67], before[0, :, :67])
         before = got[0]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_lens,declared", [(None, 1), ([1, 2, 4, 1], 4), ([8, 30, 5, 32], 32), ([8, 30, 5, 32], 1), ([60, 90, 40, 100], 100)])
+@pytest.mark.parametrize("fmt,q_dtype", [("fp8_token", torch.bfloat16), ("fp8_token", torch.float16), ("fp8_head", torch.float32), ("mx8", torch.bfloat16),
+                                         ("mx8", torch.float16), ("bf16", torch.bfloat16)])
+def test_rows_that_saw_nothing_add_nothing(fmt, q_dtype, q_lens, declared, causal):
+    """Rows with a log-sum-exp of -inf (the padding of a batch) count nothing, whatever their queries hold: the other rows' bits stay."""
+    wl = E.cache("w", lens=[130, 2900, 333, 1500], q_lens=q_lens, hq=8, hkv=2, d=64, page=16, fmt=fmt, q_dtype=q_dtype, seed=5)
+    wl.max_q_len = declared
+    lse = E.true_lse(wl, causal)
+    none = torch.rand(lse.shape, device="cuda") < 0.3
+    none[-1], none[0, :4] = True, True  # a last row, a whole group
+    lse[none] = -math.inf
+    base = torch.rand(4, 2, wl.block_tables.shape[1] * 16, device="cuda")
+    wl.query[none] = 0.0
+    want = E.accumulate(wl, lse, base.clone(), is_causal=causal)
+    for bad in (math.nan, math.inf, -math.inf):
+        wl.query[none] = bad
+        assert torch.equal(E.accumulate(wl, lse, base.clone(), is_causal=causal), want), bad
+
+
+@pytest.mark.parametrize("q_lens", [None, [2, 1], [30, 9], [90, 70]])
+@pytest.mark.parametrize("fmt", ["fp8_token", "mx8", "bf16"])
+def test_keys_that_only_rows_that_saw_nothing_meet(fmt, q_lens):
+    """Keys that are not finite where every row has a log-sum-exp of -inf: the old scores fade and nothing is added."""
+    wl = E.cache("w", lens=[2900, 333], q_lens=q_lens, hq=8, hkv=2, d=128, page=16, fmt=fmt, seed=9)
+    lse = torch.full((wl.query.shape[0], 8), -math.inf, device="cuda")
+    for t in (0, 17, 300):
+        page = wl.block_tables[:, t // 16].long()
+        wl.key_cache[page, :, 3, t % 16] = math.nan if fmt == "bf16" else 0x7f
+        if fmt == "bf16":
+            wl.key_cache[page, :, 5, (t + 1) % 16] = math.inf
+    base = torch.rand(2, 2, wl.block_tables.shape[1] * 16, device="cuda")
+    got = E.accumulate(wl, lse, base.clone(), is_causal=False, decay=0.5, keep_old=True)
+    for s, n in enumerate(wl.context_lens.tolist()):
+        assert torch.equal(got[s, :, :n], 0.5 * base[s, :, :n]) and torch.equal(got[s, :, n:], base[s, :, n:])
