@@ -116,3 +116,26 @@ def test_keys_that_only_rows_that_saw_nothing_meet(fmt, q_lens):
     got = E.accumulate(wl, lse, base.clone(), is_causal=False, decay=0.5, keep_old=True)
     for s, n in enumerate(wl.context_lens.tolist()):
         assert torch.equal(got[s, :, :n], 0.5 * base[s, :, :n]) and torch.equal(got[s, :, n:], base[s, :, n:])
+
+
+@pytest.mark.parametrize("fmt", ["fp8_token", "mx8", "bf16"])
+@pytest.mark.parametrize("group,n", [(4, 32), (1, 33), (5, 40)])
+def test_log_sum_exp_of_a_window_from_one_decode(group, n, fmt):
+    """The last n queries of two prompts in one decode: every 16 // group of them stand as a sequence of their own, with the same pages and
+    the context up to them.  Each row's weights then add up to 1 within the tolerance of the decode's log-sum-exp, 1e-3."""
+    wl = E.cache("w", lens=[700, 90], q_lens=[n, n], hq=2 * group, hkv=2, d=128, page=16, fmt=fmt, seed=n)
+    step = 16 // group
+    ends = [min(n, i + step) for i in range(0, n, step)]
+    lens = torch.tensor([c - n + e for c in wl.context_lens.tolist() for e in ends], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0] + [s * n + e for s in range(2) for e in ends], dtype=torch.int32, device="cuda")
+    tables = wl.block_tables.repeat_interleave(len(ends), 0).contiguous()
+    if fmt == "bf16":
+        _, lse = ops.paged_attention_forward(wl.query, wl.key_cache, wl.value_cache, tables, lens, wl.softmax_scale, cu_q_lens=cu, max_q_len=step,
+                                             return_lse=True)
+    else:
+        _, lse = ops.fp8_paged_attention_forward(wl.query, wl.key_cache, wl.value_cache, wl.k_scale, wl.v_scale, tables, lens, wl.softmax_scale,
+                                                 cu_q_lens=cu, max_q_len=step, return_lse=True)
+    assert ((lse - E.true_lse(wl, True)).abs() < 1e-3).all()
+    scores = E.accumulate(wl, lse, torch.zeros(2, 2, wl.block_tables.shape[1] * 16, device="cuda"))
+    for s, c in enumerate(wl.context_lens.tolist()):
+        assert ((scores[s, :, :c].sum(-1) - n * group).abs() < 1e-3 * n * group).all()
