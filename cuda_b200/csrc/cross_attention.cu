@@ -54,7 +54,7 @@ extern "C" int cuda_llm_cross_attention(const CudaLlmCrossAttentionParams* p, vo
   const long long rows = (long long)group * a.Sq, pairs = (long long)a.B * a.Hkv;
   if (a.dtype == CUDA_LLM_F32)
     return rows <= 16 ? cuda_result(launch_cross_stream(a, D, st), "cross_stream_kernel launch") : cuda_result(launch_cross_simt(a, D, st), "cross_simt_kernel launch");
-  // 16 bit, 16 x 8 pairs, 4096 states: 32 rows take 57 us streamed and 74 us on the tensor cores' 256-row blocks, 64 rows 96 and
+  // 16 bit, 16 x 8 pairs of 4 heads (groups that are no power of two were not timed), 4096 states: 32 rows take 57 us streamed and 74 us on the tensor cores' 256-row blocks, 64 rows 96 and
   // 74 us.  Those blocks walk all states in turn: where they leave SMs idle, 64 rows are streamed as well.
   if (rows <= 32 || (rows <= 64 && pairs < current_sm_count() / 2)) return cuda_result(launch_cross_token(a, D, st), "cross_token_kernel launch");
   return cuda_result(launch_cross_prompt(a, D, st), "cross_prompt_kernel launch");

@@ -7,7 +7,8 @@
 // One CTA of 256 threads takes 64 query rows (head-major: the rows of the heads that share a KV head) and walks the
 // states of its sequence; thread (ty, tx) of a 16 x 16 grid holds 4 rows x 4 states of S and 4 rows x D/16 columns of O.
 // Q, K and P sit transposed in shared memory, so that each step of a product reads two 16-byte fragments for 16 FMAs; a cluster
-// shares the states of a block of rows where blocks are few.  Bound by those shared-memory reads: 28 TFLOP/s of the 70 of the FMA
+// shares the states of a block of rows where blocks are few.  Bound by those shared-memory reads (of this tile: 8 x 8 scores a thread would
+// halve them and is not tried): 28 TFLOP/s of the 70 of the FMA
 // pipes (4 x 16 heads of 128, 512 positions, 1024 states: 603 us); 2 x 8 heads of 64, 129 positions, 300-577 states: 23 us.
 #include "cross_attention.cuh"
 

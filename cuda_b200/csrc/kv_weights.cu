@@ -3,11 +3,12 @@
 //   scores[s, h, t] = decay * old + sum over the rows r that see t of 2^(scale_log2 q_r . k_t - lse2_r)
 //
 // The log-sum-exp is known, so tokens are independent: one pass over K, no join, no atomics.  A decode step (up to 16 rows per
-// KV head) is bound by the bytes of K: 64 sequences of 1000-8192 tokens, 8 heads of 128, E4M3 with per-token scales, 65 us =
-// 5.0 TB/s (0.78 of the measured copy peak; what is missing is issue slots: 165 warp instructions per 16 tokens and head, counted
+// KV head) is bound by the bytes of K: 64 sequences of 1000-8192 tokens, 8 heads of 128, E4M3 with per-token scales, 64 us =
+// 5.1 TB/s (0.79 of the measured copy peak; what is missing is issue slots: 165 warp instructions per 16 tokens and head, counted
 // when it took 77 us).
 // Windows of a prompt with more rows go to kv_weights_window_kernel; those of up to 64 (or 128) rows stay here, bound by the latency
-// of warp-level products and exponentials (tensor pipe 35 % busy at 128 rows).
+// of warp-level products and exponentials (tensor pipe 35 % busy at 128 rows), and so do all with fp32 queries (three bf16 terms) or
+// with fp16 queries on block-scaled keys (f16 has no room for the block scale in the key): they pay 2.6 to 10 times.
 //
 // Arithmetic: K as E4M3 codes (widened exactly to f16) or as 16-bit elements, products on mma.m16n8k16 with fp32 sums, tokens on
 // the 16-wide side and query rows on the 8-wide side.  bf16 and fp32 queries against 8-bit codes are brought into f16's range by a
@@ -662,7 +663,8 @@ static cudaError_t launch_kv_weights(WeightsArgs a, int max_q_len, int sms, cuda
   const bool four = nt == 1 && a.q_dtype != CUDA_LLM_F32 && (eb == 1 || a.D == 64) && cap * a.Hkv * a.S / 16 >= 4ll * 4 * kWgtWarps * sms;
   // Many rows (16-bit queries): on tcgen05.  us here / there, E4M3 keys: 20 rows 162 / 219, 64 rows 68 / 68, 128 rows 76 / 54, 256
   // rows 360 / 66, 1024 rows 434 / 82; 16-bit keys: 64 rows 31 / 37, 128 rows 39 / 49.  8 heads of 1000 tokens, fewer tiles than
-  // SMs, 128 rows: 14.5 / 16.4.
+  // SMs, 128 rows: 14.5 / 16.4.  fp32 queries and fp16 queries on block scales have no form there (20001 and 32768 tokens x 8 heads, 128
+  // rows 374 and 137 us, 1024 rows 2650 and 1635, where bf16 queries take 53 and 255).
   const bool fills = cap * a.Hkv * a.S >= 256ll * sms;
   const bool window = (declared > kWgtRows || (declared > 64 && eb == 1 && fills)) && a.q_dtype != CUDA_LLM_F32 &&
                       !(a.q_dtype == CUDA_LLM_F16 && eb == 1 && a.scale_mode == CUDA_LLM_SCALE_MX_E8M0);

@@ -472,8 +472,8 @@ def cross_attention_forward(q, k, v, kv_lens=None, softmax_scale=None, *, return
     ``[B, Hkv, Skv, D]`` of one dtype -> ``[B, Hq, Sq, D]`` (GQA: kv_head = q_head // (Hq // Hkv)).  ``kv_lens`` (int32
     ``[B]``): how many states each sequence has; what lies behind them is not looked at.  A sequence without states
     gives zeros.  ``return_lse`` adds the natural log-sum-exp ``[B, Hq, Sq]`` (-inf without states).  Strided views
-    (``[B, S, H, D].transpose(1, 2)``, expanded batch rows) are read as they lie, and the output has q's layout.  No
-    counterpart in the reference, whose attention calls take one sequence length."""
+    (``[B, S, H, D].transpose(1, 2)``, expanded batch rows) are read as they lie, and the output has q's layout.  In 16 bits the
+    softmax weights are rounded to the type of the inputs before the second product.  No counterpart in the reference, whose attention calls take one sequence length."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError("Inputs must be on CUDA")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -538,7 +538,9 @@ def kv_cache_accumulate_weights(query, key_cache, k_scale, block_tables, context
     """Add to ``scores`` (fp32 ``[num_seqs, Hkv, tokens]``, in place, returned) the attention weight that ``query`` ``[total_q,
     Hq, D]`` spends on every cached token: ``decay * old + sum exp(scale * q . k_t - lse)`` over the queries that see the
     token and the heads that share its KV head.  ``lse`` ``[total_q, Hq]`` is what the decode of the same queries returned
-    (``return_lse=True``).  The tokens the queries brought themselves (the last q_len) start from 0; ``keep_old``: they brought
+    (``return_lse=True``); rows of -inf add nothing.  For more queries than one decode row block holds (16 per KV head) give the decode
+    every ``16 // group`` of them as a sequence of their own: same pages, the context up to the last of them.  Queries that the decode
+    rotates (``rope_cos``) are rotated by the caller here.  The tokens the queries brought themselves (the last q_len) start from 0; ``keep_old``: they brought
     none, old scores count everywhere; ``decay=0`` reads no old score.  ``is_causal=False``: every query sees every token.  For an
     encoder's states in a paged cache give ``is_causal=False, keep_old=True``.  ``key_cache`` and ``k_scale`` as in ``fp8_paged_attention_forward``, or a 16-bit cache of the query's type with ``k_scale=None``.
     ``status``: int32 tensor into which run-time findings (``ST_*`` bits) are OR-ed.  No counterpart in the reference."""
@@ -609,7 +611,8 @@ def kv_cache_evict(scores, key_cache, value_cache, k_scale, v_scale, block_table
     and scales, bit for bit.  Returns ``(kept, new_context_lens)``: int32 ``[num_seqs, Hkv, budget]`` with the old position of
     every kept token (-1 behind the new length) and int32 ``[num_seqs]``.  ``new_block_tables``: copy the kept tokens there and
     leave the old pages alone (pages shared with other sequences).  ``new_scores`` (it may be ``scores``) receives the kept
-    tokens' scores.  Caches as in ``fp8_paged_attention_forward`` / ``paged_attention_forward``; scales ``None`` for 16- and
+    tokens' scores.  Keys keep the rotation of their old positions: a decode with ``rope_cos`` needs ``rope_positions`` from then on (its
+    default counts from the shortened context).  For fp32 caches the scores are the caller's own.  Caches as in ``fp8_paged_attention_forward`` / ``paged_attention_forward``; scales ``None`` for 16- and
     32-bit caches; per-block scales are refused.  No counterpart in the reference."""
     if not (scores.is_cuda and key_cache.is_cuda and value_cache.is_cuda):
         raise RuntimeError("Inputs must be on CUDA")

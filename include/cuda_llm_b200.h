@@ -338,7 +338,9 @@ int cuda_llm_mx_attention_tcgen05_launches(uint64_t* launches);
  * (beams) or heads; over the positions of 16-bit inputs it is refused.  A dimension of one element may carry any
  * stride.  `out` overlaps no input.  No workspace; any number of calls may be in flight, on any streams.
  *   16-bit types: few query rows per KV head stream the states once, split over a thread-block cluster and joined
- *   through its shared memory; more rows run on tcgen05.mma.  fp32: a plain fp32 kernel. */
+ *   through its shared memory; more rows run on tcgen05.mma.  The softmax weights are rounded to the operand type before the
+ *   product with v (half a step of it, relative); scores, sums and the log-sum-exp stay in fp32.  fp32: fp32 throughout.
+ *   The same call gives the same bits; the split depends on the batch, so a row alone may differ in its last bits. */
 typedef struct CudaLlmCrossAttentionParams {
   const void* q;           /* [batch_size, num_q_heads, q_len, head_dim] of dtype              */
   const void* k;           /* [batch_size, num_kv_heads, kv_len, head_dim]                     */
@@ -372,7 +374,9 @@ int cuda_llm_cross_attention_wait_timeouts(uint32_t* count);
  *   scores[s, h, t] = decay * old + sum exp(softmax_scale * q . k_t - lse[q])
  * over the query tokens of sequence s that see t and the num_q_heads / num_kv_heads heads that share KV head h.  `lse` is
  * what the decode of the same queries returned (a row of -inf saw nothing and adds nothing, whatever its query and the
- * keys hold: the padding of a batch).  Which query sees which token: is_causal, token t < context_len - q_len + 1 + j
+ * keys hold: the padding of a batch).  A decode gives it for up to 16 rows per KV head; longer windows are cut into sequences of
+ * their own over the same pages, each with the context up to its last query.  Queries that the decode rotated itself
+ * (rope_cos) are given rotated here.  Which query sees which token: is_causal, token t < context_len - q_len + 1 + j
  * for query token j, as in the decode; otherwise every query sees every token below the context length.  `old` is 0 for the tokens that the queries brought themselves, t >=
  * context_len - q_len, so that a token's score needs no clearing when it is appended.  keep_old says that they brought
  * none (an encoder's states in a paged cache): the old scores of all tokens count.  decay 0 reads no old score at all.
@@ -424,7 +428,8 @@ int cuda_llm_kv_accumulate_weights(const CudaLlmKvWeightsParams* params, void* s
  * `new_scores`, if not NULL, receives the kept tokens' scores.  It may be `scores` itself, with the same strides, if whole rows
  * (up to the table's or the row's end) are apart, and must not overlap it otherwise.  Where tokens went, -0 comes back as
  * +0 and NaN as one NaN.  Entries behind the new length are not written, in the caches, the scales and new_scores
- * alike.  Per-block scales are refused: tokens
+ * alike.  Keys keep the rotation of their old positions, so a decode that rotates its queries itself needs rope_positions from
+ * then on: its default counts from the shortened context.  Per-block scales are refused: tokens
  * of pages with different scales cannot share a page without being quantised again.  Lengths that pass the table or
  * the score row are cut (CUDA_LLM_ST_BAD_CTX); tokens whose old or new page index is outside the pool are not
  * moved (CUDA_LLM_ST_BAD_BLOCK). */
